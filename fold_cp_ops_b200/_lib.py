@@ -1,4 +1,5 @@
-"""ctypes binding of ``libtrimul_sm100.so`` (C ABI declared in ``include/trimul_sm100.h``).
+"""ctypes binding of ``libtrimul_sm100.so`` (C ABI declared in ``include/trimul_sm100.h``
+and ``include/pair_stream_sm100.h``).
 
 There is exactly one compute path: the hand-written sm_100a kernels in that library.  If the
 library is missing or the device is not compute capability 10.x the functions here raise; nothing
@@ -49,6 +50,16 @@ EXPORTED_SYMBOLS = (
     "trimul_sm100_peer_wait",
 )
 
+#: every symbol include/pair_stream_sm100.h declares
+PAIR_SYMBOLS = (
+    "pair_sm100_add_norm",
+    "pair_sm100_add_norm_grad_workspace",
+    "pair_sm100_add_norm_grad",
+    "pair_sm100_embed",
+    "pair_sm100_embed_grad_workspace",
+    "pair_sm100_embed_grad",
+)
+
 
 class Caps(C.Structure):
     _fields_ = [("cc_major", C.c_int32), ("cc_minor", C.c_int32), ("num_sms", C.c_int32),
@@ -95,6 +106,30 @@ class ReshardPlan(C.Structure):
                 ("chan_offset", C.c_int32), ("pad", C.c_int32), ("rows", C.c_int64)]
 
 
+PAIR_BF16, PAIR_FP16, PAIR_FP32 = 0, 1, 2
+PAIR_SHARED_NONE, PAIR_SHARED_ROWS, PAIR_SHARED_COLUMNS = 0, 1, 2
+PAIR_MAX_WIDTH = 8192
+
+
+class PairDropoutDesc(C.Structure):
+    _fields_ = [("seed", C.c_uint64), ("offset", C.c_uint32), ("keep", C.c_uint32), ("device_seed", C.c_void_p),
+                ("shared", C.c_int32), ("origin_b", C.c_int32), ("origin_i", C.c_int32), ("origin_j", C.c_int32)]
+
+
+class PairTensor(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_i", C.c_int64), ("stride_j", C.c_int64)]
+
+
+class PairNormDesc(C.Structure):
+    _fields_ = [("b", C.c_int32), ("i", C.c_int32), ("j", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("group", C.c_int32), ("eps", C.c_float), ("dropout", PairDropoutDesc)]
+
+
+class PairEmbedDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("d", C.c_int32), ("rows", C.c_int32), ("index_bits", C.c_int32),
+                ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("scale", C.c_float)]
+
+
 class TrimulLibraryError(RuntimeError):
     """The native library is missing, cannot be loaded, or a call into it failed."""
 
@@ -139,7 +174,7 @@ def load():
             lib = C.CDLL(str(path))
         except OSError as exc:  # pragma: no cover - depends on the host
             raise TrimulLibraryError(f"cannot load {path}: {exc}") from exc
-        missing = [name for name in EXPORTED_SYMBOLS if not hasattr(lib, name)]
+        missing = [name for name in EXPORTED_SYMBOLS + PAIR_SYMBOLS if not hasattr(lib, name)]
         if missing:
             raise TrimulLibraryError(
                 f"{path} was built from older sources: it does not export {missing}. Rebuild it with "
@@ -184,6 +219,15 @@ def load():
                      "trimul_sm100_forward", "trimul_sm100_peer_signal", "trimul_sm100_peer_wait",
                      "trimul_sm100_plan_create", "trimul_sm100_plan_ln_gated_proj", "trimul_sm100_plan_tri_contract",
                      "trimul_sm100_plan_ln_out_proj"):
+            getattr(lib, name).restype = C.c_int
+        norm, embed, tensor, bytes_out = (C.POINTER(t) for t in (PairNormDesc, PairEmbedDesc, PairTensor, C.c_uint64))
+        lib.pair_sm100_add_norm.argtypes = [norm, tensor, tensor, vp, vp, vp, vp, vp]
+        lib.pair_sm100_add_norm_grad_workspace.argtypes = [norm, bytes_out]
+        lib.pair_sm100_add_norm_grad.argtypes = [norm, tensor, tensor, tensor, vp, vp, vp, vp, vp, vp]
+        lib.pair_sm100_embed.argtypes = [embed, vp, vp, vp, vp, vp]
+        lib.pair_sm100_embed_grad_workspace.argtypes = [embed, bytes_out]
+        lib.pair_sm100_embed_grad.argtypes = [embed, vp, vp, vp, vp, vp]
+        for name in PAIR_SYMBOLS:
             getattr(lib, name).restype = C.c_int
         _lib = lib
         return lib

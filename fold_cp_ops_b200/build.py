@@ -18,14 +18,16 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libtrimul_sm100.so"
 
 SOURCES = ("trimul_capi.cu", "ln_gated_proj.cu", "tri_contract.cu", "tri_contract_pair.cu", "ln_out_proj.cu", "peer_sync.cu",
-           "forward_static.cu")
-HEADERS = ("sm100_ptx.cuh", "trimul_common.cuh", "trimul_kernels.h", "tri_contract_epilogue.cuh")
+           "forward_static.cu", "pair_norm.cu", "pair_norm_grad.cu", "pair_embed.cu")
+HEADERS = ("sm100_ptx.cuh", "trimul_common.cuh", "trimul_kernels.h", "tri_contract_epilogue.cuh", "pair_stream.cuh")
+PUBLIC_HEADERS = ("trimul_sm100.h", "pair_stream_sm100.h")
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-shared",
     "--use_fast_math",
+    "--threads", "0",
     "-diag-suppress", "177",
 )
 
@@ -37,7 +39,7 @@ def source_digest() -> str:
     import hashlib
 
     h = hashlib.sha256()
-    for f in [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / "trimul_sm100.h"]:
+    for f in [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]:
         h.update(f.name.encode())
         h.update(f.read_bytes())
     return h.hexdigest()[:32]
@@ -54,7 +56,7 @@ def is_stale() -> bool:
     if not LIB_PATH.exists():
         return True
     t = LIB_PATH.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / "trimul_sm100.h"]
+    deps = [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]
     return any(d.exists() and d.stat().st_mtime > t for d in deps)
 
 

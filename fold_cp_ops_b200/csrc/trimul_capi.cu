@@ -509,6 +509,18 @@ struct trimul_plan {
 namespace trimul {
 // Lets other translation units of the library leave a message in the slot trimul_sm100_last_error reads.
 void set_last_error(const char* msg) { fail(0, "%s", msg); }
+
+// For the entry points of the other source files: their messages come back through trimul_sm100_last_error() too.
+int report_error(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int current_device_sms() { return num_sms_current(); }
+
 }  // namespace trimul
 
 extern "C" {
