@@ -220,13 +220,13 @@ def load():
                      "trimul_sm100_plan_create", "trimul_sm100_plan_ln_gated_proj", "trimul_sm100_plan_tri_contract",
                      "trimul_sm100_plan_ln_out_proj"):
             getattr(lib, name).restype = C.c_int
-        norm, embed, tensor, bytes_out = (C.POINTER(t) for t in (PairNormDesc, PairEmbedDesc, PairTensor, C.c_uint64))
-        lib.pair_sm100_add_norm.argtypes = [norm, tensor, tensor, vp, vp, vp, vp, vp]
-        lib.pair_sm100_add_norm_grad_workspace.argtypes = [norm, bytes_out]
-        lib.pair_sm100_add_norm_grad.argtypes = [norm, tensor, tensor, tensor, vp, vp, vp, vp, vp, vp]
-        lib.pair_sm100_embed.argtypes = [embed, vp, vp, vp, vp, vp]
-        lib.pair_sm100_embed_grad_workspace.argtypes = [embed, bytes_out]
-        lib.pair_sm100_embed_grad.argtypes = [embed, vp, vp, vp, vp, vp]
+        # the pair-stream records come as packed bytes or by reference: plain pointers either way
+        lib.pair_sm100_add_norm.argtypes = [vp] * 8
+        lib.pair_sm100_add_norm_grad_workspace.argtypes = [vp, C.POINTER(C.c_uint64)]
+        lib.pair_sm100_add_norm_grad.argtypes = [vp] * 10
+        lib.pair_sm100_embed.argtypes = [vp] * 6
+        lib.pair_sm100_embed_grad_workspace.argtypes = [vp, C.POINTER(C.c_uint64)]
+        lib.pair_sm100_embed_grad.argtypes = [vp] * 6
         for name in PAIR_SYMBOLS:
             getattr(lib, name).restype = C.c_int
         _lib = lib

@@ -16,7 +16,7 @@
 namespace pair {
 namespace {
 
-constexpr int kSlabOcts = 32;            // octs (256 channels) of a row that one warp covers
+constexpr int kSlab = 256;               // channels of a row that one warp covers
 constexpr int kSortWarps = 4;            // warps per CTA of the sorting kernels
 constexpr int kMaxDigitBits = 11;        // bins of one sorting pass: 2^11 counters of 4 bytes per warp
 constexpr uint32_t kNone = 0xffffffffu;  // key of a token without an embedding
@@ -36,49 +36,73 @@ struct IndexView {
   }
 };
 
-template <bool kWide>
-__device__ __forceinline__ void load_table(const void* table, int dtype, int64_t at, int n, float (&f)[8]) {
+// Eight channels of a row per lane: whole octs of aligned rows (kWide), or channels that lie kGroup apart, so that the accesses of
+// the lanes are contiguous either way.
+template <bool kWide, int kGroup>
+__device__ __forceinline__ int channel_of(int lane, int e) { return kWide ? lane * 8 + e : lane + e * kGroup; }
+
+template <bool kWide, int kGroup, typename T>
+__device__ __forceinline__ Unit<T, 8> load_eight(const T* row, int lane, int left) {
   if constexpr (kWide) {
-    if (dtype == PAIR_FP32) {
-      const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(table) + at);
-      const float4 x = __ldg(p), y = __ldg(p + 1);
-      f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w, f[4] = y.x, f[5] = y.y, f[6] = y.z, f[7] = y.w;
-    } else {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(table) + at));
-      if (dtype == PAIR_FP16)
-        unpack(reinterpret_cast<const Oct<__half>&>(x), f);
-      else
-        unpack(reinterpret_cast<const Oct<__nv_bfloat16>&>(x), f);
-    }
+    return lane * 8 < left ? load_unit<T, 8>(row + lane * 8) : zero_unit<T, 8>();
   } else {
+    Unit<T, 8> o;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = k < n ? load_any(table, at + k, dtype) : 0.f;
+    for (int e = 0; e < 8; ++e) o.e[e] = lane + e * kGroup < left ? load_unit<T, 1>(row + lane + e * kGroup).e[0] : from_f32<T>(0.f);
+    return o;
   }
 }
 
-template <bool kWide>
-__device__ __forceinline__ void store_table(void* table, int dtype, int64_t at, int n, const float (&f)[8]) {
+template <bool kWide, int kGroup>
+__device__ __forceinline__ void store_eight(void* table, int dtype, int64_t at, int lane, int left, const float (&f)[8]) {
   if constexpr (kWide) {
+    if (lane * 8 >= left) return;
+    Vals<8> v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.p[e] = make_float2(f[2 * e], f[2 * e + 1]);
+    at += lane * 8;
     if (dtype == PAIR_FP32)
-      store_oct<true>(static_cast<float*>(table) + at, pack<float>(f), 8);
+      store_unit<float, 8>(static_cast<float*>(table) + at, pack<float, 8>(v));
     else if (dtype == PAIR_FP16)
-      store_oct<true>(static_cast<__half*>(table) + at, pack<__half>(f), 8);
+      store_unit<__half, 8>(static_cast<__half*>(table) + at, pack<__half, 8>(v));
     else
-      store_oct<true>(static_cast<__nv_bfloat16*>(table) + at, pack<__nv_bfloat16>(f), 8);
+      store_unit<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(table) + at, pack<__nv_bfloat16, 8>(v));
   } else {
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) store_any(table, at + k, dtype, f[k]);
+    for (int e = 0; e < 8; ++e)
+      if (lane + e * kGroup < left) store_any(table, at + lane + e * kGroup, dtype, f[e]);
   }
 }
 
 // ---------------------------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------------------------
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(kThreads) embed_kernel(IndexView index, const void* table, int table_dtype, const T* base,
-                                                         T* out, uint32_t tokens, int d, int octs, FastDiv by_octs, float scale) {
-  const int64_t total = static_cast<int64_t>(tokens) * octs;
+struct EmbedArgs {
+  IndexView index;
+  const void* table;
+  const void* base;
+  void* out;
+  uint32_t tokens;
+  int d, octs, table_dtype;
+  float scale;
+};
+
+__device__ __forceinline__ Vals<8> table_oct(const void* table, int dtype, int64_t at) {
+  if (dtype == PAIR_FP32) {
+    Unit<float, 8> x;
+    reinterpret_cast<uint4*>(&x)[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(table) + at));
+    reinterpret_cast<uint4*>(&x)[1] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(table) + at) + 1);
+    return unpack(x);
+  }
+  const uint4 x = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(table) + at));
+  return dtype == PAIR_FP16 ? unpack(reinterpret_cast<const Unit<__half, 8>&>(x)) : unpack(reinterpret_cast<const Unit<__nv_bfloat16, 8>&>(x));
+}
+
+// Whole octs: one per thread and step.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embed_octs_kernel(const EmbedArgs a, const FastDiv by_octs) {
+  const T* base = static_cast<const T*>(a.base);
+  const int64_t total = static_cast<int64_t>(a.tokens) * a.octs;
   const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
   for (int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; n < total; n += step) {
     uint32_t t, v;
@@ -86,29 +110,40 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(IndexView index, const 
       t = by_octs.div(static_cast<uint32_t>(n));
       v = static_cast<uint32_t>(n) - t * by_octs.d;
     } else {
-      t = static_cast<uint32_t>(n / octs);
-      v = static_cast<uint32_t>(n - static_cast<int64_t>(t) * octs);
+      t = static_cast<uint32_t>(n / a.octs);
+      v = static_cast<uint32_t>(n - static_cast<int64_t>(t) * a.octs);
     }
-    const int left = d - static_cast<int>(v) * 8;
-    const int64_t at = static_cast<int64_t>(t) * d + v * 8;
-    const uint32_t row = index.at(t);
-    Oct<T> b;
-    if (base != nullptr) b = load_oct<kWide>(base + at, left);
-    float f[8], g[8];
+    const uint32_t row = a.index.at(t);
+    Unit<T, 8> b = zero_unit<T, 8>();
+    if (base != nullptr) b = load_unit<T, 8>(base + n * 8);
+    Vals<8> f = unpack(b);
     if (row != kNone) {
-      load_table<kWide>(table, table_dtype, static_cast<int64_t>(row) * d + v * 8, left, f);
+      const Vals<8> x = table_oct(a.table, a.table_dtype, static_cast<int64_t>(row) * a.d + v * 8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= scale;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = 0.f;
+      for (int e = 0; e < 4; ++e) f.p[e] = __ffma2_rn(x.p[e], both(a.scale), f.p[e]);
     }
-    if (base != nullptr) {
-      unpack(b, g);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += g[e];
+    store_unit<T, 8>(static_cast<T*>(a.out) + n * 8, pack<T, 8>(f));
+  }
+}
+
+// Other rows: a warp per token, channels 32 apart.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embed_rows_kernel(const EmbedArgs a) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t span = gridDim.x * (kThreads / 32);
+  for (uint32_t t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); t < a.tokens; t += span) {
+    const uint32_t row = a.index.at(t);
+    const T* base = a.base != nullptr ? static_cast<const T*>(a.base) + static_cast<int64_t>(t) * a.d : nullptr;
+    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(t) * a.d;
+    const int64_t at = static_cast<int64_t>(row) * a.d;
+#pragma unroll 8
+    for (int c = lane; c < a.d; c += 32) {
+      float f = row != kNone ? load_any(a.table, at + c, a.table_dtype) * a.scale : 0.f;
+      if (base != nullptr) f += to_f32(load_unit<T, 1>(base + c).e[0]);
+      Unit<T, 1> o;
+      o.e[0] = from_f32<T>(f);
+      store_unit<T, 1>(out + c, o);
     }
-    store_oct<kWide>(out + at, pack<T>(f), left);
   }
 }
 
@@ -119,12 +154,12 @@ __global__ void __launch_bounds__(kThreads) embed_kernel(IndexView index, const 
 // add the rows that match, in ascending order; the warps' sums are joined in order.
 template <typename T, bool kWide>
 __global__ void __launch_bounds__(kThreads) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table,
-                                                                  int table_dtype, uint32_t tokens, int d, int octs, float scale) {
-  __shared__ float sums[kThreads / 32][kSlabOcts * 8 + 8];
+                                                                  int table_dtype, uint32_t tokens, int d, float scale) {
+  constexpr int kAhead = 4;
+  __shared__ float sums[kThreads / 32][kSlab];
   const uint32_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int v = blockIdx.y * kSlabOcts + lane;
-  const bool on = v < octs;
+  const int slab = blockIdx.y * kSlab, left = d - slab;
   const uint32_t share = ((tokens + 8 * 32 - 1) / (8 * 32)) * 32;
   const uint32_t lo = warp * share, hi = min(tokens, lo + share);
   float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -132,38 +167,32 @@ __global__ void __launch_bounds__(kThreads) embed_grad_few_kernel(IndexView inde
     const uint32_t t = t0 + lane;
     uint32_t hit = __ballot_sync(0xffffffffu, t < hi && index.at(t) == row);
     while (hit != 0) {
-      Oct<T> o[4];
-      int n = 0;
+      Unit<T, 8> o[kAhead];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
+      for (int k = 0; k < kAhead; ++k) {
+        o[k] = zero_unit<T, 8>();
         if (hit != 0) {
-          const uint32_t at = t0 + __ffs(hit) - 1;
+          o[k] = load_eight<kWide, 32>(d_out + static_cast<int64_t>(t0 + __ffs(hit) - 1) * d + slab, lane, left);
           hit &= hit - 1;
-          o[k] = on ? load_oct<kWide>(d_out + static_cast<int64_t>(at) * d + v * 8, d - v * 8) : zero_oct<T>();
-          n = k + 1;
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (k < n) {
-          float f[8];
-          unpack(o[k], f);
+      for (int k = 0; k < kAhead; ++k)
 #pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] += f[e];
-        }
+        for (int e = 0; e < 8; ++e) acc[e] += to_f32(o[k].e[e]);
     }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
+  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = acc[e];
   __syncthreads();
-  if (warp != 0 || !on) return;
+  if (warp != 0) return;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
 #pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) acc[e] += sums[w][lane * 8 + e];
+    for (int w = 1; w < kThreads / 32; ++w) acc[e] += sums[w][lane + e * 32];
     acc[e] *= scale;
   }
-  store_table<kWide>(d_table, table_dtype, static_cast<int64_t>(row) * d + v * 8, d - v * 8, acc);
+  store_eight<kWide, 32>(d_table, table_dtype, static_cast<int64_t>(row) * d + slab, lane, left, acc);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -179,6 +208,8 @@ struct SortArgs {
   uint32_t* totals;  // (bins)
   uint32_t tokens, tiles, tile;
   int shift, bins;
+  uint4* clear;  // nullable: the first pass also clears the table's gradient, for the rows that no token names
+  int64_t clear_vecs;
 };
 
 // Tokens without an embedding sort behind all others: their key is the number of rows.
@@ -192,6 +223,10 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortA
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t* mine = smem + warp * a.bins;
   const uint32_t w = blockIdx.x * kSortWarps + warp;
+  if (a.clear != nullptr)
+    for (int64_t n = static_cast<int64_t>(blockIdx.x) * (kSortWarps * 32) + threadIdx.x; n < a.clear_vecs;
+         n += static_cast<int64_t>(gridDim.x) * (kSortWarps * 32))
+      a.clear[n] = make_uint4(0, 0, 0, 0);
   for (int k = lane; k < a.bins; k += 32) mine[k] = 0;
   __syncwarp();
   if (w >= a.tiles) return;
@@ -301,151 +336,196 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_place_kernel(const SortA
 // ---------------------------------------------------------------------------------------------
 // sums over the sorted tokens
 // ---------------------------------------------------------------------------------------------
+// The sorted tokens are cut into equal shares, one per group of lanes; the shares of a CTA are neighbours.  A run (equal
+// indices) inside one share goes straight to the table.  A run that crosses shares leaves a piece in each: the CTA joins the pieces of
+// its own shares, and what crosses CTAs is left in the workspace with the CTA's edges, for the second kernel.
+struct Edge {
+  uint32_t first, last;  // index of the first and last run
+  uint32_t bits;
+  uint32_t pad;
+};
+constexpr uint32_t kFromLeft = 1, kToRight = 2, kOneRun = 4;
+
 template <typename T>
 struct SumArgs {
   IndexView index;
   const uint32_t* sorted;
   const T* d_out;
   void* d_table;
-  float* pieces;  // (shares, 2, padded width): sums of runs that cross into [0] / out of [1] the share
-  uint32_t tokens, share, shares;
-  int d, octs, table_dtype;
+  float* pieces;  // (CTAs, 2, width): what crosses into the CTA, and what begins in it and crosses out
+  Edge* edges;    // (CTAs)
+  uint32_t tokens, share, ctas;
+  int d, width, table_dtype;
   float scale;
   __device__ __forceinline__ uint32_t key(uint32_t p) const { return index.at(sorted[p]); }
 };
 
-// kGroup lanes sum one share of sorted tokens over one slab of channels (blockIdx.y).
 template <typename T, int kGroup, bool kWide>
-__global__ void __launch_bounds__(kThreads) sum_runs_kernel(const SumArgs<T> a) {
-  constexpr int kAhead = 8;  // rows of d_out in flight per lane
-  const int lane = threadIdx.x % kGroup;
-  const uint32_t mask = kGroup == 32 ? 0xffffffffu : ((1u << kGroup) - 1) << ((threadIdx.x & 31) / kGroup * kGroup);
-  const uint32_t share = blockIdx.x * (kThreads / kGroup) + threadIdx.x / kGroup;
-  if (share >= a.shares) return;
-  const int v = blockIdx.y * kSlabOcts + lane;
-  const bool on = v < a.octs;
-  const uint32_t lo = share * a.share, hi = min(a.tokens, lo + a.share);
+__global__ void __launch_bounds__(kThreads, 3) sum_runs_kernel(const SumArgs<T> a) {
+  constexpr int kAhead = kWide ? 8 : 4;  // rows of d_out in flight per lane
+  constexpr int kGroups = kThreads / kGroup;
+  constexpr int kChannels = kGroup * 8;
+  __shared__ float piece[2][kGroups][kChannels];
+  __shared__ Edge edge[kGroups];
+  const int lane = threadIdx.x % kGroup, group = threadIdx.x / kGroup;
+  const uint32_t mask = kGroup == 32 ? 0xffffffffu : ((1u << (kGroup & 31)) - 1) << ((threadIdx.x & 31) / kGroup * kGroup);
+  const uint32_t share = blockIdx.x * kGroups + group;
+  const int slab = blockIdx.y * kSlab, left = a.d - slab;
+  // 64 bits: the last CTA's shares may begin behind 2^32
+  const uint64_t begin = static_cast<uint64_t>(share) * a.share;
+  const uint32_t lo = begin < a.tokens ? static_cast<uint32_t>(begin) : a.tokens;
+  const uint32_t hi = min(a.tokens, lo + a.share);
 
-  double total[8];
-  float acc[8];
+  if (lo < hi) {
+    float total[8], acc[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) total[e] = 0.0, acc[e] = 0.f;
-  uint32_t run = a.key(lo);  // index of the run at hand
-  bool from_left = lo > 0 && a.key(lo - 1) == run;
+    for (int e = 0; e < 8; ++e) total[e] = acc[e] = 0.f;
+    const uint32_t first = a.key(lo);
+    const bool crosses_in = lo > 0 && a.key(lo - 1) == first;
+    const uint32_t next = hi < a.tokens ? a.key(hi) : kNone;
+    uint32_t run = first;  // index of the run at hand
+    bool from_left = crosses_in, one = true;
 
-  auto flush = [&](bool to_right) {
-    if (run == kNone || !on) return;
-    float f[8];
-    if (from_left || to_right) {
-      float* p = a.pieces + (static_cast<int64_t>(share) * 2 + (from_left ? 0 : 1)) * (a.octs * 8) + v * 8;
+    for (uint32_t p0 = lo; p0 < hi; p0 += kGroup) {
+      const uint32_t p = p0 + lane;
+      const uint32_t my_token = p < hi ? a.sorted[p] : 0;
+      const uint32_t my_key = p < hi ? a.index.at(my_token) : kNone;
+      const int here = min(static_cast<uint32_t>(kGroup), hi - p0);
+      for (int e0 = 0; e0 < here; e0 += kAhead) {
+        Unit<T, 8> o[kAhead];
+        uint32_t key[kAhead];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(total[e] + acc[e]);
-      reinterpret_cast<float4*>(p)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(p)[1] = make_float4(f[4], f[5], f[6], f[7]);
-    } else {
+        for (int k = 0; k < kAhead; ++k) {
+          const uint32_t t = __shfl_sync(mask, my_token, e0 + k, kGroup);
+          key[k] = __shfl_sync(mask, my_key, e0 + k, kGroup);
+          o[k] = key[k] != kNone ? load_eight<kWide, kGroup>(a.d_out + static_cast<int64_t>(t) * a.d + slab, lane, left)
+                                 : zero_unit<T, 8>();
+        }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = static_cast<float>(total[e] + acc[e]) * a.scale;
-      store_table<kWide>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + v * 8, a.d - v * 8, f);
-    }
-  };
-
-  for (uint32_t p0 = lo; p0 < hi; p0 += kGroup) {
-    const uint32_t p = p0 + lane;
-    const uint32_t my_token = p < hi ? a.sorted[p] : 0;
-    const uint32_t my_key = p < hi ? a.index.at(my_token) : kNone;
-    const int here = min(static_cast<uint32_t>(kGroup), hi - p0);
-    for (int e0 = 0; e0 < here; e0 += kAhead) {
-      Oct<T> o[kAhead];
-      uint32_t key[kAhead];
+        for (int k = 0; k < kAhead; ++k) {
+          if (e0 + k < here) {
+            if (key[k] != run) {
+              if (from_left) {
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        const uint32_t t = __shfl_sync(mask, my_token, e0 + k, kGroup);
-        key[k] = __shfl_sync(mask, my_key, e0 + k, kGroup);
-        o[k] = on && e0 + k < here && key[k] != kNone
-                   ? load_oct<kWide>(a.d_out + static_cast<int64_t>(t) * a.d + v * 8, a.d - v * 8)
-                   : zero_oct<T>();
-      }
+                for (int e = 0; e < 8; ++e) piece[0][group][channel_of<kWide, kGroup>(lane, e)] = total[e] + acc[e];
+              } else {
+                float f[8];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        if (e0 + k < here) {
-          if (key[k] != run) {
-            flush(false);
-            run = key[k];
-            from_left = false;
+                for (int e = 0; e < 8; ++e) f[e] = (total[e] + acc[e]) * a.scale;
+                store_eight<kWide, kGroup>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + slab, lane, left, f);
+              }
+              run = key[k];
+              from_left = one = false;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) total[e] = 0.0, acc[e] = 0.f;
+              for (int e = 0; e < 8; ++e) total[e] = acc[e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] += to_f32(o[k].e[e]);
           }
-          float f[8];
-          unpack(o[k], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] += f[e];
         }
       }
-    }
-    // fp32 sums of at most 32 terms are carried over to 64 bits
+      // sums of at most 32 terms first: the error grows with the root of either count
 #pragma unroll
-    for (int e = 0; e < 8; ++e) total[e] += acc[e], acc[e] = 0.f;
-  }
-  flush(hi < a.tokens && a.key(hi) == run);
-}
-
-// The share in which a crossing run begins adds up its pieces: its own [1], then [0] of the shares that follow.
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(kThreads) join_runs_kernel(const SumArgs<T> a) {
-  __shared__ double sums[kThreads / 32][kSlabOcts * 8];
-  __shared__ uint32_t last;
-  const uint32_t share = blockIdx.x;
-  const uint32_t lo = share * a.share, hi = lo + a.share;
-  if (hi >= a.tokens) return;
-  const uint32_t run = a.key(hi - 1);
-  if (run == kNone || a.key(hi) != run) return;
-  if (lo > 0 && a.key(lo - 1) == run) return;  // the run began before this share
-  // the last share that the run reaches: the first keys of the shares are sorted
-  if (threadIdx.x == 0) last = share;
-  __syncthreads();
-  uint32_t from = share + 1, until = a.shares;  // shares [from, until) may begin with the run
-  while (from < until) {
-    const uint32_t step = (until - from + kThreads - 1) / kThreads;
-    const uint32_t at = from + threadIdx.x * step;
-    const bool mine = at < until && a.key(at * a.share) == run;
-    const int n = __syncthreads_count(mine);  // a prefix of the probes
-    if (n == 0) break;
-    const uint32_t reached = from + (n - 1) * step;
-    if (threadIdx.x == 0) last = reached;
-    from = reached + 1;
-    until = min(until, reached + step);
-  }
-  __syncthreads();
-  const uint32_t end = last + 1;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t width = a.octs * 8;
-  // eight warps, each an equal part of the pieces in order
-  const uint32_t pieces = end - share, per = (pieces + 7) / 8;
-  const uint32_t p_lo = share + min(pieces, warp * per), p_hi = share + min(pieces, (warp + 1) * per);
-  for (int slab = 0; slab * kSlabOcts < a.octs; ++slab) {
-    const int v = slab * kSlabOcts + lane;
-    double acc[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (v < a.octs) {
-#pragma unroll 4
-      for (uint32_t s = p_lo; s < p_hi; ++s) {
-        const float4* p = reinterpret_cast<const float4*>(a.pieces + (static_cast<int64_t>(s) * 2 + (s == share ? 1 : 0)) * width + v * 8);
-        const float4 x = p[0], y = p[1];
-        acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
-        acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
-      }
+      for (int e = 0; e < 8; ++e) total[e] += acc[e], acc[e] = 0.f;
     }
+    const bool to_right = run != kNone && next == run;
+    if (from_left || to_right) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[warp][lane * 8 + e] = acc[e];
-    __syncthreads();
-    if (warp == 0 && v < a.octs) {
+      for (int e = 0; e < 8; ++e) piece[from_left ? 0 : 1][group][channel_of<kWide, kGroup>(lane, e)] = total[e];
+    } else if (run != kNone) {
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-#pragma unroll
-        for (int w = 1; w < kThreads / 32; ++w) acc[e] += sums[w][lane * 8 + e];
-        f[e] = static_cast<float>(acc[e]) * a.scale;
+      for (int e = 0; e < 8; ++e) f[e] = total[e] * a.scale;
+      store_eight<kWide, kGroup>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + slab, lane, left, f);
+    }
+    if (lane == 0) edge[group] = Edge{first, run, (crosses_in ? kFromLeft : 0) | (to_right ? kToRight : 0) | (one ? kOneRun : 0), 0};
+  } else if (lane == 0) {
+    edge[group] = Edge{kNone, kNone, kOneRun, 0};
+  }
+  __syncthreads();
+
+  // Join the pieces of neighbouring shares, one channel per thread.
+  const int c = threadIdx.x;
+  if (c < kChannels && c < left) {
+    double sum = 0.0;
+    bool before = false;  // the run at hand began before this CTA
+    bool open = false;
+    for (int g = 0; g < kGroups; ++g) {
+      const Edge s = edge[g];
+      if (s.first == kNone) break;  // tokens without an embedding, or behind the last one
+      if (s.bits & kFromLeft) {
+        if (g == 0) before = true;
+        sum += piece[0][g][c];
+        open = (s.bits & kOneRun) && (s.bits & kToRight);
+        if (!open) {
+          if (before)
+            a.pieces[static_cast<int64_t>(blockIdx.x) * 2 * a.width + slab + c] = static_cast<float>(sum);
+          else
+            store_any(a.d_table, static_cast<int64_t>(s.first) * a.d + slab + c, a.table_dtype, static_cast<float>(sum) * a.scale);
+          before = false;
+        }
       }
-      store_table<kWide>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + v * 8, a.d - v * 8, f);
+      if ((s.bits & kToRight) && !((s.bits & kOneRun) && (s.bits & kFromLeft))) {
+        sum = piece[1][g][c];
+        open = true;
+      }
+    }
+    if (open) a.pieces[(static_cast<int64_t>(blockIdx.x) * 2 + (before ? 0 : 1)) * a.width + slab + c] = static_cast<float>(sum);
+  }
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
+    // the CTA's own edges: it is one run when every share that has tokens is, and is entered or left as its outer shares are
+    Edge out = edge[0];
+    bool one = true;
+    for (int g = 0; g < kGroups; ++g) {
+      if (static_cast<uint64_t>(blockIdx.x * kGroups + g) * a.share >= a.tokens) break;
+      one = one && (edge[g].bits & kOneRun) && edge[g].first == out.first;
+      out.last = edge[g].last;
+      out.bits = (out.bits & kFromLeft) | (edge[g].bits & kToRight);
+    }
+    out.bits |= one ? kOneRun : 0;
+    a.edges[blockIdx.x] = out;
+  }
+}
+
+// The CTA in which a crossing run begins adds up its pieces: its own [1], then [0] of the CTAs that follow.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_runs_kernel(const SumArgs<T> a) {
+  __shared__ float4 sums[kThreads / 32][32];
+  const uint32_t cta = blockIdx.x;
+  const Edge own = a.edges[cta];
+  if (!(own.bits & kToRight) || ((own.bits & kOneRun) && (own.bits & kFromLeft))) return;
+  // the run ends in the first CTA that it does not fill and leave (the last CTA is left by none)
+  __shared__ uint32_t stop;
+  if (threadIdx.x == 0) stop = 0xffffffffu;
+  for (uint32_t from = cta + 1;; from += kThreads) {
+    __syncthreads();
+    const uint32_t at = from + threadIdx.x;
+    if (at >= a.ctas || (a.edges[at].bits & (kOneRun | kToRight)) != (kOneRun | kToRight)) atomicMin(&stop, at);
+    __syncthreads();
+    if (stop != 0xffffffffu) break;
+  }
+  const uint32_t end = stop + 1;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // eight warps, each an equal part of the pieces in order; 128 channels at a time
+  const uint32_t pieces = end - cta, per = (pieces + 7) / 8;
+  const uint32_t p_lo = min(pieces, warp * per), p_hi = min(pieces, (warp + 1) * per);
+  for (int c0 = blockIdx.y * 128; c0 < a.width; c0 += gridDim.y * 128) {
+    const int c = c0 + lane * 4;
+    double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
+    if (c < a.width) {
+#pragma unroll 8
+      for (uint32_t k = p_lo; k < p_hi; ++k) {
+        const float4 x = *reinterpret_cast<const float4*>(a.pieces + (static_cast<int64_t>(cta + k) * 2 + (k == 0 ? 1 : 0)) * a.width + c);
+        s0 += x.x, s1 += x.y, s2 += x.z, s3 += x.w;
+      }
+    }
+    sums[warp][lane] = make_float4(static_cast<float>(s0), static_cast<float>(s1), static_cast<float>(s2), static_cast<float>(s3));
+    __syncthreads();
+    if (threadIdx.x < 128 && c0 + threadIdx.x < a.d) {
+      double sum = 0.0;
+#pragma unroll
+      for (int w = 0; w < kThreads / 32; ++w) sum += reinterpret_cast<const float*>(sums[w])[threadIdx.x];
+      store_any(a.d_table, static_cast<int64_t>(own.last) * a.d + c0 + threadIdx.x, a.table_dtype, static_cast<float>(sum) * a.scale);
     }
     __syncthreads();
   }
@@ -456,20 +536,17 @@ __global__ void __launch_bounds__(kThreads) join_runs_kernel(const SumArgs<T> a)
 // ---------------------------------------------------------------------------------------------
 struct Plan {
   bool few;
-  int octs, passes, digit_bits, bins;
-  uint32_t tiles, tile, share, shares;
-  uint64_t sorted_at[2], counts_at, totals_at, pieces_at, bytes;
+  int passes, digit_bits, bins, group, slabs, width;
+  uint32_t tiles, tile, share, ctas;
+  uint64_t sorted_at[2], counts_at, totals_at, pieces_at, edges_at, bytes;
 };
 
 inline uint64_t up256(uint64_t n) { return (n + 255) & ~255ull; }
 
-// Lanes that cover a row (of at most one slab).
-inline int group_of(int octs) { return octs <= 8 ? 8 : octs <= 16 ? 16 : 32; }
-
 Plan make_plan(const pair_embed_desc_t* d, int sms) {
   Plan p = {};
   const uint64_t tokens = static_cast<uint64_t>(d->tokens);
-  p.octs = (d->d + 7) / 8;
+  p.slabs = (d->d + kSlab - 1) / kSlab;
   p.few = tokens <= 2048 && tokens * static_cast<uint64_t>(d->rows) <= (1u << 22);
   if (p.few) {
     p.bytes = 256;
@@ -487,30 +564,48 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   if (tiles > most) tiles = most;
   p.tile = static_cast<uint32_t>(((tokens + tiles - 1) / tiles + 31) / 32 * 32);
   p.tiles = static_cast<uint32_t>((tokens + p.tile - 1) / p.tile);
-  // shares: one wave of resident groups, of at least 32 tokens
-  const uint64_t groups = static_cast<uint64_t>(sms) * (4 * kThreads / group_of(p.octs));
-  uint64_t share = (tokens + groups - 1) / groups;
-  if (share < 32) share = 32;
+  // shares: one wave of resident groups (three CTAs an SM over all slabs), of at least 8 tokens
+  p.group = d->d <= 64 ? 8 : d->d <= 128 ? 16 : 32;
+  p.width = (d->d + 7) / 8 * 8;
+  const int held = kThreads / p.group;
+  uint64_t ctas = static_cast<uint64_t>(sms) * 3 / p.slabs;
+  if (ctas < 1) ctas = 1;
+  uint64_t share = (tokens + ctas * held - 1) / (ctas * held);
+  if (share < 8) share = 8;
   p.share = static_cast<uint32_t>(share);
-  p.shares = static_cast<uint32_t>((tokens + share - 1) / share);
+  p.ctas = static_cast<uint32_t>((tokens + share * held - 1) / (share * held));
   uint64_t at = 0;
   p.sorted_at[0] = at, at += up256(tokens * 4);
   p.sorted_at[1] = at, at += p.passes > 1 ? up256(tokens * 4) : 0;
   p.counts_at = at, at += up256(static_cast<uint64_t>(p.bins) * p.tiles * 4);
   p.totals_at = at, at += up256(static_cast<uint64_t>(p.bins) * 4);
-  p.pieces_at = at, at += up256(static_cast<uint64_t>(p.shares) * 2 * p.octs * 8 * 4);
+  p.pieces_at = at, at += up256(static_cast<uint64_t>(p.ctas) * 2 * p.width * 4);
+  p.edges_at = at, at += up256(static_cast<uint64_t>(p.ctas) * sizeof(Edge));
   p.bytes = at;
   return p;
 }
 
-template <typename T, bool kWide>
+template <typename T>
 cudaError_t embed_run(const pair_embed_desc_t* d, const IndexView& index, const void* table, const void* base, void* out,
-                      int sms, cudaStream_t s) {
-  const int octs = (d->d + 7) / 8;
-  const int64_t need = (d->tokens * octs + kThreads - 1) / kThreads, most = static_cast<int64_t>(sms) * 8;
-  embed_kernel<T, kWide><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(
-      index, table, d->table_dtype, static_cast<const T*>(base), static_cast<T*>(out), static_cast<uint32_t>(d->tokens), d->d,
-      octs, make_fast_div(octs), d->scale);
+                      bool wide, int sms, cudaStream_t s) {
+  EmbedArgs a;
+  a.index = index;
+  a.table = table;
+  a.base = base;
+  a.out = out;
+  a.tokens = static_cast<uint32_t>(d->tokens);
+  a.d = d->d;
+  a.octs = (d->d + 7) / 8;
+  a.table_dtype = d->table_dtype;
+  a.scale = d->scale;
+  const int64_t most = static_cast<int64_t>(sms) * 8;
+  if (wide) {
+    const int64_t need = (d->tokens * a.octs + kThreads - 1) / kThreads;
+    embed_octs_kernel<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, make_fast_div(a.octs));
+  } else {
+    const int64_t need = (d->tokens + kThreads / 32 - 1) / (kThreads / 32);
+    embed_rows_kernel<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
+  }
   return cudaGetLastError();
 }
 
@@ -519,16 +614,13 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
                      int sms, cudaStream_t s) {
   const Plan p = make_plan(d, sms);
   const uint32_t tokens = static_cast<uint32_t>(d->tokens);
-  const int slabs = (p.octs + kSlabOcts - 1) / kSlabOcts;
   if (p.few) {
-    embed_grad_few_kernel<T, kWide><<<dim3(d->rows, slabs), kThreads, 0, s>>>(
-        index, static_cast<const T*>(d_out), d_table, d->table_dtype, tokens, d->d, p.octs, d->scale);
+    embed_grad_few_kernel<T, kWide><<<dim3(d->rows, p.slabs), kThreads, 0, s>>>(
+        index, static_cast<const T*>(d_out), d_table, d->table_dtype, tokens, d->d, d->scale);
     return cudaGetLastError();
   }
   char* ws = static_cast<char*>(workspace);
-  // rows that no token names; the others are written afterwards
-  cudaError_t e = cudaMemsetAsync(d_table, 0, static_cast<size_t>(d->rows) * d->d * type_bytes(d->table_dtype), s);
-  if (e != cudaSuccess) return e;
+  cudaError_t e;
   SortArgs a;
   a.index = index;
   a.counts = reinterpret_cast<uint32_t*>(ws + p.counts_at);
@@ -538,6 +630,16 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   a.tile = p.tile;
   a.bins = p.bins;
   a.in = nullptr;
+  // rows that no token names become 0; the others are written afterwards
+  const uint64_t table_bytes = static_cast<uint64_t>(d->rows) * d->d * type_bytes(d->table_dtype);
+  a.clear = nullptr;
+  a.clear_vecs = static_cast<int64_t>(table_bytes / 16);
+  if (aligned(d_table, 16) && table_bytes % 16 == 0) {
+    a.clear = static_cast<uint4*>(d_table);
+  } else {
+    e = cudaMemsetAsync(d_table, 0, table_bytes, s);
+    if (e != cudaSuccess) return e;
+  }
   const int count_smem = kSortWarps * p.bins * 4, place_smem = (kSortWarps + 1) * p.bins * 4;
   const unsigned grid = (p.tiles + kSortWarps - 1) / kSortWarps;
   for (int pass = 0; pass < p.passes; ++pass) {
@@ -550,6 +652,7 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
     e = cudaGetLastError();
     if (e != cudaSuccess) return e;
     a.in = a.out;
+    a.clear = nullptr;
   }
   SumArgs<T> m;
   m.index = index;
@@ -557,25 +660,24 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   m.d_out = static_cast<const T*>(d_out);
   m.d_table = d_table;
   m.pieces = reinterpret_cast<float*>(ws + p.pieces_at);
+  m.edges = reinterpret_cast<Edge*>(ws + p.edges_at);
   m.tokens = tokens;
   m.share = p.share;
-  m.shares = p.shares;
+  m.ctas = p.ctas;
   m.d = d->d;
-  m.octs = p.octs;
+  m.width = p.width;
   m.table_dtype = d->table_dtype;
   m.scale = d->scale;
-  const int group = group_of(p.octs);
-  const int held = kThreads / group;
-  const dim3 sum_grid((p.shares + held - 1) / held, slabs);
-  if (group == 8)
+  const dim3 sum_grid(p.ctas, p.slabs);
+  if (p.group == 8)
     sum_runs_kernel<T, 8, kWide><<<sum_grid, kThreads, 0, s>>>(m);
-  else if (group == 16)
+  else if (p.group == 16)
     sum_runs_kernel<T, 16, kWide><<<sum_grid, kThreads, 0, s>>>(m);
   else
     sum_runs_kernel<T, 32, kWide><<<sum_grid, kThreads, 0, s>>>(m);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  join_runs_kernel<T, kWide><<<p.shares, kThreads, 0, s>>>(m);
+  join_runs_kernel<T><<<dim3(p.ctas, (p.width + 127) / 128 < 4 ? (p.width + 127) / 128 : 4), kThreads, 0, s>>>(m);
   return cudaGetLastError();
 }
 
@@ -610,17 +712,14 @@ extern "C" int pair_sm100_embed(const pair_embed_desc_t* desc, const void* index
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   const IndexView view{index, desc->index_bits, static_cast<uint32_t>(desc->rows)};
-  const bool wide = desc->d % 8 == 0 && aligned16(table) && aligned16(base) && aligned16(out);
+  const bool wide = desc->d % 8 == 0 && aligned(table, 16) && aligned(base, 16) && aligned(out, 16);
   cudaError_t e;
   if (desc->dtype == PAIR_FP32)
-    e = wide ? embed_run<float, true>(desc, view, table, base, out, sms, cuda_stream)
-             : embed_run<float, false>(desc, view, table, base, out, sms, cuda_stream);
+    e = embed_run<float>(desc, view, table, base, out, wide, sms, cuda_stream);
   else if (desc->dtype == PAIR_FP16)
-    e = wide ? embed_run<__half, true>(desc, view, table, base, out, sms, cuda_stream)
-             : embed_run<__half, false>(desc, view, table, base, out, sms, cuda_stream);
+    e = embed_run<__half>(desc, view, table, base, out, wide, sms, cuda_stream);
   else
-    e = wide ? embed_run<__nv_bfloat16, true>(desc, view, table, base, out, sms, cuda_stream)
-             : embed_run<__nv_bfloat16, false>(desc, view, table, base, out, sms, cuda_stream);
+    e = embed_run<__nv_bfloat16>(desc, view, table, base, out, wide, sms, cuda_stream);
   if (e != cudaSuccess) return report_error(TRIMUL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   return TRIMUL_OK;
 }
@@ -650,12 +749,12 @@ extern "C" int pair_sm100_embed_grad(const pair_embed_desc_t* desc, const void* 
     return TRIMUL_OK;
   }
   if (index == nullptr || d_out == nullptr) return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: index and d_out must not be NULL", who);
-  if (workspace == nullptr || !aligned16(workspace))
+  if (workspace == nullptr || !aligned(workspace, 16))
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace", who);
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   const IndexView view{index, desc->index_bits, static_cast<uint32_t>(desc->rows)};
-  const bool wide = desc->d % 8 == 0 && aligned16(d_out) && aligned16(d_table);
+  const bool wide = desc->d % 8 == 0 && aligned(d_out, 16) && aligned(d_table, 16);
   if (desc->dtype == PAIR_FP32)
     e = wide ? grad_run<float, true>(desc, view, d_out, d_table, workspace, sms, cuda_stream)
              : grad_run<float, false>(desc, view, d_out, d_table, workspace, sms, cuda_stream);

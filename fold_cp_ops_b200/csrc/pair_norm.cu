@@ -5,10 +5,13 @@
 // of the stream would give, and the gradient needs nothing but z.  The sum of squares and s are fp32.
 // e4m3 output: a = max |y| over a group of channels, scale = a / 448, q = e4m3(y / scale).
 //
-// Bound.  HBM: update and residual are read, z and y written once; nothing else moves.
+// Bound.  HBM: update and residual are read, z and y written once; nothing else moves.  Behind it come the issue slots:
+// a 16-bit oct has about 4 x 2 clocks' worth of them per SM while its 48 to 64 bytes move, so the arithmetic is in
+// packed fp32 pairs (and in packed 16-bit additions where there is no dropout).
 // Split.  A row of up to 256 channels is one oct (eight channels, 16 bytes of a 16-bit type) per lane of 8, 16 or 32
-// lanes, so that the reductions stay inside a warp; up to 1024 channels it is two or four octs per lane of a warp;
-// wider rows take a CTA.
+// lanes, so that the reductions stay inside a warp;
+// up to 512 channels it is two octs per lane of a warp; wider rows take a CTA with one oct per thread.  A group holds two
+// rows at a time where that is one 16-byte access per lane, row and tensor: more bytes in flight.
 #include "pair_stream.cuh"
 
 namespace pair {
@@ -16,7 +19,7 @@ namespace {
 
 constexpr float kE4m3Max = 448.f;
 
-enum Mode { kNorm = 0, kNormE4m3 = 1 };
+enum Mode { kNorm = 0, kNormE4m3 = 1, kAdd = 2 };
 
 template <typename T>
 struct NormArgs {
@@ -31,138 +34,207 @@ struct NormArgs {
   int d, octs;
   int weight_dtype;
   int group;  // channels per scale
-  float eps;
+  int flat;   // the rows of update and residual lie at a constant distance
+  float eps, inv_d;
 };
 
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
+__device__ __forceinline__ uint32_t e4m3x2(float2 v) {
   uint16_t r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(v.y), "f"(v.x));
   return r;
 }
 
-template <typename T, int kGroup, int kOcts, bool kWide, int kMode>
-__global__ void __launch_bounds__(kThreads) add_norm_kernel(const __grid_constant__ NormArgs<T> a) {
-  __shared__ float sums[2 * 8];
-  __shared__ float tops[2 * 8];
-  constexpr int kRows = kThreads / kGroup;  // rows a CTA holds at a time
+// kU channels per access, kGroup lanes per row, kUnits units per lane, kFlight rows of a group in flight.
+template <typename T, int kU, int kGroup, int kUnits, int kFlight, int kMode>
+__global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup)) add_norm_kernel(const __grid_constant__ NormArgs<T> a) {
+  __shared__ float sums[2 * 32 * kFlight];
+  __shared__ float tops[2 * 32 * kFlight];
+  constexpr int kRows = threads_of(kGroup) / kGroup;  // rows a CTA holds side by side
+  constexpr int kPairs = (kU + 1) / 2;
   const int lane = threadIdx.x % kGroup;
+  const int units = a.d / kU;
+  const bool dropping = a.drop.keep < 65536u;
+  const bool has_residual = a.residual.p != nullptr;
+  const uint32_t line = a.drop.keep << 16;
   Dropout drop = a.drop;
-  if (drop.keep < 65536u) resolve_seed(drop);
+  if (dropping) resolve_seed(drop);
 
-  float w[kOcts][8];
+  Vals<kU> w[kMode == kAdd ? 1 : kUnits];
+  if constexpr (kMode != kAdd) {
 #pragma unroll
-  for (int k = 0; k < kOcts; ++k)
+    for (int k = 0; k < kUnits; ++k) {
+      float f[kPairs * 2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = (lane + k * kGroup) * 8 + e;
-      w[k][e] = c < a.d ? load_any(a.weight, c, a.weight_dtype) : 0.f;
+      for (int e = 0; e < kPairs * 2; ++e) {
+        const int n = lane + k * kGroup;
+        f[e] = n < units && e < kU ? load_any(a.weight, n * kU + e, a.weight_dtype) : 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) w[k].p[e] = make_float2(f[2 * e], f[2 * e + 1]);
     }
+  }
 
   int parity = 0;
+  const uint32_t span = gridDim.x * kRows;
   // the bound is the CTA's first row: lanes whose row lies behind the end still take part in the reductions
-  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += gridDim.x * kRows, parity ^= 1) {
-    const uint32_t row = first + threadIdx.x / kGroup;
-    const bool valid = row < a.rows;
-    uint32_t b, i, j;
-    a.walk.at(valid ? row : 0, b, i, j);
-    const T* up = a.update.row(b, i, j);
-    const T* rp = a.residual.p != nullptr ? a.residual.row(b, i, j) : nullptr;
-    const int64_t out_row = static_cast<int64_t>(row) * a.d;
-
-    Oct<T> u[kOcts], r[kOcts];
+  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += kFlight * span, parity ^= 1) {
+    Unit<T, kU> u[kFlight][kUnits], r[kFlight][kUnits];
+    uint32_t b[kFlight], i[kFlight], j[kFlight];
 #pragma unroll
-    for (int k = 0; k < kOcts; ++k) {
-      const int v = lane + k * kGroup;
-      const bool on = valid && v < a.octs;
-      u[k] = on ? load_oct<kWide>(up + v * 8, a.d - v * 8) : zero_oct<T>();
-      r[k] = on && rp != nullptr ? load_oct<kWide>(rp + v * 8, a.d - v * 8) : zero_oct<T>();
-    }
-
-    float ss[1] = {0.f};
-#pragma unroll
-    for (int k = 0; k < kOcts; ++k) {
-      const int v = lane + k * kGroup;
-      float f[8], g[8];
-      unpack(u[k], f);
-      if (drop.keep < 65536u) apply_dropout(drop, b, i, j, v, f);
-      if (rp != nullptr) {
-        unpack(r[k], g);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] += g[e];
+    for (int f = 0; f < kFlight; ++f) {
+      const uint32_t row = first + f * span + threadIdx.x / kGroup;
+      const T *up, *rp;
+      b[f] = i[f] = j[f] = 0;
+      if (row < a.rows) {
+        if (dropping || !a.flat) a.walk.at(row, b[f], i[f], j[f]);
+        if (a.flat) {
+          up = a.update.flat(row);
+          rp = a.residual.flat(row);
+        } else {
+          up = a.update.row(b[f], i[f], j[f]);
+          rp = a.residual.row(b[f], i[f], j[f]);
+        }
       }
-      u[k] = pack<T>(f);
-      if (valid && v < a.octs) {
-        if (a.stream != nullptr) store_oct<kWide>(a.stream + out_row + v * 8, u[k], a.d - v * 8);
-        unpack(u[k], f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss[0] += (kWide || v * 8 + e < a.d) ? f[e] * f[e] : 0.f;
+      for (int k = 0; k < kUnits; ++k) {
+        const int n = lane + k * kGroup;
+        const bool on = row < a.rows && n < units;
+        u[f][k] = on ? load_unit<T, kU>(up + n * kU) : zero_unit<T, kU>();
+        r[f][k] = on && has_residual ? load_unit<T, kU>(rp + n * kU) : zero_unit<T, kU>();
       }
     }
-    group_sum<kGroup, 1>(ss, sums, parity);
-    const float rstd = rsqrtf(ss[0] / static_cast<float>(a.d) + a.eps);
+
+    float ss[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const uint32_t row = first + f * span + threadIdx.x / kGroup;
+      if (dropping) {
+        if constexpr (kU == 8) {
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) {
+            Vals<8> v = unpack(u[f][k]);
+            drop_oct(draw_oct(drop, b[f], i[f], j[f], lane + k * kGroup), line, drop.gain, v);
+            const Vals<8> x = unpack(r[f][k]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
+            u[f][k] = pack<T, 8>(v);
+          }
+        } else {
+          const auto mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b[f], i[f], j[f], lane & ~31, a.octs);
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) {
+            const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
+            Vals<kU> v = unpack(u[f][k]);
+            v.p[0].x = bits & 1u ? v.p[0].x * drop.gain : 0.f;
+            if constexpr (kU > 1) v.p[0].y = bits & 2u ? v.p[0].y * drop.gain : 0.f;
+            const Vals<kU> x = unpack(r[f][k]);
+            v.p[0] = __fadd2_rn(v.p[0], x.p[0]);
+            u[f][k] = pack<T, kU>(v);
+          }
+        }
+      } else if (has_residual) {
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) u[f][k] = add_units(u[f][k], r[f][k]);
+      }
+      if (a.stream != nullptr && row < a.rows) {
+        T* zp = a.stream + static_cast<int64_t>(row) * a.d;
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k)
+          if (lane + k * kGroup < units) store_unit<T, kU>(zp + (lane + k * kGroup) * kU, u[f][k]);
+      }
+      if constexpr (kMode != kAdd) {
+        float2 s = both(0.f);
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+          const Vals<kU> v = unpack(u[f][k]);
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) s = __ffma2_rn(v.p[e], v.p[e], s);
+        }
+        ss[f] = s.x + s.y;
+      }
+    }
+    if constexpr (kMode == kAdd) continue;
+    group_sum<kGroup, kFlight>(ss, sums, parity);
 
     if constexpr (kMode == kNorm) {
-      T* yp = static_cast<T*>(a.y) + out_row;
 #pragma unroll
-      for (int k = 0; k < kOcts; ++k) {
-        const int v = lane + k * kGroup;
-        float f[8];
-        unpack(u[k], f);
+      for (int f = 0; f < kFlight; ++f) {
+        const uint32_t row = first + f * span + threadIdx.x / kGroup;
+        if (row >= a.rows) break;
+        const float2 rstd = both(rsqrtf(ss[f] * a.inv_d + a.eps));
+        T* yp = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.d;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] *= rstd * w[k][e];
-        if (valid && v < a.octs) store_oct<kWide>(yp + v * 8, pack<T>(f), a.d - v * 8);
+        for (int k = 0; k < kUnits; ++k) {
+          Vals<kU> v = unpack(u[f][k]);
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) v.p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
+          if (lane + k * kGroup < units) store_unit<T, kU>(yp + (lane + k * kGroup) * kU, pack<T, kU>(v));
+        }
       }
-    } else {
-      uint8_t* yp = static_cast<uint8_t*>(a.y) + out_row;
-      float top[kOcts];
+    } else if constexpr (kMode == kNormE4m3) {
+      const bool whole = a.group == a.d;
+      const int per = a.group / 8;  // octs per scale; 4, 8 or 16 unless the whole row has one (the only form of narrow units)
+      float top[kFlight][kUnits];
+      Vals<kU> y[kFlight][kUnits];
 #pragma unroll
-      for (int k = 0; k < kOcts; ++k) {
-        const int v = lane + k * kGroup;
-        float f[8];
-        unpack(u[k], f);
-        top[k] = 0.f;
+      for (int f = 0; f < kFlight; ++f) {
+        const float2 rstd = both(rsqrtf(ss[f] * a.inv_d + a.eps));
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (kWide || v * 8 + e < a.d) top[k] = fmaxf(top[k], fabsf(f[e] * (rstd * w[k][e])));
+        for (int k = 0; k < kUnits; ++k) {
+          const Vals<kU> v = unpack(u[f][k]);
+          top[f][k] = 0.f;
+#pragma unroll
+          for (int e = 0; e < kPairs; ++e) {
+            y[f][k].p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
+            top[f][k] = fmaxf(top[f][k], fmaxf(fabsf(y[f][k].p[e].x), fabsf(y[f][k].p[e].y)));
+          }
+        }
       }
-      const int per = a.group >> 3;  // octs per scale
-      if (a.group == a.d) {
-        float m = 0.f;
+      if (whole) {
+        float m[kFlight];
 #pragma unroll
-        for (int k = 0; k < kOcts; ++k) m = fmaxf(m, top[k]);
-        m = group_max<kGroup>(m, tops, parity);
+        for (int f = 0; f < kFlight; ++f) {
+          m[f] = top[f][0];
 #pragma unroll
-        for (int k = 0; k < kOcts; ++k) top[k] = m;
+          for (int k = 1; k < kUnits; ++k) m[f] = fmaxf(m[f], top[f][k]);
+        }
+        group_max<kGroup, kFlight>(m, tops, parity);
+#pragma unroll
+        for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) top[f][k] = m[f];
       } else {
-        // a group of 32, 64 or 128 channels is 4, 8 or 16 neighbouring lanes
+        // 32, 64 or 128 channels are 4, 8 or 16 neighbouring lanes
         for (int o = 1; o < per; o <<= 1)
 #pragma unroll
-          for (int k = 0; k < kOcts; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+          for (int f = 0; f < kFlight; ++f)
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) top[f][k] = fmaxf(top[f][k], __shfl_xor_sync(0xffffffffu, top[f][k], o));
       }
 #pragma unroll
-      for (int k = 0; k < kOcts; ++k) {
-        const int v = lane + k * kGroup;
-        const float scale = top[k] > 0.f ? fmaxf(top[k] / kE4m3Max, 1.17549435e-38f) : 1.f;
-        if (valid && v < a.octs) {
-          if (a.group == a.d) {
-            if (v == 0) a.scales[row] = scale;
-          } else if (v % per == 0) {
-            a.scales[static_cast<int64_t>(row) * (a.d / a.group) + v / per] = scale;
-          }
-          const float inv = 1.f / scale;
-          float f[8];
-          unpack(u[k], f);
+      for (int f = 0; f < kFlight; ++f) {
+        const uint32_t row = first + f * span + threadIdx.x / kGroup;
+        if (row >= a.rows) break;
+        uint8_t* yp = static_cast<uint8_t*>(a.y) + static_cast<int64_t>(row) * a.d;
+        float* sp = a.scales + static_cast<int64_t>(row) * (whole ? 1 : a.d / a.group);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= rstd * w[k][e];
-          uint2 q;
-          q.x = e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
-          q.y = e4m3x2(f[4] * inv, f[5] * inv) | (e4m3x2(f[6] * inv, f[7] * inv) << 16);
-          if constexpr (kWide) {
-            __stcs(reinterpret_cast<uint2*>(yp + v * 8), q);
+        for (int k = 0; k < kUnits; ++k) {
+          const int n = lane + k * kGroup;
+          if (n >= units) continue;
+          const float scale = top[f][k] > 0.f ? fmaxf(top[f][k] * (1.f / kE4m3Max), 1.17549435e-38f) : 1.f;
+          if (whole ? n == 0 : n % per == 0) sp[whole ? 0 : n / per] = scale;
+          const float2 inv = both(1.f / scale);
+          if constexpr (kU == 8) {
+            uint32_t q[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[e] = e4m3x2(__fmul2_rn(y[f][k].p[e], inv));
+            __stcs(reinterpret_cast<uint2*>(yp + n * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
           } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (v * 8 + e < a.d) yp[v * 8 + e] = static_cast<uint8_t>((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+            const uint32_t q = e4m3x2(__fmul2_rn(y[f][k].p[0], inv));
+            if constexpr (kU == 2)
+              *reinterpret_cast<uint16_t*>(yp + n * 2) = static_cast<uint16_t>(q);
+            else
+              yp[n] = static_cast<uint8_t>(q);
           }
         }
       }
@@ -170,65 +242,114 @@ __global__ void __launch_bounds__(kThreads) add_norm_kernel(const __grid_constan
   }
 }
 
-// The addition alone: no reduction, one oct per thread and step.
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(kThreads) add_kernel(const __grid_constant__ NormArgs<T> a, const FastDiv by_octs) {
+// The addition alone, of whole octs: no reduction, kFlight octs per thread and step.
+template <typename T, int kFlight>
+__global__ void __launch_bounds__(kThreads) add_octs_kernel(const __grid_constant__ NormArgs<T> a, const FastDiv by_octs) {
   Dropout drop = a.drop;
-  if (drop.keep < 65536u) resolve_seed(drop);
+  const bool dropping = drop.keep < 65536u;
+  const bool has_residual = a.residual.p != nullptr;
+  const uint32_t line = drop.keep << 16;
+  if (dropping) resolve_seed(drop);
   const int64_t total = static_cast<int64_t>(a.rows) * a.octs;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kThreads;
-  for (int64_t n = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; n < total; n += step) {
-    uint32_t row, v;
-    if (total <= 0x7fffffff) {
-      row = by_octs.div(static_cast<uint32_t>(n));
-      v = static_cast<uint32_t>(n) - row * by_octs.d;
-    } else {
-      row = static_cast<uint32_t>(n / a.octs);
-      v = static_cast<uint32_t>(n - static_cast<int64_t>(row) * a.octs);
-    }
-    uint32_t b, i, j;
-    a.walk.at(row, b, i, j);
-    const int left = a.d - static_cast<int>(v) * 8;
-    const Oct<T> u = load_oct<kWide>(a.update.row(b, i, j) + v * 8, left);
-    Oct<T> r;
-    if (a.residual.p != nullptr) r = load_oct<kWide>(a.residual.row(b, i, j) + v * 8, left);
-    float f[8], g[8];
-    unpack(u, f);
-    if (drop.keep < 65536u) apply_dropout(drop, b, i, j, v, f);
-    if (a.residual.p != nullptr) {
-      unpack(r, g);
+  const int64_t span = static_cast<int64_t>(gridDim.x) * kThreads;
+  for (int64_t n0 = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; n0 < total; n0 += kFlight * span) {
+    Unit<T, 8> u[kFlight], r[kFlight];
+    uint32_t b[kFlight], i[kFlight], j[kFlight], oct[kFlight];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] += g[e];
+    for (int f = 0; f < kFlight; ++f) {
+      const int64_t n = n0 + f * span;
+      if (n < total) {
+        uint32_t row;
+        if (total <= 0x7fffffff) {
+          row = by_octs.div(static_cast<uint32_t>(n));
+          oct[f] = static_cast<uint32_t>(n) - row * by_octs.d;
+        } else {
+          row = static_cast<uint32_t>(n / a.octs);
+          oct[f] = static_cast<uint32_t>(n - static_cast<int64_t>(row) * a.octs);
+        }
+        if (dropping || !a.flat) a.walk.at(row, b[f], i[f], j[f]);
+        u[f] = load_unit<T, 8>((a.flat ? a.update.flat(row) : a.update.row(b[f], i[f], j[f])) + oct[f] * 8);
+        if (has_residual) r[f] = load_unit<T, 8>((a.flat ? a.residual.flat(row) : a.residual.row(b[f], i[f], j[f])) + oct[f] * 8);
+      }
     }
-    store_oct<kWide>(a.stream + static_cast<int64_t>(row) * a.d + v * 8, pack<T>(f), left);
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      const int64_t n = n0 + f * span;
+      if (n >= total) break;
+      if (dropping) {
+        Vals<8> v = unpack(u[f]);
+        drop_oct(draw_oct(drop, b[f], i[f], j[f], oct[f]), line, drop.gain, v);
+        if (has_residual) {
+          const Vals<8> x = unpack(r[f]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
+        }
+        u[f] = pack<T, 8>(v);
+      } else if (has_residual) {
+        u[f] = add_units(u[f], r[f]);
+      }
+      store_unit<T, 8>(a.stream + n * 8, u[f]);
+    }
   }
 }
 
-template <typename T, int kGroup, int kOcts, bool kWide, int kMode>
-cudaError_t launch(const NormArgs<T>& a, int sms, cudaStream_t stream) {
-  constexpr uint32_t kRows = kThreads / kGroup;
-  const uint32_t need = (a.rows + kRows - 1) / kRows;
-  const uint32_t most = static_cast<uint32_t>(sms) * 8;
-  add_norm_kernel<T, kGroup, kOcts, kWide, kMode><<<need < most ? need : most, kThreads, 0, stream>>>(a);
+template <typename T>
+cudaError_t launch_add(const NormArgs<T>& a, int sms, cudaStream_t s) {
+  constexpr int kFlight = sizeof(T) == 2 ? 2 : 1;
+  const int64_t total = static_cast<int64_t>(a.rows) * a.octs;
+  const int64_t need = (total + kThreads - 1) / kThreads, most = static_cast<int64_t>(sms) * 8;
+  add_octs_kernel<T, kFlight><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, make_fast_div(a.octs));
   return cudaGetLastError();
 }
 
-template <typename T, bool kWide, int kMode>
-cudaError_t by_width(const NormArgs<T>& a, int sms, cudaStream_t s) {
+template <typename T, int kU, int kGroup, int kUnits, int kFlight, int kMode>
+cudaError_t launch(const NormArgs<T>& a, int sms, cudaStream_t stream) {
+  constexpr uint32_t kWide = threads_of(kGroup), kRows = kWide / kGroup;
+  const uint32_t need = (a.rows + kRows - 1) / kRows;
+  const uint32_t most = static_cast<uint32_t>(sms) * (2048 / kWide);
+  add_norm_kernel<T, kU, kGroup, kUnits, kFlight, kMode><<<need < most ? need : most, kWide, 0, stream>>>(a);
+  return cudaGetLastError();
+}
+
+// Octs: two rows in flight where a lane has one 16-byte oct of each.
+template <typename T, int kMode>
+cudaError_t wide_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
+  constexpr int kTwo = sizeof(T) == 2 ? 2 : 1;
   const int o = a.octs;
-  if (o <= 8) return launch<T, 8, 1, kWide, kMode>(a, sms, s);
-  if (o <= 16) return launch<T, 16, 1, kWide, kMode>(a, sms, s);
-  if (o <= 32) return launch<T, 32, 1, kWide, kMode>(a, sms, s);
-  if (o <= 64) return launch<T, 32, 2, kWide, kMode>(a, sms, s);
-  if (o <= 128) return launch<T, 32, 4, kWide, kMode>(a, sms, s);
-  if (o <= 256) return launch<T, 256, 1, kWide, kMode>(a, sms, s);
-  if (o <= 512) return launch<T, 256, 2, kWide, kMode>(a, sms, s);
-  return launch<T, 256, 4, kWide, kMode>(a, sms, s);
+  if (o <= 8) return launch<T, 8, 8, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 16) return launch<T, 8, 16, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 32) return launch<T, 8, 32, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 64) return launch<T, 8, 32, 2, 1, kMode>(a, sms, s);
+  if (o <= 128) return launch<T, 8, 128, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 256) return launch<T, 8, 256, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 512) return launch<T, 8, 512, 1, kTwo, kMode>(a, sms, s);
+  return launch<T, 8, 1024, 1, kTwo, kMode>(a, sms, s);
+}
+
+// Units of one or two channels: four or eight channels per lane of a warp, then of a CTA.
+template <typename T, int kU, int kMode>
+cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
+  if (a.d <= 128) return launch<T, kU, 32, 4 / kU, 2, kMode>(a, sms, s);
+  if (a.d <= 256) return launch<T, kU, 32, 8 / kU, 1, kMode>(a, sms, s);
+  if (a.d <= 512) return launch<T, kU, 128, 4 / kU, 2, kMode>(a, sms, s);
+  if (a.d <= 1024) return launch<T, kU, 256, 4 / kU, 2, kMode>(a, sms, s);
+  if (a.d <= 2048) return launch<T, kU, 512, 4 / kU, 2, kMode>(a, sms, s);
+  if (a.d <= 4096) return launch<T, kU, 1024, 4 / kU, 2, kMode>(a, sms, s);
+  return launch<T, kU, 1024, 8 / kU, 1, kMode>(a, sms, s);
+}
+
+template <typename T, int kMode>
+cudaError_t by_unit(const NormArgs<T>& a, int unit, int sms, cudaStream_t s) {
+  if constexpr (kMode != kAdd)
+    if (unit == 8) return wide_rows<T, kMode>(a, sms, s);
+  if constexpr (sizeof(T) == 2)
+    if (unit == 2) return narrow_rows<T, 2, kMode>(a, sms, s);
+  return narrow_rows<T, 1, kMode>(a, sms, s);
 }
 
 template <typename T>
 cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* update, const pair_tensor_t* residual, const void* weight,
-                void* stream, void* y, float* scales, int sms, cudaStream_t s) {
+                void* stream, void* y, float* scales, int unit, int sms, cudaStream_t s) {
   NormArgs<T> a;
   a.update = strided<T>(update);
   a.residual = strided<T>(residual);
@@ -243,22 +364,12 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* update, const pa
   a.octs = (d->d + 7) / 8;
   a.weight_dtype = d->weight_dtype;
   a.group = d->group;
+  a.flat = collapses(update, d->b, d->i, d->j) && collapses(residual, d->b, d->i, d->j);
   a.eps = d->eps;
-  const bool wide = d->d % 8 == 0 && rows_aligned(update, sizeof(T)) && rows_aligned(residual, sizeof(T)) &&
-                    aligned16(stream) && aligned16(y);
-  if (y == nullptr) {
-    const int64_t total = static_cast<int64_t>(a.rows) * a.octs;
-    const int64_t need = (total + kThreads - 1) / kThreads, most = static_cast<int64_t>(sms) * 8;
-    const unsigned grid = static_cast<unsigned>(need < most ? need : most);
-    const FastDiv by_octs = make_fast_div(a.octs);
-    if (wide)
-      add_kernel<T, true><<<grid, kThreads, 0, s>>>(a, by_octs);
-    else
-      add_kernel<T, false><<<grid, kThreads, 0, s>>>(a, by_octs);
-    return cudaGetLastError();
-  }
-  if (d->group != 0) return wide ? by_width<T, true, kNormE4m3>(a, sms, s) : by_width<T, false, kNormE4m3>(a, sms, s);
-  return wide ? by_width<T, true, kNorm>(a, sms, s) : by_width<T, false, kNorm>(a, sms, s);
+  a.inv_d = 1.f / static_cast<float>(d->d);
+  if (y == nullptr && unit == 8) return launch_add<T>(a, sms, s);
+  if (y == nullptr) return by_unit<T, kAdd>(a, unit, sms, s);
+  return d->group != 0 ? by_unit<T, kNormE4m3>(a, unit, sms, s) : by_unit<T, kNorm>(a, unit, sms, s);
 }
 
 }  // namespace
@@ -317,15 +428,20 @@ extern "C" int pair_sm100_add_norm(const pair_norm_desc_t* desc, const pair_tens
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: an e4m3 output needs y and scales", who);
   if (update == nullptr || update->data == nullptr)
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: update is NULL", who);
+  const int size = type_bytes(desc->dtype);
+  const int unit = unit_of(desc->d, size, {update, residual}, {stream, g == 0 ? y : nullptr});
+  if (g != 0 && g != desc->d && (unit != 8 || !aligned(y, 8)))
+    return report_error(TRIMUL_ERR_UNSUPPORTED_SHAPE, "%s: scales per group need rows that start on 16-byte boundaries", who);
+  if (g != 0 && !aligned(y, unit)) return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: an e4m3 output starts on an 8-byte boundary", who);
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   cudaError_t e;
   if (desc->dtype == PAIR_FP32)
-    e = run<float>(desc, update, residual, weight, stream, y, scales, sms, cuda_stream);
+    e = run<float>(desc, update, residual, weight, stream, y, scales, unit, sms, cuda_stream);
   else if (desc->dtype == PAIR_FP16)
-    e = run<__half>(desc, update, residual, weight, stream, y, scales, sms, cuda_stream);
+    e = run<__half>(desc, update, residual, weight, stream, y, scales, unit, sms, cuda_stream);
   else
-    e = run<__nv_bfloat16>(desc, update, residual, weight, stream, y, scales, sms, cuda_stream);
+    e = run<__nv_bfloat16>(desc, update, residual, weight, stream, y, scales, unit, sms, cuda_stream);
   if (e != cudaSuccess) return report_error(TRIMUL_ERR_CUDA, "%s: %s", who, cudaGetErrorString(e));
   return TRIMUL_OK;
 }

@@ -30,110 +30,130 @@ struct GradArgs {
   uint32_t rows;
   int d, octs;
   int weight_dtype;
-  float eps;
+  int flat;  // the rows of z, dy and dz lie at a constant distance
+  float eps, inv_d;
 };
 
-template <typename T, int kGroup, int kOcts, bool kWide>
-__global__ void __launch_bounds__(kThreads) norm_grad_kernel(const __grid_constant__ GradArgs<T> a) {
-  __shared__ float sums[2 * 8 * 2];
-  extern __shared__ double fold[];  // [oct of the lane][channel of the oct][thread]
-  constexpr int kRows = kThreads / kGroup;
+// As add_norm_kernel: kU channels per access, kGroup lanes per row, kUnits units per lane.
+template <typename T, int kU, int kGroup, int kUnits>
+__global__ void __launch_bounds__(threads_of(kGroup)) norm_grad_kernel(const __grid_constant__ GradArgs<T> a) {
+  __shared__ float sums[2 * 32 * 2];
+  extern __shared__ double fold[];  // [unit of the lane][channel of the unit][thread]
+  constexpr int kWide = threads_of(kGroup);
+  constexpr int kRows = kWide / kGroup;
+  constexpr int kPairs = (kU + 1) / 2;
   const int lane = threadIdx.x % kGroup;
+  const int units = a.d / kU;
+  const bool dropping = a.drop.keep < 65536u && a.d_update != nullptr;
+  const uint32_t line = a.drop.keep << 16;
   Dropout drop = a.drop;
-  if (drop.keep < 65536u) resolve_seed(drop);
+  if (dropping) resolve_seed(drop);
 
-  float w[kOcts][8], dw[kOcts][8];
+  Vals<kU> w[kUnits], dw[kUnits];
 #pragma unroll
-  for (int k = 0; k < kOcts; ++k)
+  for (int k = 0; k < kUnits; ++k) {
+    float f[kPairs * 2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const int c = (lane + k * kGroup) * 8 + e;
-      w[k][e] = c < a.d ? load_any(a.weight, c, a.weight_dtype) : 0.f;
-      dw[k][e] = 0.f;
-      if (a.partial != nullptr) fold[(k * 8 + e) * kThreads + threadIdx.x] = 0.0;
+    for (int e = 0; e < kPairs * 2; ++e) {
+      const int n = lane + k * kGroup;
+      f[e] = n < units && e < kU ? load_any(a.weight, n * kU + e, a.weight_dtype) : 0.f;
+      if (e < kU && a.partial != nullptr) fold[(k * kU + e) * kWide + threadIdx.x] = 0.0;
     }
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) {
+      w[k].p[e] = make_float2(f[2 * e], f[2 * e + 1]);
+      dw[k].p[e] = both(0.f);
+    }
+  }
+  auto carry = [&] {
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k)
+#pragma unroll
+      for (int e = 0; e < kU; ++e) {
+        fold[(k * kU + e) * kWide + threadIdx.x] += e & 1 ? dw[k].p[e / 2].y : dw[k].p[e / 2].x;
+        (e & 1 ? dw[k].p[e / 2].y : dw[k].p[e / 2].x) = 0.f;
+      }
+  };
 
-  const float inv_d = 1.f / static_cast<float>(a.d);
   int parity = 0, held = 0;
   for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += gridDim.x * kRows, parity ^= 1) {
     const uint32_t row = first + threadIdx.x / kGroup;
     const bool valid = row < a.rows;
-    uint32_t b, i, j;
-    a.walk.at(valid ? row : 0, b, i, j);
-    const T* zp = a.z.row(b, i, j);
-    const T* yp = a.dy.p != nullptr ? a.dy.row(b, i, j) : nullptr;
-    const T* gp = a.dz.p != nullptr ? a.dz.row(b, i, j) : nullptr;
+    uint32_t b = 0, i = 0, j = 0;
+    if (valid && (dropping || !a.flat)) a.walk.at(row, b, i, j);
+    const T* zp = a.flat ? a.z.flat(row) : a.z.row(b, i, j);
+    const T* yp = a.flat ? a.dy.flat(row) : a.dy.row(b, i, j);
+    const T* gp = a.flat ? a.dz.flat(row) : a.dz.row(b, i, j);
 
-    Oct<T> z[kOcts], dy[kOcts], dz[kOcts];
+    Unit<T, kU> z[kUnits], dy[kUnits], dz[kUnits];
 #pragma unroll
-    for (int k = 0; k < kOcts; ++k) {
-      const int v = lane + k * kGroup;
-      const bool on = valid && v < a.octs;
-      z[k] = on ? load_oct<kWide>(zp + v * 8, a.d - v * 8) : zero_oct<T>();
-      dy[k] = on && yp != nullptr ? load_oct<kWide>(yp + v * 8, a.d - v * 8) : zero_oct<T>();
-      dz[k] = on && gp != nullptr ? load_oct<kWide>(gp + v * 8, a.d - v * 8) : zero_oct<T>();
+    for (int k = 0; k < kUnits; ++k) {
+      const int n = lane + k * kGroup;
+      const bool on = valid && n < units;
+      z[k] = on ? load_unit<T, kU>(zp + n * kU) : zero_unit<T, kU>();
+      dy[k] = on && a.dy.p != nullptr ? load_unit<T, kU>(yp + n * kU) : zero_unit<T, kU>();
+      dz[k] = on && a.dz.p != nullptr ? load_unit<T, kU>(gp + n * kU) : zero_unit<T, kU>();
     }
 
-    float s[2] = {0.f, 0.f};
+    float2 zz = both(0.f), tz = both(0.f);
 #pragma unroll
-    for (int k = 0; k < kOcts; ++k) {
-      float fz[8], fy[8];
-      unpack(z[k], fz);
-      unpack(dy[k], fy);
+    for (int k = 0; k < kUnits; ++k) {
+      const Vals<kU> vz = unpack(z[k]), vy = unpack(dy[k]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        s[0] += fz[e] * fz[e];
-        s[1] += fy[e] * w[k][e] * fz[e];
+      for (int e = 0; e < kPairs; ++e) {
+        zz = __ffma2_rn(vz.p[e], vz.p[e], zz);
+        tz = __ffma2_rn(__fmul2_rn(vy.p[e], w[k].p[e]), vz.p[e], tz);
       }
     }
+    float s[2] = {zz.x + zz.y, tz.x + tz.y};
     group_sum<kGroup, 2>(s, sums, parity);
-    const float rstd = rsqrtf(s[0] * inv_d + a.eps);
+    const float rstd = rsqrtf(s[0] * a.inv_d + a.eps);
     // in this order a row of zeros gives 0 even where rstd^3 would overflow
-    const float back = rstd * (rstd * (rstd * (s[1] * inv_d)));
+    const float back = -rstd * (rstd * (rstd * (s[1] * a.inv_d)));
     const int64_t out_row = static_cast<int64_t>(row) * a.d;
+    NarrowMask<kU < 8 ? kU : 1, kUnits> mask;
+    if constexpr (kU < 8)
+      if (dropping) mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b, i, j, lane & ~31, a.octs);
 
 #pragma unroll
-    for (int k = 0; k < kOcts; ++k) {
-      const int v = lane + k * kGroup;
-      float fz[8], fy[8], g[8];
-      unpack(z[k], fz);
-      unpack(dy[k], fy);
-      unpack(dz[k], g);
+    for (int k = 0; k < kUnits; ++k) {
+      const int n = lane + k * kGroup;
+      const bool on = valid && n < units;
+      const Vals<kU> vz = unpack(z[k]), vy = unpack(dy[k]);
+      Vals<kU> g = unpack(dz[k]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        g[e] += rstd * (w[k][e] * fy[e]) - fz[e] * back;
-        dw[k][e] += valid ? fy[e] * (fz[e] * rstd) : 0.f;
+      for (int e = 0; e < kPairs; ++e) {
+        const float2 y = __fmul2_rn(vy.p[e], both(rstd));
+        g.p[e] = __ffma2_rn(vz.p[e], both(back), __ffma2_rn(w[k].p[e], y, g.p[e]));
+        dw[k].p[e] = __ffma2_rn(vz.p[e], y, dw[k].p[e]);
       }
-      if (valid && v < a.octs) {
-        if (a.d_stream != nullptr) store_oct<kWide>(a.d_stream + out_row + v * 8, pack<T>(g), a.d - v * 8);
-        if (a.d_update != nullptr) {
-          if (drop.keep < 65536u) apply_dropout(drop, b, i, j, v, g);
-          store_oct<kWide>(a.d_update + out_row + v * 8, pack<T>(g), a.d - v * 8);
+      if (on && a.d_stream != nullptr) store_unit<T, kU>(a.d_stream + out_row + n * kU, pack<T, kU>(g));
+      if (a.d_update != nullptr) {
+        if (dropping) {
+          if constexpr (kU == 8) {
+            drop_oct(draw_oct(drop, b, i, j, n), line, drop.gain, g);
+          } else {
+            const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
+            g.p[0].x = bits & 1u ? g.p[0].x * drop.gain : 0.f;
+            if constexpr (kU > 1) g.p[0].y = bits & 2u ? g.p[0].y * drop.gain : 0.f;
+          }
         }
+        if (on) store_unit<T, kU>(a.d_update + out_row + n * kU, pack<T, kU>(g));
       }
     }
     if (a.partial != nullptr && ++held == kFold) {
       held = 0;
-#pragma unroll
-      for (int k = 0; k < kOcts; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          fold[(k * 8 + e) * kThreads + threadIdx.x] += dw[k][e];
-          dw[k][e] = 0.f;
-        }
+      carry();
     }
   }
 
   if (a.partial == nullptr) return;
-#pragma unroll
-  for (int k = 0; k < kOcts; ++k)
-#pragma unroll
-    for (int e = 0; e < 8; ++e) fold[(k * 8 + e) * kThreads + threadIdx.x] += dw[k][e];
+  carry();
   __syncthreads();
-  // channel c belongs to lane (c / 8) % kGroup, oct (c / 8) / kGroup of every row the CTA holds
-  for (int c = threadIdx.x; c < a.d; c += kThreads) {
-    const int v = c >> 3;
-    const double* f = fold + (v / kGroup * 8 + (c & 7)) * kThreads + v % kGroup;
+  // channel c is part of unit c / kU: lane (c / kU) % kGroup, unit (c / kU) / kGroup of every row the CTA holds
+  for (int c = threadIdx.x; c < a.d; c += kWide) {
+    const int n = c / kU;
+    const double* f = fold + (n / kGroup * kU + c % kU) * kWide + n % kGroup;
     double sum = 0.0;
 #pragma unroll
     for (int r = 0; r < kRows; ++r) sum += f[r * kGroup];
@@ -141,68 +161,87 @@ __global__ void __launch_bounds__(kThreads) norm_grad_kernel(const __grid_consta
   }
 }
 
-// d_w[c] = sum over the CTAs' sums: 32 channels per CTA, eight rows of sums at a time.
-__global__ void __launch_bounds__(kThreads) join_weight_kernel(const double* partial, int parts, int d, void* d_weight,
-                                                               int dtype) {
-  __shared__ double s[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), y = threadIdx.x >> 5;
+// d_w[c] = sum over the CTAs' sums: 16 channels and 64 rows of sums per CTA, four rows of a thread in flight.
+constexpr int kJoinChannels = 16, kJoinRows = 64;
+__global__ void __launch_bounds__(kJoinChannels* kJoinRows) join_weight_kernel(const double* partial, int parts, int d,
+                                                                              void* d_weight, int dtype) {
+  __shared__ double s[kJoinRows][kJoinChannels + 1];
+  const int x = threadIdx.x % kJoinChannels, y = threadIdx.x / kJoinChannels;
+  const int c = blockIdx.x * kJoinChannels + x;
   double sum = 0.0;
-  if (c < d)
-    for (int p = y; p < parts; p += 8) sum += partial[static_cast<int64_t>(p) * d + c];
-  s[y][threadIdx.x & 31] = sum;
-  __syncthreads();
-  if (y == 0 && c < d) {
-    for (int k = 1; k < 8; ++k) sum += s[k][threadIdx.x & 31];
-    store_any(d_weight, c, dtype, static_cast<float>(sum));
+  if (c < d) {
+    const double* p = partial + c;
+#pragma unroll 4
+    for (int r = y; r < parts; r += kJoinRows) sum += p[static_cast<int64_t>(r) * d];
   }
+  s[y][x] = sum;
+#pragma unroll
+  for (int half = kJoinRows / 2; half > 0; half /= 2) {
+    __syncthreads();
+    if (y < half) s[y][x] += s[y + half][x];
+  }
+  if (y == 0 && c < d) store_any(d_weight, c, dtype, static_cast<float>(s[0][x]));
 }
 
-struct Width {
-  int group, octs;
+// Lanes per row and channels per lane, by unit (8, 2 or 1 channels) and width.
+struct Shape {
+  int group, channels;
 };
-inline Width width_of(int octs) {
-  if (octs <= 8) return {8, 1};
-  if (octs <= 16) return {16, 1};
-  if (octs <= 32) return {32, 1};
-  if (octs <= 64) return {32, 2};
-  if (octs <= 128) return {32, 4};
-  if (octs <= 256) return {256, 1};
-  if (octs <= 512) return {256, 2};
-  return {256, 4};
+inline Shape shape_of(int unit, int d) {
+  if (unit == 8) {
+    if (d <= 64) return {8, 8};
+    if (d <= 128) return {16, 8};
+    if (d <= 256) return {32, 8};
+    if (d <= 512) return {32, 16};
+    return {d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024, 8};
+  }
+  if (d <= 128) return {32, 4};
+  if (d <= 256) return {32, 8};
+  return {d <= 512 ? 128 : d <= 1024 ? 256 : d <= 2048 ? 512 : 1024, d <= 4096 ? 4 : 8};
 }
 
-// CTAs of the gradient kernel: what stays resident beside the shared sums (16, 32 or 64 KB a CTA), or one per row.
-inline uint32_t grid_of(uint32_t rows, int octs, int sms) {
-  const Width w = width_of(octs);
-  const uint32_t held = kThreads / w.group;
+// CTAs of the gradient kernel: what 64 registers a thread let be resident (half of that for 16 channels a lane), or one
+// per group of rows.
+inline uint32_t grid_of(uint32_t rows, Shape w, int sms) {
+  const uint32_t threads = threads_of(w.group), held = threads / w.group;
   const uint32_t need = (rows + held - 1) / held;
-  const uint32_t most = static_cast<uint32_t>(sms) * (w.octs == 1 ? 4 : w.octs == 2 ? 3 : 2);
+  const uint32_t most = static_cast<uint32_t>(sms) * ((w.channels == 16 ? 512 : 1024) / threads);
   return need < most ? need : most;
 }
 
-template <typename T, int kGroup, int kOcts, bool kWide>
+template <typename T, int kU, int kGroup, int kUnits>
 cudaError_t launch(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream) {
-  const int smem = a.partial != nullptr ? kOcts * 8 * kThreads * static_cast<int>(sizeof(double)) : 0;
+  constexpr int kWide = threads_of(kGroup);
+  const int smem = a.partial != nullptr ? kUnits * kU * kWide * static_cast<int>(sizeof(double)) : 0;
   if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, kGroup, kOcts, kWide>,
+    cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, kU, kGroup, kUnits>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
   }
-  norm_grad_kernel<T, kGroup, kOcts, kWide><<<grid, kThreads, smem, stream>>>(a);
+  norm_grad_kernel<T, kU, kGroup, kUnits><<<grid, kWide, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
-template <typename T, bool kWide>
-cudaError_t by_width(const GradArgs<T>& a, uint32_t grid, cudaStream_t s) {
-  const int o = a.octs;
-  if (o <= 8) return launch<T, 8, 1, kWide>(a, grid, s);
-  if (o <= 16) return launch<T, 16, 1, kWide>(a, grid, s);
-  if (o <= 32) return launch<T, 32, 1, kWide>(a, grid, s);
-  if (o <= 64) return launch<T, 32, 2, kWide>(a, grid, s);
-  if (o <= 128) return launch<T, 32, 4, kWide>(a, grid, s);
-  if (o <= 256) return launch<T, 256, 1, kWide>(a, grid, s);
-  if (o <= 512) return launch<T, 256, 2, kWide>(a, grid, s);
-  return launch<T, 256, 4, kWide>(a, grid, s);
+template <typename T, int kU>
+cudaError_t by_shape(const GradArgs<T>& a, Shape w, uint32_t grid, cudaStream_t s) {
+  if constexpr (kU == 8) {
+    if (w.group == 8) return launch<T, 8, 8, 1>(a, grid, s);
+    if (w.group == 16) return launch<T, 8, 16, 1>(a, grid, s);
+    if (w.group == 32 && w.channels == 8) return launch<T, 8, 32, 1>(a, grid, s);
+    if (w.group == 32) return launch<T, 8, 32, 2>(a, grid, s);
+    if (w.group == 128) return launch<T, 8, 128, 1>(a, grid, s);
+    if (w.group == 256) return launch<T, 8, 256, 1>(a, grid, s);
+    if (w.group == 512) return launch<T, 8, 512, 1>(a, grid, s);
+    return launch<T, 8, 1024, 1>(a, grid, s);
+  } else {
+    if (w.group == 32 && w.channels == 4) return launch<T, kU, 32, 4 / kU>(a, grid, s);
+    if (w.group == 32) return launch<T, kU, 32, 8 / kU>(a, grid, s);
+    if (w.group == 128) return launch<T, kU, 128, 4 / kU>(a, grid, s);
+    if (w.group == 256) return launch<T, kU, 256, 4 / kU>(a, grid, s);
+    if (w.group == 512) return launch<T, kU, 512, 4 / kU>(a, grid, s);
+    if (w.channels == 4) return launch<T, kU, 1024, 4 / kU>(a, grid, s);
+    return launch<T, kU, 1024, 8 / kU>(a, grid, s);
+  }
 }
 
 template <typename T>
@@ -223,14 +262,24 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* z, const pair_te
   a.d = d->d;
   a.octs = (d->d + 7) / 8;
   a.weight_dtype = d->weight_dtype;
+  a.flat = collapses(z, d->b, d->i, d->j) && collapses(dy, d->b, d->i, d->j) && collapses(dz, d->b, d->i, d->j);
   a.eps = d->eps;
-  const uint32_t grid = grid_of(a.rows, a.octs, sms);
-  const bool wide = d->d % 8 == 0 && rows_aligned(z, sizeof(T)) && rows_aligned(dy, sizeof(T)) &&
-                    rows_aligned(dz, sizeof(T)) && aligned16(d_stream) && aligned16(d_update);
-  cudaError_t e = wide ? by_width<T, true>(a, grid, s) : by_width<T, false>(a, grid, s);
+  a.inv_d = 1.f / static_cast<float>(d->d);
+  const int unit = unit_of(d->d, sizeof(T), {z, dy, dz}, {d_stream, d_update});
+  const Shape w = shape_of(unit, d->d);
+  const uint32_t grid = grid_of(a.rows, w, sms);
+  cudaError_t e = cudaSuccess;
+  if (unit == 8) {
+    e = by_shape<T, 8>(a, w, grid, s);
+  } else {
+    if constexpr (sizeof(T) == 2) {
+      if (unit == 2) e = by_shape<T, 2>(a, w, grid, s);
+    }
+    if (unit == 1) e = by_shape<T, 1>(a, w, grid, s);
+  }
   if (e != cudaSuccess || d_weight == nullptr) return e;
-  join_weight_kernel<<<(a.d + 31) / 32, kThreads, 0, s>>>(a.partial, static_cast<int>(grid), a.d, d_weight,
-                                                        d->weight_dtype);
+  join_weight_kernel<<<(a.d + kJoinChannels - 1) / kJoinChannels, kJoinChannels * kJoinRows, 0, s>>>(
+      a.partial, static_cast<int>(grid), a.d, d_weight, d->weight_dtype);
   return cudaGetLastError();
 }
 
@@ -245,7 +294,13 @@ extern "C" int pair_sm100_add_norm_grad_workspace(const pair_norm_desc_t* desc, 
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return trimul::report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   const uint32_t rows = static_cast<uint32_t>(desc->b) * desc->i * desc->j;
-  *bytes = static_cast<uint64_t>(grid_of(rows, (desc->d + 7) / 8, sms)) * desc->d * sizeof(double);
+  // the unit depends on addresses that are not known here: room for the largest grid
+  uint32_t most = 0;
+  for (int unit : {8, 2}) {
+    const uint32_t grid = grid_of(rows, shape_of(unit, desc->d), sms);
+    most = grid > most ? grid : most;
+  }
+  *bytes = static_cast<uint64_t>(most) * desc->d * sizeof(double);
   return TRIMUL_OK;
 }
 

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
 #include "../../include/pair_stream_sm100.h"
 
 namespace trimul {
@@ -16,8 +18,12 @@ int current_device_sms();
 namespace pair {
 
 // ---------------------------------------------------------------------------------------------
-// eight channels of one row
+// units: the channels that one memory access of a lane moves
 // ---------------------------------------------------------------------------------------------
+// Rows that start on 16-byte boundaries and have whole octs are moved in units of eight channels (16 bytes of a 16-bit
+// type, 32 of fp32).  All others are moved in units of two 16-bit channels where rows start on 4-byte boundaries, else of one
+// channel: a warp's accesses are then still contiguous, where eight-channel groups at odd addresses would make
+// each access of a warp touch every line of the row (131 fp16 channels, 80000 rows: 25 us against 9).
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -36,62 +42,107 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Raw storage of eight elements: 16 bytes for the 16-bit types, 32 for fp32.
-template <typename T>
-struct alignas(16) Oct {
-  T e[8];
+template <typename T, int kU>
+struct alignas(sizeof(T) * kU < 16 ? sizeof(T) * kU : 16) Unit {
+  T e[kU];
 };
 
-// `kWide`: the address is 16-byte aligned and all eight channels exist (one or two 16-byte accesses); otherwise the
-// first n channels are moved one by one.  Loads carry the streaming hint: every activation is read once.
-template <bool kWide, typename T>
-__device__ __forceinline__ Oct<T> load_oct(const T* p, int n) {
-  Oct<T> o;
-  if constexpr (kWide) {
+// Loads carry the streaming hint: every activation is read once.
+template <typename T, int kU>
+__device__ __forceinline__ Unit<T, kU> load_unit(const T* p) {
+  Unit<T, kU> o;
+  constexpr int kBytes = sizeof(T) * kU;
+  if constexpr (kBytes >= 16) {
     uint4* w = reinterpret_cast<uint4*>(&o);
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(o) / 16); ++k) w[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+    for (int k = 0; k < kBytes / 16; ++k) w[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+  } else if constexpr (kBytes == 4) {
+    *reinterpret_cast<uint32_t*>(&o) = __ldcs(reinterpret_cast<const uint32_t*>(p));
   } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) o.e[k] = k < n ? p[k] : from_f32<T>(0.f);
+    static_assert(kBytes == 2, "a unit is 2, 4, 16 or 32 bytes");
+    *reinterpret_cast<uint16_t*>(&o) = __ldcs(reinterpret_cast<const uint16_t*>(p));
   }
   return o;
 }
 
-template <bool kWide, typename T>
-__device__ __forceinline__ void store_oct(T* p, const Oct<T>& o, int n) {
-  if constexpr (kWide) {
+template <typename T, int kU>
+__device__ __forceinline__ void store_unit(T* p, const Unit<T, kU>& o) {
+  constexpr int kBytes = sizeof(T) * kU;
+  if constexpr (kBytes >= 16) {
     const uint4* w = reinterpret_cast<const uint4*>(&o);
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(o) / 16); ++k) __stcs(reinterpret_cast<uint4*>(p) + k, w[k]);
+    for (int k = 0; k < kBytes / 16; ++k) __stcs(reinterpret_cast<uint4*>(p) + k, w[k]);
+  } else if constexpr (kBytes == 4) {
+    __stcs(reinterpret_cast<uint32_t*>(p), *reinterpret_cast<const uint32_t*>(&o));
   } else {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) p[k] = o.e[k];
+    __stcs(reinterpret_cast<uint16_t*>(p), *reinterpret_cast<const uint16_t*>(&o));
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const Oct<T>& o, float (&f)[8]) {
+template <typename T, int kU>
+__device__ __forceinline__ Unit<T, kU> zero_unit() {
+  Unit<T, kU> o;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = to_f32(o.e[k]);
-}
-
-template <typename T>
-__device__ __forceinline__ Oct<T> pack(const float (&f)[8]) {
-  Oct<T> o;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) o.e[k] = from_f32<T>(f[k]);
+  for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(0.f);
   return o;
 }
 
-template <typename T>
-__device__ __forceinline__ Oct<T> zero_oct() {
-  Oct<T> o;
+// The fp32 values of a unit, in pairs for the packed fp32 instructions (one issue slot for two operations).
+template <int kU>
+struct Vals {
+  float2 p[(kU + 1) / 2];  // of a single channel, .y is 0
+};
+
+template <typename T, int kU>
+__device__ __forceinline__ Vals<kU> unpack(const Unit<T, kU>& o) {
+  Vals<kU> v;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) o.e[k] = from_f32<T>(0.f);
+  for (int k = 0; k < (kU + 1) / 2; ++k) {
+    v.p[k].x = to_f32(o.e[2 * k]);
+    v.p[k].y = 2 * k + 1 < kU ? to_f32(o.e[2 * k + 1 < kU ? 2 * k + 1 : 0]) : 0.f;
+  }
+  return v;
+}
+
+template <typename T, int kU>
+__device__ __forceinline__ Unit<T, kU> pack(const Vals<kU>& v) {
+  Unit<T, kU> o;
+  if constexpr (sizeof(T) == 2 && kU > 1) {
+#pragma unroll
+    for (int k = 0; k < kU / 2; ++k) {
+      if constexpr (__is_same(T, __half))
+        reinterpret_cast<__half2*>(&o)[k] = __float22half2_rn(v.p[k]);
+      else
+        reinterpret_cast<__nv_bfloat162*>(&o)[k] = __float22bfloat162_rn(v.p[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(k & 1 ? v.p[k / 2].y : v.p[k / 2].x);
+  }
   return o;
 }
+
+// a + b in the unit's type, rounded once: for 16-bit pairs the packed addition, which rounds the exact sum.
+template <typename T, int kU>
+__device__ __forceinline__ Unit<T, kU> add_units(const Unit<T, kU>& a, const Unit<T, kU>& b) {
+  Unit<T, kU> o;
+  if constexpr (sizeof(T) == 2 && kU > 1) {
+#pragma unroll
+    for (int k = 0; k < kU / 2; ++k) {
+      if constexpr (__is_same(T, __half))
+        reinterpret_cast<__half2*>(&o)[k] = __hadd2_rn(reinterpret_cast<const __half2*>(&a)[k], reinterpret_cast<const __half2*>(&b)[k]);
+      else
+        reinterpret_cast<__nv_bfloat162*>(&o)[k] =
+            __hadd2_rn(reinterpret_cast<const __nv_bfloat162*>(&a)[k], reinterpret_cast<const __nv_bfloat162*>(&b)[k]);
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(to_f32(a.e[k]) + to_f32(b.e[k]));
+  }
+  return o;
+}
+
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
 // One value of a tensor whose type is known at run time only (gains: read once per CTA).
 __device__ __forceinline__ float load_any(const void* p, int64_t at, int dtype) {
@@ -143,6 +194,8 @@ template <typename T>
 struct Strided {
   const T* p;
   int64_t sb, si, sj;
+  // rows of a tensor whose b, i and j axes collapse into one
+  __device__ __forceinline__ const T* flat(uint32_t row) const { return p + static_cast<int64_t>(row) * sj; }
   __device__ __forceinline__ const T* row(uint32_t b, uint32_t i, uint32_t j) const {
     return p + (static_cast<int64_t>(b) * sb + static_cast<int64_t>(i) * si + static_cast<int64_t>(j) * sj);
   }
@@ -152,6 +205,12 @@ template <typename T>
 inline Strided<T> strided(const pair_tensor_t* t) {
   if (t == nullptr) return Strided<T>{nullptr, 0, 0, 0};
   return Strided<T>{static_cast<const T*>(t->data), t->stride_b, t->stride_i, t->stride_j};
+}
+
+// Whether row * stride_j reaches every row.
+inline bool collapses(const pair_tensor_t* t, int bb, int ii, int jj) {
+  if (t == nullptr || t->data == nullptr) return true;
+  return (ii == 1 || t->stride_i == t->stride_j * jj) && (bb == 1 || t->stride_b == t->stride_j * jj * ii);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -208,78 +267,142 @@ __device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint32_t c2, u
   return make_uint4(c0, c1, c2, c3);
 }
 
-// A dropped element becomes 0 whatever it was (an infinity or NaN included): selected, not multiplied.
-__device__ __forceinline__ void apply_dropout(const Dropout& d, uint32_t b, uint32_t i, uint32_t j, uint32_t oct,
-                                              float (&f)[8]) {
+// The four words of oct `oct` (channels 8 oct ...) of position (b, i, j) of this block.
+__device__ __forceinline__ uint4 draw_oct(const Dropout& d, uint32_t b, uint32_t i, uint32_t j, uint32_t oct) {
   const uint32_t ci = d.shared == PAIR_SHARED_ROWS ? 0u : i + d.i0;
   const uint32_t cj = d.shared == PAIR_SHARED_COLUMNS ? 0u : j + d.j0;
-  const uint4 r = philox(((b + d.b0) << 16) | oct, cj, ci, d.offset, d.key0, d.key1);
+  return philox(((b + d.b0) << 16) | oct, cj, ci, d.offset, d.key0, d.key1);
+}
+
+// Dropout of the eight channels of an oct.  `line` is keep << 16: the high half of a word is below keep exactly when the
+// word is below that, the low half when the word shifted up is (keep is at most 65535 here).  A dropped element becomes
+// 0 whatever it was (an infinity or NaN included): it is selected, and what is kept is multiplied.
+__device__ __forceinline__ void drop_oct(const uint4 r, uint32_t line, float gain, Vals<8>& v) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    f[2 * k] = (w[k] & 0xffffu) < d.keep ? f[2 * k] * d.gain : 0.f;
-    f[2 * k + 1] = (w[k] >> 16) < d.keep ? f[2 * k + 1] * d.gain : 0.f;
+    v.p[k].x = (w[k] << 16) < line ? v.p[k].x : 0.f;
+    v.p[k].y = w[k] < line ? v.p[k].y : 0.f;
+    v.p[k] = __fmul2_rn(v.p[k], both(gain));
   }
+}
+
+// What an oct keeps, one bit per channel.
+__device__ __forceinline__ uint32_t keep_bits(const uint4 r, uint32_t line) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+  uint32_t bits = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    bits |= (((w[k] << 16) < line ? 1u : 0u) | (w[k] < line ? 2u : 0u)) << (2 * k);
+  return bits;
+}
+
+// Narrow units: unit n of a row lies in oct n kU / 8, so the lanes of a warp would draw every oct 8 / kU times.  Instead they
+// draw each oct of the warp's units once and hand the bits around.  `first` is the warp's first unit of step 0, step k begins
+// kStep units further; afterwards the bits of unit (first + lane + k kStep) come from `narrow_bits`.
+template <int kU, int kUnits>
+struct NarrowMask {
+  static constexpr int kPer = 4 * kU;                             // octs of a warp's 32 units
+  static constexpr int kSlots = (kUnits * kPer + 31) / 32;        // octs a lane draws
+  uint32_t bits[(kSlots + 3) / 4];
+};
+
+template <int kU, int kUnits, int kStep>
+__device__ __forceinline__ NarrowMask<kU, kUnits> draw_narrow(const Dropout& d, uint32_t line, uint32_t b, uint32_t i, uint32_t j,
+                                                              int first, int octs) {
+  NarrowMask<kU, kUnits> m;
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 0; s < (m.kSlots + 3) / 4; ++s) m.bits[s] = 0;
+#pragma unroll
+  for (int s = 0; s < m.kSlots; ++s) {
+    const int q = lane + 32 * s;
+    const int oct = (first + q / m.kPer * kStep) * kU / 8 + q % m.kPer;
+    if (q < kUnits * m.kPer && oct < octs) m.bits[s / 4] |= keep_bits(draw_oct(d, b, i, j, oct), line) << (8 * (s & 3));
+  }
+  return m;
+}
+
+// The bits of the lane's unit of step k, lowest channel first.  Every lane of the warp takes part.
+template <int kU, int kUnits>
+__device__ __forceinline__ uint32_t narrow_bits(const NarrowMask<kU, kUnits>& m, int k) {
+  const int lane = threadIdx.x & 31;
+  const int q = m.kPer * k + lane * kU / 8;  // kPer is 4 or 8, so all lanes share the slot q / 32
+  const int slot = m.kPer * k / 32;
+  const uint32_t byte = (__shfl_sync(0xffffffffu, m.bits[slot / 4], q & 31) >> (8 * (slot & 3))) & 0xffu;
+  return byte >> (lane * kU % 8);
 }
 
 // ---------------------------------------------------------------------------------------------
 // sums over the lanes that share a row
 // ---------------------------------------------------------------------------------------------
+// A row has kGroup lanes: 8, 16 or 32 of a warp, or a CTA of its own of 128 to 1024 threads.
 constexpr int kThreads = 256;
+__host__ __device__ constexpr int threads_of(int group) { return group <= 32 ? kThreads : group; }
 
-// kGroup <= 32: lanes of one warp; kGroup == kThreads: the CTA.  Every lane of the warp takes part, every lane gets
-// the result.  `buf` holds 2 x 8 x kN floats for the CTA form and alternates with `parity`, so one barrier per call
-// is enough: a warp can only be one call ahead of another.
-template <int kGroup, int kN>
-__device__ __forceinline__ void group_sum(float (&v)[kN], float* buf, int parity) {
+template <bool kMax>
+__device__ __forceinline__ float merge(float a, float b) { return kMax ? fmaxf(a, b) : a + b; }
+
+// Sums (or maxima) of kN values over the lanes of a row; every lane of the warp takes part, every lane gets the results.
+// `buf` holds 2 x 32 x kN floats for the CTA form and alternates with `parity`, so that one barrier per call is enough: a
+// warp that writes one half again has passed the barrier of the call between, and so have the readers of that half.
+template <int kGroup, int kN, bool kMax>
+__device__ __forceinline__ void group_merge(float (&v)[kN], float* buf, int parity) {
   constexpr int kLanes = kGroup < 32 ? kGroup : 32;
 #pragma unroll
   for (int o = kLanes / 2; o > 0; o >>= 1)
 #pragma unroll
-    for (int n = 0; n < kN; ++n) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+    for (int n = 0; n < kN; ++n) v[n] = merge<kMax>(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
   if constexpr (kGroup > 32) {
-    float* b = buf + parity * 8 * kN;
-    const int warp = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0)
+    constexpr int kWarps = kGroup / 32;
+    float* b = buf + parity * 32 * kN;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0)
 #pragma unroll
-      for (int n = 0; n < kN; ++n) b[warp * kN + n] = v[n];
+      for (int n = 0; n < kN; ++n) b[(threadIdx.x >> 5) * kN + n] = v[n];
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < kN; ++n) {
-      float s = 0.f;
+    for (int n = 0; n < kN; ++n) v[n] = b[(lane % kWarps) * kN + n];
 #pragma unroll
-      for (int w = 0; w < kThreads / 32; ++w) s += b[w * kN + n];
-      v[n] = s;
-    }
+    for (int o = kWarps / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int n = 0; n < kN; ++n) v[n] = merge<kMax>(v[n], __shfl_xor_sync(0xffffffffu, v[n], o));
   }
 }
 
-template <int kGroup>
-__device__ __forceinline__ float group_max(float v, float* buf, int parity) {
-  constexpr int kLanes = kGroup < 32 ? kGroup : 32;
-#pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if constexpr (kGroup > 32) {
-    float* b = buf + parity * 8;
-    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = b[0];
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, b[w]);
-  }
-  return v;
+template <int kGroup, int kN>
+__device__ __forceinline__ void group_sum(float (&v)[kN], float* buf, int parity) {
+  group_merge<kGroup, kN, false>(v, buf, parity);
+}
+template <int kGroup, int kN>
+__device__ __forceinline__ void group_max(float (&v)[kN], float* buf, int parity) {
+  group_merge<kGroup, kN, true>(v, buf, parity);
 }
 
 // Host-side checks shared by the entry points.
 int check_norm_desc(const pair_norm_desc_t* d, const char* who);
 int check_dtype(int dtype, const char* what, const char* who);
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-// every row of the tensor starts on a 16-byte boundary
-inline bool rows_aligned(const pair_tensor_t* t, int bytes) {
+inline bool aligned(const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+// every row of the tensor starts on a multiple of `bytes`
+inline bool rows_aligned(const pair_tensor_t* t, int type_size, int bytes) {
   if (t == nullptr || t->data == nullptr) return true;
-  const int64_t m = 16 / bytes;
-  return aligned16(t->data) && t->stride_b % m == 0 && t->stride_i % m == 0 && t->stride_j % m == 0;
+  const int64_t m = bytes / type_size;
+  return aligned(t->data, bytes) && t->stride_b % m == 0 && t->stride_i % m == 0 && t->stride_j % m == 0;
+}
+
+// Channels per memory access that every tensor of a call allows: 8, 2 (16-bit types) or 1.
+inline int unit_of(int d, int type_size, std::initializer_list<const pair_tensor_t*> strided, std::initializer_list<const void*> flat) {
+  auto fits = [&](int unit, int bytes) {
+    if (d % unit != 0) return false;
+    for (const pair_tensor_t* t : strided)
+      if (!rows_aligned(t, type_size, bytes)) return false;
+    for (const void* p : flat)
+      if (!aligned(p, bytes)) return false;
+    return true;
+  };
+  if (fits(8, 16)) return 8;
+  return type_size == 2 && fits(2, 4) ? 2 : 1;
 }
 
 }  // namespace pair

@@ -38,6 +38,7 @@ __all__ = ["PairDropout", "dropout_add", "add_rms_norm", "add_rms_norm_fp8", "pa
 
 _SHARED = {None: _lib.PAIR_SHARED_NONE, "rows": _lib.PAIR_SHARED_ROWS, "columns": _lib.PAIR_SHARED_COLUMNS}
 _BYTE = torch.uint8
+_PLAIN = frozenset((Tensor, torch.nn.Parameter, type(None)))
 _NO_DTENSOR_GRADIENT = "gradients through DTensors are not supported: pass the local blocks, with PairDropout.origin"
 
 
@@ -79,10 +80,10 @@ class PairDropout:
         """How many of 65536 values are kept."""
         return math.floor((1.0 - self.p) * 65536.0 + 0.5)
 
-    def _desc(self) -> _lib.PairDropoutDesc:
-        if isinstance(self.seed, Tensor):
-            return PK.dropout_desc(self.keep, 0, 0, _SHARED[self.shared], self.origin, self.seed)
-        return PK.dropout_desc(self.keep, self.seed, self.offset, _SHARED[self.shared], self.origin)
+    def _record(self) -> tuple:
+        on_device = isinstance(self.seed, Tensor)
+        return PK.dropout_record(self.keep, 0 if on_device else self.seed, self.offset, _SHARED[self.shared], self.origin,
+                                 self.seed if on_device else None)
 
 
 def pair_block_origin(x) -> Tuple[int, int, int]:
@@ -103,6 +104,8 @@ def _needs_grad(*tensors) -> bool:
 
 def _locals_of(names: Sequence[str], tensors: Sequence[Optional[Tensor]]):
     """The ranks' local blocks of DTensors that are sharded alike, and their :class:`_Wrap` (``None`` where all are plain)."""
+    if all(type(t) in _PLAIN for t in tensors):
+        return tensors, None
     given = [(n, t) for n, t in zip(names, tensors) if t is not None]
     if not any(_is_dtensor(t) for _, t in given):
         return tensors, None
@@ -163,15 +166,23 @@ def _check_overlap(out: Tensor, t: Optional[Tensor], name: str) -> None:
         raise ValueError(f"out overlaps {name} without being it")
 
 
-def _as_pair(t: Optional[Tensor], name: str) -> Optional[Tensor]:
-    """A four-dimensional view with contiguous channels."""
+def _as_pair(t: Optional[Tensor]) -> Optional[Tensor]:
+    """A four-dimensional view with contiguous channels (a copy where they are not)."""
     if t is None:
         return None
-    if not 1 <= t.dim() <= 4:
-        raise ValueError(f"{name} must have one to four dims, (B, N_i, N_j, D) or its last ones; got {tuple(t.shape)}")
     if t.stride(-1) != 1 and t.shape[-1] != 1:
         t = t.contiguous()
     return t if t.dim() == 4 else t[(None,) * (4 - t.dim())]
+
+
+def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:
+    """``t``, or a copy of it where its rows do not start on 16-byte boundaries."""
+    if t is None:
+        return None
+    unit = 16 // t.element_size()
+    if t.data_ptr() % 16 == 0 and all(s % unit == 0 for s in t.stride()[:-1]) and (t.stride(-1) == 1 or t.shape[-1] == 1):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_pair(update: Tensor, residual: Optional[Tensor]) -> None:
@@ -201,104 +212,122 @@ def _check_weight(weight: Tensor, update: Tensor, eps: float) -> None:
         raise ValueError(f"eps must be a normal float32 number > 0; got {eps}")
 
 
-class _on:
-    """Makes a tensor's device current where it is not."""
+def _elsewhere(device: torch.device):
+    """A context that makes ``device`` current, or ``None`` where it is."""
+    return None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
-    __slots__ = ("ctx",)
 
-    def __init__(self, device):
-        self.ctx = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.ctx is not None:
-            self.ctx.__enter__()
-
-    def __exit__(self, *exc):
-        if self.ctx is not None:
-            self.ctx.__exit__(*exc)
+def _new(like: Tensor, dtype: Optional[torch.dtype] = None) -> Tensor:
+    return torch.empty_like(like, dtype=dtype, memory_format=torch.contiguous_format)
 
 
 # ---------------------------------------------------------------------------------------------
 # the addition and the norm
 # ---------------------------------------------------------------------------------------------
-def _run_add(update, residual, dropout, out=None) -> Tensor:
-    u, r = _as_pair(update, "update"), _as_pair(residual, "residual")
-    z = torch.empty(update.shape, dtype=update.dtype, device=update.device) if out is None else out
-    with _on(update.device):
-        PK.add_norm(u, r, None, _as_pair(z, "out"), None, dropout=None if dropout is None else dropout._desc())
+# The _run_* functions take checked tensors, allocate what they return and launch on the current stream of the tensors'
+# device.  A dropout comes as the library's record.
+def _run_add(update, residual, record, out=None) -> Tensor:
+    elsewhere = _elsewhere(update.device)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run_add(update, residual, record, out)
+    z = _new(update) if out is None else out
+    PK.launch_add_norm(_as_pair(update), _as_pair(residual), None, _as_pair(z), None, None, 1.0, 0, record)
     return z
 
 
-def _run_norm(update, residual, weight, eps, dropout, group=0):
-    u, r = _as_pair(update, "update"), _as_pair(residual, "residual")
-    dev = update.device
+def _run_norm(update, residual, weight, eps, record, group=0):
+    elsewhere = _elsewhere(update.device)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run_norm(update, residual, weight, eps, record, group)
     # without a residual and a dropout the stream is the update itself
-    z = None if residual is None and dropout is None else torch.empty(update.shape, dtype=update.dtype, device=dev)
-    y = torch.empty(update.shape, dtype=torch.float8_e4m3fn if group else update.dtype, device=dev)
-    scales = torch.empty((*update.shape[:-1], update.shape[-1] // group), dtype=torch.float32, device=dev) if group else None
-    with _on(dev):
-        PK.add_norm(u, r, weight.contiguous(), _as_pair(z, "stream"), _as_pair(y, "y"), scales, eps=eps, group=group,
-                    dropout=None if dropout is None else dropout._desc())
+    z = None if residual is None and record is PK.NO_DROPOUT else _new(update)
+    y, scales = _new(update, torch.float8_e4m3fn if group else None), None
+    if group:
+        scales = torch.empty((*update.shape[:-1], update.shape[-1] // group), dtype=torch.float32, device=update.device)
+    PK.launch_add_norm(_as_pair(update), _as_pair(residual), weight.contiguous(), _as_pair(z), _as_pair(y), scales, eps, group,
+                       record)
     return y, z, scales
 
 
-def _save(ctx, dropout, *tensors) -> None:
-    """Saves the tensors, and a device seed with them: a change of its values before the gradient is an error then."""
-    ctx.dropout = dropout
-    seed = dropout.seed if dropout is not None and isinstance(dropout.seed, Tensor) else None
-    ctx.save_for_backward(*tensors, seed)
+def _run_norm_grad(z, dy, dz, weight, eps, record, need_u, need_r, need_w):
+    """``(d_update, d_residual, d_weight)``; without a dropout the first two are one tensor."""
+    elsewhere = _elsewhere(z.device)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run_norm_grad(z, dy, dz, weight, eps, record, need_u, need_r, need_w)
+    dropped = record is not PK.NO_DROPOUT
+    du = _new(z) if need_u and (dropped or not need_r) else None
+    dr = _new(z) if need_r else None
+    dw = workspace = None
+    if need_w:
+        dw = _new(weight)
+        workspace = torch.empty(PK.add_norm_grad_workspace(z), dtype=_BYTE, device=z.device)
+    PK.launch_add_norm_grad(_as_pair(z), _as_pair(dy), _as_pair(dz), weight.contiguous(), _as_pair(dr), _as_pair(du), dw,
+                            workspace, eps, record)
+    return dr if need_u and du is None else du, dr, dw
 
 
-class _DropoutAdd(torch.autograd.Function):
+def _seed_of(dropout: Optional[PairDropout]) -> Optional[Tensor]:
+    """A device seed, to be saved for the gradient: a change of its values until then is an error."""
+    return dropout.seed if dropout is not None and isinstance(dropout.seed, Tensor) else None
+
+
+def _record_of(dropout: Optional[PairDropout]) -> tuple:
+    return PK.NO_DROPOUT if dropout is None else dropout._record()
+
+
+class _Once(torch.autograd.Function):
+    """A function without a second derivative.  ``once_differentiable`` costs host time and matters only where a graph of
+    the gradient is being made."""
+
+    @classmethod
+    def backward(cls, ctx, *grads):
+        return cls.marked(ctx, *grads) if torch.is_grad_enabled() else cls.gradient(ctx, *grads)
+
+    def __init_subclass__(cls):
+        cls.marked = staticmethod(once_differentiable(cls.gradient))
+
+
+class _DropoutAdd(_Once):
     @staticmethod
     def forward(ctx, update, residual, dropout):
         ctx.set_materialize_grads(False)
-        _save(ctx, dropout)
-        return _run_add(update, residual, dropout)
+        ctx.record = _record_of(dropout)
+        ctx.save_for_backward(_seed_of(dropout))
+        return _run_add(update, residual, ctx.record)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dz):
+    def gradient(ctx, dz):
         if dz is None:
             return None, None, None
         ctx.saved_tensors  # raises where the seed's values were changed
+        need_u, need_r, _ = ctx.needs_input_grad
         du = None
-        if ctx.needs_input_grad[0]:
-            du = dz if ctx.dropout is None else _run_add(dz, None, ctx.dropout)
-        return du, dz if ctx.needs_input_grad[1] else None, None
+        if need_u:
+            du = dz if ctx.record is PK.NO_DROPOUT else _run_add(dz, None, ctx.record)
+        return du, dz if need_r else None, None
 
 
-class _AddRmsNorm(torch.autograd.Function):
+class _AddRmsNorm(_Once):
     @staticmethod
     def forward(ctx, update, residual, weight, eps, dropout):
         ctx.set_materialize_grads(False)
-        y, z, _ = _run_norm(update, residual, weight, eps, dropout)
+        record = _record_of(dropout)
+        y, z, _ = _run_norm(update, residual, weight, eps, record)
         if z is None:
             z = update.view_as(update)
-        ctx.eps = eps
-        _save(ctx, dropout, z, weight)
+        ctx.args = eps, record
+        ctx.save_for_backward(z, weight, _seed_of(dropout))
         return y, z
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dz):
-        z, weight, _ = ctx.saved_tensors
+    def gradient(ctx, dy, dz):
         if dy is None and dz is None:
-            return (None,) * 5
-        need_u, need_r, need_w = ctx.needs_input_grad[:3]
-        dropout, dev = ctx.dropout, z.device
-        new = lambda: torch.empty(z.shape, dtype=z.dtype, device=dev)  # noqa: E731
-        du = new() if need_u and (dropout is not None or not need_r) else None
-        dr = new() if need_r else None
-        dw = torch.empty_like(weight, memory_format=torch.contiguous_format) if need_w else None
-        zp, w = _as_pair(z, "stream"), weight.contiguous()
-        with _on(dev):
-            workspace = None
-            if need_w:
-                workspace = torch.empty(PK.add_norm_grad_workspace(PK.norm_desc(zp, w, ctx.eps)), dtype=_BYTE, device=dev)
-            PK.add_norm_grad(zp, _as_pair(dy, "dy"), _as_pair(dz, "dz"), w, _as_pair(dr, "d_stream"), _as_pair(du, "d_update"),
-                             dw, workspace, eps=ctx.eps, dropout=None if dropout is None else dropout._desc())
-        return dr if need_u and du is None else du, dr, dw, None, None
+            return None, None, None, None, None
+        z, weight, _ = ctx.saved_tensors
+        return (*_run_norm_grad(z, dy, dz, weight, *ctx.args, *ctx.needs_input_grad[:3]), None, None)
 
 
 def dropout_add(update: Tensor, residual: Optional[Tensor] = None, dropout: Optional[PairDropout] = None, *,
@@ -322,7 +351,7 @@ def dropout_add(update: Tensor, residual: Optional[Tensor] = None, dropout: Opti
         _check_overlap(out, residual, "residual")
     elif _needs_grad(update, residual):
         return _DropoutAdd.apply(update, residual, dropout)
-    z = _run_add(update, residual, dropout, out)
+    z = _run_add(update, residual, _record_of(dropout), out)
     if given is not None:
         return given
     return z if wrap is None else wrap(z)
@@ -343,7 +372,7 @@ def add_rms_norm(update: Tensor, residual: Optional[Tensor], weight: Tensor, *, 
         if wrap is not None:
             raise ValueError(_NO_DTENSOR_GRADIENT)
         return _AddRmsNorm.apply(update, residual, weight, eps, dropout)
-    y, z, _ = _run_norm(update, residual, weight, eps, dropout)
+    y, z, _ = _run_norm(update, residual, weight, eps, _record_of(dropout))
     z = update if z is None else z
     return (y, z) if wrap is None else (wrap(y), wrap(z))
 
@@ -364,7 +393,9 @@ def add_rms_norm_fp8(update: Tensor, residual: Optional[Tensor], weight: Tensor,
         raise ValueError(f"group must be 32, 64 or 128 and divide D={width}, or None for one scale per row; got {group}")
     if _needs_grad(update, residual, weight):
         raise ValueError("the e4m3 form has no gradient: run it under torch.no_grad()")
-    y, z, scales = _run_norm(update, residual, weight, eps, dropout, group or width)
+    if group is not None:  # lanes reduce a group's octs: rows have to start on 16-byte boundaries
+        update, residual = _aligned(update), _aligned(residual)
+    y, z, scales = _run_norm(update, residual, weight, eps, _record_of(dropout), group or width)
     z = update if z is None else z
     return (y, scales, z) if wrap is None else (wrap(y), wrap(scales), wrap(z))
 
@@ -373,35 +404,40 @@ def add_rms_norm_fp8(update: Tensor, residual: Optional[Tensor], weight: Tensor,
 # the embedding
 # ---------------------------------------------------------------------------------------------
 def _run_embed(index, table, base, scale, dtype) -> Tensor:
+    elsewhere = _elsewhere(index.device)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run_embed(index, table, base, scale, dtype)
     out = torch.empty((*index.shape, table.shape[1]), dtype=dtype, device=index.device)
-    with _on(index.device):
-        PK.embed(index.contiguous(), table.contiguous(), None if base is None else base.contiguous(), out, scale=scale)
+    PK.launch_embed(index, table.contiguous(), None if base is None else base.contiguous(), out, scale)
     return out
 
 
-class _PairEmbedding(torch.autograd.Function):
+def _run_embed_grad(index, d_out, rows, table_dtype, scale) -> Tensor:
+    elsewhere = _elsewhere(index.device)
+    if elsewhere is not None:
+        with elsewhere:
+            return _run_embed_grad(index, d_out, rows, table_dtype, scale)
+    d_table = torch.empty((rows, d_out.shape[-1]), dtype=table_dtype, device=index.device)
+    workspace = torch.empty(PK.embed_grad_workspace(index, d_table), dtype=_BYTE, device=index.device)
+    PK.launch_embed_grad(index, d_out.contiguous(), d_table, workspace, scale)
+    return d_table
+
+
+class _PairEmbedding(_Once):
     @staticmethod
     def forward(ctx, index, table, base, scale, dtype):
         ctx.set_materialize_grads(False)
-        index = index.contiguous()
         ctx.save_for_backward(index)
-        ctx.scale, ctx.rows, ctx.table_dtype = scale, table.shape[0], table.dtype
+        ctx.args = table.shape[0], table.dtype, scale
         return _run_embed(index, table, base, scale, dtype)
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, d_out):
+    def gradient(ctx, d_out):
         if d_out is None:
-            return (None,) * 5
+            return None, None, None, None, None
         (index,) = ctx.saved_tensors
-        d_table = None
-        if ctx.needs_input_grad[1]:
-            dev = index.device
-            d_table = torch.empty((ctx.rows, d_out.shape[-1]), dtype=ctx.table_dtype, device=dev)
-            with _on(dev):
-                need = PK.embed_grad_workspace(PK.embed_desc(index, d_table, d_out.dtype, ctx.scale))
-                workspace = torch.empty(need, dtype=_BYTE, device=dev)
-                PK.embed_grad(index, d_out.contiguous(), d_table, workspace, scale=ctx.scale)
+        d_table = _run_embed_grad(index, d_out, *ctx.args) if ctx.needs_input_grad[1] else None
         return None, d_table, d_out if ctx.needs_input_grad[2] else None, None, None
 
 
@@ -437,6 +473,7 @@ def pair_embedding(index: Tensor, table: Tensor, *, scale: float = 1.0, base: Op
         raise ValueError(f"the embedding's type must be bfloat16, float16 or float32; got {dtype}")
     if not math.isfinite(scale):
         raise ValueError(f"scale must be finite; got {scale}")
+    index = index.contiguous()
     if _needs_grad(table, base):
         if wrap is not None:
             raise ValueError(_NO_DTENSOR_GRADIENT)

@@ -95,8 +95,16 @@ def test_ctypes_mirrors_match_the_pair_headers_structs(tmp_path):
     assert [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()] == want
 
 
+def test_packed_records_have_the_headers_layout():
+    drop = (0x0123456789ABCDEF, 7, 65535, 0x1000, 2, 3, 4, 5)
+    args = (1, 2, 3, 64, 2, 1, 32, 0.5)
+    assert PK._pack_norm(*args, *drop) == bytes(_lib.PairNormDesc(*args, _lib.PairDropoutDesc(*drop)))
+    assert PK._pack_tensor(0x1000, 1 << 40, -2, 3) == bytes(_lib.PairTensor(0x1000, 1 << 40, -2, 3))
+    assert PK._pack_embed(1 << 30, 64, 9, 32, 1, 2, 0.5) == bytes(_lib.PairEmbedDesc(1 << 30, 64, 9, 32, 1, 2, 0.5))
+
+
 def _norm(**kw):
-    d = _lib.PairNormDesc(1, 2, 3, 64, _lib.PAIR_BF16, _lib.PAIR_BF16, 0, 1e-5, PK.dropout_desc())
+    d = _lib.PairNormDesc(1, 2, 3, 64, _lib.PAIR_BF16, _lib.PAIR_BF16, 0, 1e-5, _lib.PairDropoutDesc(*PK.NO_DROPOUT))
     for k, v in kw.items():
         setattr(d.dropout if k in ("keep", "shared", "origin_b", "origin_i") else d, k, v)
     return d
@@ -184,7 +192,7 @@ def test_dropout_keeps_the_nearest_of_65536():
 def test_there_is_no_cpu_path():
     x, w = torch.zeros(2, 3, 4, 8), torch.ones(8)
     for call in (lambda: P.dropout_add(x, x), lambda: P.add_rms_norm(x, None, w), lambda: P.add_rms_norm_fp8(x, x, w, group=None),
-                 lambda: P.pair_embedding(torch.zeros(3, dtype=torch.int64), w[None]), lambda: PK.norm_desc(x, w)):
+                 lambda: P.pair_embedding(torch.zeros(3, dtype=torch.int64), w[None]), lambda: PK.add_norm(x, x, None, x, None)):
         with pytest.raises(ValueError, match="CUDA"):
             call()
 

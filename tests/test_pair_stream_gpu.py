@@ -289,6 +289,20 @@ def test_add_rms_norm_fp8(shape, dtype):
             assert (err <= torch.maximum(2.0 ** -4 * unit.abs(), torch.full_like(unit, 2.0 ** -10)) * (1 + 2.0 ** -15)).all()
 
 
+@pytest.mark.parametrize("layout", ["block", "transposed", "broadcast", "channels", "shifted"])
+def test_fp8_reads_strided_inputs(layout):
+    p, shape, w = P(), (2, 6, 9, 192), (1 + rand(192, seed=5, scale=0.1))
+    for dtype in TYPES:
+        u, r = layouts(shape, dtype, 3, layout), layouts(shape, dtype, 4, "whole" if layout == "shifted" else layout)
+        for group in (None, 64):
+            got = p.add_rms_norm_fp8(u, r, w, group=group)
+            want = p.add_rms_norm_fp8(u.clone(memory_format=torch.contiguous_format), r.clone(memory_format=torch.contiguous_format), w, group=group)
+            # the same values in another order of the row's sum: scales within 2^-17, q within a step of e4m3
+            assert torch.equal(got[2], want[2]) and ((got[1] - want[1]).abs() <= 2.0 ** -17 * want[1]).all()
+            a, b = got[0].float(), want[0].float()
+            assert ((a - b).abs() <= torch.maximum(2.0 ** -3 * b.abs(), torch.full_like(b, 2.0 ** -9))).all()
+
+
 def test_fp8_of_groups_of_zeros_and_bad_rows():
     p, w = P(), torch.ones(128, device=DEV)
     x = rand(1, 2, 2, 128, seed=3)
