@@ -50,7 +50,7 @@ EXPORTED_SYMBOLS = (
     "trimul_sm100_peer_wait",
 )
 
-#: every symbol include/pair_stream_sm100.h declares
+#: every symbol include/pair_stream_sm100.h declares (called by the host module `_pair_host`, which gets their addresses)
 PAIR_SYMBOLS = (
     "pair_sm100_add_norm",
     "pair_sm100_add_norm_grad_workspace",
@@ -104,30 +104,6 @@ class ReshardPlan(C.Structure):
                 ("walk_rows", C.c_int64), ("plane_elems", C.c_int64), ("dst_base", C.c_int64), ("dst_line", C.c_int64),
                 ("d_loc", C.c_int32), ("planes", C.c_int32), ("ni_loc", C.c_int32), ("nj_loc", C.c_int32),
                 ("chan_offset", C.c_int32), ("pad", C.c_int32), ("rows", C.c_int64)]
-
-
-PAIR_BF16, PAIR_FP16, PAIR_FP32 = 0, 1, 2
-PAIR_SHARED_NONE, PAIR_SHARED_ROWS, PAIR_SHARED_COLUMNS = 0, 1, 2
-PAIR_MAX_WIDTH = 8192
-
-
-class PairDropoutDesc(C.Structure):
-    _fields_ = [("seed", C.c_uint64), ("offset", C.c_uint32), ("keep", C.c_uint32), ("device_seed", C.c_void_p),
-                ("shared", C.c_int32), ("origin_b", C.c_int32), ("origin_i", C.c_int32), ("origin_j", C.c_int32)]
-
-
-class PairTensor(C.Structure):
-    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_i", C.c_int64), ("stride_j", C.c_int64)]
-
-
-class PairNormDesc(C.Structure):
-    _fields_ = [("b", C.c_int32), ("i", C.c_int32), ("j", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
-                ("weight_dtype", C.c_int32), ("group", C.c_int32), ("eps", C.c_float), ("dropout", PairDropoutDesc)]
-
-
-class PairEmbedDesc(C.Structure):
-    _fields_ = [("tokens", C.c_int64), ("d", C.c_int32), ("rows", C.c_int32), ("index_bits", C.c_int32),
-                ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("scale", C.c_float)]
 
 
 class TrimulLibraryError(RuntimeError):
@@ -220,17 +196,40 @@ def load():
                      "trimul_sm100_plan_create", "trimul_sm100_plan_ln_gated_proj", "trimul_sm100_plan_tri_contract",
                      "trimul_sm100_plan_ln_out_proj"):
             getattr(lib, name).restype = C.c_int
-        # the pair-stream records come as packed bytes or by reference: plain pointers either way
-        lib.pair_sm100_add_norm.argtypes = [vp] * 8
-        lib.pair_sm100_add_norm_grad_workspace.argtypes = [vp, C.POINTER(C.c_uint64)]
-        lib.pair_sm100_add_norm_grad.argtypes = [vp] * 10
-        lib.pair_sm100_embed.argtypes = [vp] * 6
-        lib.pair_sm100_embed_grad_workspace.argtypes = [vp, C.POINTER(C.c_uint64)]
-        lib.pair_sm100_embed_grad.argtypes = [vp] * 6
         for name in PAIR_SYMBOLS:
             getattr(lib, name).restype = C.c_int
         _lib = lib
         return lib
+
+
+_pair = None
+
+
+def pair_host():
+    """The native host module of the pair-stream operators (``csrc/pair_host.cpp``), bound to the loaded library."""
+    global _pair
+    if _pair is not None:
+        return _pair
+    lib = load()
+    with _lock:
+        if _pair is not None:
+            return _pair
+        try:
+            from . import _pair_host as host
+        except ImportError as exc:
+            raise TrimulLibraryError(
+                f"cannot load the host module {_PKG_DIR / '_pair_host.so'}: {exc}. Build it with "
+                "`python -m fold_cp_ops_b200.build`.") from exc
+        from .build import source_digest
+
+        if host.build_id() != source_digest():
+            raise TrimulLibraryError(
+                f"{host.__file__} was not built from the sources next to it (build id {host.build_id()}, sources "
+                f"{source_digest()}); rebuild it with `python -m fold_cp_ops_b200.build`.")
+        names = PAIR_SYMBOLS + ("trimul_sm100_last_error",)
+        host.bind({n: C.cast(getattr(lib, n), C.c_void_p).value for n in names}, TrimulLibraryError)
+        _pair = host
+        return host
 
 
 def last_error() -> str:

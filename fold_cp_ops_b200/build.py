@@ -1,7 +1,8 @@
-"""Ahead-of-time build of ``libtrimul_sm100.so`` with nvcc for sm_100a.
+"""Ahead-of-time build of ``libtrimul_sm100.so`` with nvcc for sm_100a, and of the host module ``_pair_host.so``.
 
-The library is built in-tree (next to this file) so that it travels with a snapshot of the
-repository; there is no JIT and no torch extension machinery involved.  ``python -m
+Both are built in-tree (next to this file) so that they travel with a snapshot of the repository; there is no JIT.  The
+library holds every kernel and knows nothing of torch; the host module (argument checks, allocation and gradients of
+the pair-stream operators, C++ against torch's headers) holds no kernel and calls the library.  ``python -m
 fold_cp_ops_b200.build`` rebuilds it; :func:`ensure_built` rebuilds only when a source is newer
 than the library.
 """
@@ -21,6 +22,8 @@ SOURCES = ("trimul_capi.cu", "ln_gated_proj.cu", "tri_contract.cu", "tri_contrac
            "forward_static.cu", "pair_norm.cu", "pair_norm_grad.cu", "pair_embed.cu")
 HEADERS = ("sm100_ptx.cuh", "trimul_common.cuh", "trimul_kernels.h", "tri_contract_epilogue.cuh", "pair_stream.cuh")
 PUBLIC_HEADERS = ("trimul_sm100.h", "pair_stream_sm100.h")
+HOST_SOURCE = "pair_host.cpp"
+HOST_PATH = PKG_DIR / "_pair_host.so"
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -39,7 +42,7 @@ def source_digest() -> str:
     import hashlib
 
     h = hashlib.sha256()
-    for f in [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]:
+    for f in [CSRC / s for s in SOURCES + HEADERS + (HOST_SOURCE,)] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]:
         h.update(f.name.encode())
         h.update(f.read_bytes())
     return h.hexdigest()[:32]
@@ -53,15 +56,15 @@ def _nvcc() -> str:
 
 
 def is_stale() -> bool:
-    if not LIB_PATH.exists():
+    if not LIB_PATH.exists() or not HOST_PATH.exists():
         return True
-    t = LIB_PATH.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]
+    t = min(LIB_PATH.stat().st_mtime, HOST_PATH.stat().st_mtime)
+    deps = [CSRC / s for s in SOURCES + HEADERS + (HOST_SOURCE,)] + [PKG_DIR.parent / "include" / h for h in PUBLIC_HEADERS]
     return any(d.exists() and d.stat().st_mtime > t for d in deps)
 
 
 def build(verbose: bool = False, ptxas_info: bool = False, ablate: int = 0) -> Path:
-    """Compile every kernel for sm_100a into one shared library; returns its path.
+    """Compile every kernel for sm_100a into one shared library, and the host module; returns the library's path.
 
     ``ablate`` != 0 builds a PROFILING library ``libtrimul_sm100_ablate<bits>.so`` beside the real one, in
     which roles of the projection kernel do no work (``TRIMUL_ABLATE`` in ``csrc/ln_gated_proj.cu``); select
@@ -78,7 +81,35 @@ def build(verbose: bool = False, ptxas_info: bool = False, ablate: int = 0) -> P
         raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
     if verbose or ptxas_info:
         sys.stderr.write(proc.stderr)
+    if not ablate:
+        _build_host(verbose)
     return out
+
+
+def _build_host(verbose: bool = False) -> Path:
+    """Compile the host module against the installed torch."""
+    import sysconfig
+
+    import torch
+
+    cxx = shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("g++ not found; _pair_host.so cannot be built")
+    root = Path(torch.__file__).parent
+    cuda = Path(_nvcc()).resolve().parent.parent
+    include = (root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+               Path(sysconfig.get_paths()["include"]))
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_pair_host",
+           "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           f'-DTRIMUL_BUILD_ID="{source_digest()}"', *(a for p in include for a in ("-isystem", str(p))),
+           str(CSRC / HOST_SOURCE), "-o", str(HOST_PATH), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch",
+           "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    return HOST_PATH
 
 
 def ensure_built() -> Path:

@@ -10,7 +10,7 @@
 // packed fp32 pairs (and in packed 16-bit additions where there is no dropout).
 // Split.  A row of up to 256 channels is one oct (eight channels, 16 bytes of a 16-bit type) per lane of 8, 16 or 32
 // lanes, so that the reductions stay inside a warp;
-// up to 512 channels it is two octs per lane of a warp; wider rows take a CTA with one oct per thread.  A group holds two
+// up to 512 channels it is three octs of 16 lanes or two of 32; wider rows take a CTA with one oct per thread.  A group holds two
 // rows at a time where that is one 16-byte access per lane, row and tensor: more bytes in flight.
 #include "pair_stream.cuh"
 
@@ -33,7 +33,8 @@ struct NormArgs {
   uint32_t rows;
   int d, octs;
   int weight_dtype;
-  int group;  // channels per scale
+  int scales_per_row;
+  int scale_shift;  // log2 of the octs per scale; -1: the row has one scale
   int flat;   // the rows of update and residual lie at a constant distance
   float eps, inv_d;
 };
@@ -44,13 +45,22 @@ __device__ __forceinline__ uint32_t e4m3x2(float2 v) {
   return r;
 }
 
-// kU channels per access, kGroup lanes per row, kUnits units per lane, kFlight rows of a group in flight.
-template <typename T, int kU, int kGroup, int kUnits, int kFlight, int kMode>
+// Stages of the ring that the lanes' units pass through, by a lane's bytes of one row and tensor.  More stages gain nothing: fewer
+// CTAs are resident then (1024 x 1024 rows of 256 to e4m3: three stages 336 us, four 351, two 348; 384 channels: two 42.5,
+// three 44, four 51).
+__host__ __device__ constexpr int ring_of(int lane_bytes) { return lane_bytes <= 16 ? 3 : 2; }
+
+// kU channels per access, kGroup lanes per row, kUnits units per lane.
+template <typename T, int kU, int kGroup, int kUnits, int kMode>
 __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup)) add_norm_kernel(const __grid_constant__ NormArgs<T> a) {
-  __shared__ float sums[2 * 32 * kFlight];
-  __shared__ float tops[2 * 32 * kFlight];
-  constexpr int kRows = threads_of(kGroup) / kGroup;  // rows a CTA holds side by side
+  __shared__ float sums[2 * 32];
+  __shared__ float tops[2 * 32];
+  extern __shared__ uint4 ring[];
+  constexpr int kWide = threads_of(kGroup);
+  constexpr int kRows = kWide / kGroup;  // rows a CTA holds side by side
   constexpr int kPairs = (kU + 1) / 2;
+  constexpr int kBytes = sizeof(T) * kU;
+  constexpr int kRing = ring_of(kUnits * kBytes);
   const int lane = threadIdx.x % kGroup;
   const int units = a.d / kU;
   const bool dropping = a.drop.keep < 65536u;
@@ -74,168 +84,177 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
     }
   }
 
-  int parity = 0;
   const uint32_t span = gridDim.x * kRows;
-  // the bound is the CTA's first row: lanes whose row lies behind the end still take part in the reductions
-  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += kFlight * span, parity ^= 1) {
-    Unit<T, kU> u[kFlight][kUnits], r[kFlight][kUnits];
-    uint32_t b[kFlight], i[kFlight], j[kFlight];
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const uint32_t row = first + f * span + threadIdx.x / kGroup;
+  auto rows_of = [&](uint32_t row, const T*& up, const T*& rp) {
+    if (a.flat) {
+      up = a.update.flat(row);
+      rp = a.residual.flat(row);
+    } else {
+      uint32_t b, i, j;
+      a.walk.at(row, b, i, j);
+      up = a.update.row(b, i, j);
+      rp = a.residual.row(b, i, j);
+    }
+  };
+  // one stage: the update's units, then the residual's, each kWide lanes side by side
+  const int stage_bytes = kUnits * kWide * kBytes * (has_residual ? 2 : 1);
+  char* const slots = reinterpret_cast<char*>(ring) + threadIdx.x * kBytes;
+  auto fetch = [&](uint32_t row, char* slot) {
+    if (row < a.rows) {
       const T *up, *rp;
-      b[f] = i[f] = j[f] = 0;
-      if (row < a.rows) {
-        if (dropping || !a.flat) a.walk.at(row, b[f], i[f], j[f]);
-        if (a.flat) {
-          up = a.update.flat(row);
-          rp = a.residual.flat(row);
-        } else {
-          up = a.update.row(b[f], i[f], j[f]);
-          rp = a.residual.row(b[f], i[f], j[f]);
-        }
-      }
+      rows_of(row, up, rp);
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
         const int n = lane + k * kGroup;
-        const bool on = row < a.rows && n < units;
-        u[f][k] = on ? load_unit<T, kU>(up + n * kU) : zero_unit<T, kU>();
-        r[f][k] = on && has_residual ? load_unit<T, kU>(rp + n * kU) : zero_unit<T, kU>();
+        if (n < units) {
+          stage_unit<T, kU>(slot + k * kWide * kBytes, up + n * kU);
+          if (has_residual) stage_unit<T, kU>(slot + (kUnits + k) * kWide * kBytes, rp + n * kU);
+        }
+      }
+    }
+    stage_commit();
+  };
+
+  const uint32_t mine = threadIdx.x / kGroup;
+  if constexpr (kCanStage<T, kU>) {
+#pragma unroll
+    for (int s = 0; s < kRing - 1; ++s) fetch(blockIdx.x * kRows + mine + s * span, slots + s * stage_bytes);
+  }
+  int parity = 0, stage = 0;
+  // the bound is the CTA's first row: lanes whose row lies behind the end still take part in the reductions
+  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += span, parity ^= 1) {
+    const uint32_t row = first + mine;
+    const bool valid = row < a.rows;
+    Unit<T, kU> u[kUnits], r[kUnits];
+    if constexpr (kCanStage<T, kU>) {
+      fetch(row + (kRing - 1) * span, slots + ((stage + kRing - 1) % kRing) * stage_bytes);
+      stage_wait<kRing - 1>();
+      const char* slot = slots + stage * stage_bytes;
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        const bool on = valid && lane + k * kGroup < units;
+        u[k] = on ? staged_unit<T, kU>(slot + k * kWide * kBytes) : zero_unit<T, kU>();
+        r[k] = on && has_residual ? staged_unit<T, kU>(slot + (kUnits + k) * kWide * kBytes) : zero_unit<T, kU>();
+      }
+      stage = (stage + 1) % kRing;
+    } else {
+      const T *up = nullptr, *rp = nullptr;
+      if (valid) rows_of(row, up, rp);
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        const int n = lane + k * kGroup;
+        const bool on = valid && n < units;
+        u[k] = on ? load_unit<T, kU>(up + n * kU) : zero_unit<T, kU>();
+        r[k] = on && has_residual ? load_unit<T, kU>(rp + n * kU) : zero_unit<T, kU>();
       }
     }
 
-    float ss[kFlight];
-#pragma unroll
-    for (int f = 0; f < kFlight; ++f) {
-      const uint32_t row = first + f * span + threadIdx.x / kGroup;
-      if (dropping) {
-        if constexpr (kU == 8) {
-#pragma unroll
-          for (int k = 0; k < kUnits; ++k) {
-            Vals<8> v = unpack(u[f][k]);
-            drop_oct(draw_oct(drop, b[f], i[f], j[f], lane + k * kGroup), line, drop.gain, v);
-            const Vals<8> x = unpack(r[f][k]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
-            u[f][k] = pack<T, 8>(v);
-          }
-        } else {
-          const auto mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b[f], i[f], j[f], lane & ~31, a.octs);
-#pragma unroll
-          for (int k = 0; k < kUnits; ++k) {
-            const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
-            Vals<kU> v = unpack(u[f][k]);
-            v.p[0].x = bits & 1u ? v.p[0].x * drop.gain : 0.f;
-            if constexpr (kU > 1) v.p[0].y = bits & 2u ? v.p[0].y * drop.gain : 0.f;
-            const Vals<kU> x = unpack(r[f][k]);
-            v.p[0] = __fadd2_rn(v.p[0], x.p[0]);
-            u[f][k] = pack<T, kU>(v);
-          }
-        }
-      } else if (has_residual) {
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) u[f][k] = add_units(u[f][k], r[f][k]);
-      }
-      if (a.stream != nullptr && row < a.rows) {
-        T* zp = a.stream + static_cast<int64_t>(row) * a.d;
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k)
-          if (lane + k * kGroup < units) store_unit<T, kU>(zp + (lane + k * kGroup) * kU, u[f][k]);
-      }
-      if constexpr (kMode != kAdd) {
-        float2 s = both(0.f);
+    if (dropping) {
+      uint32_t b, i, j;
+      a.walk.at(valid ? row : 0, b, i, j);
+      if constexpr (kU == 8) {
 #pragma unroll
         for (int k = 0; k < kUnits; ++k) {
-          const Vals<kU> v = unpack(u[f][k]);
+          Vals<8> v = unpack(u[k]);
+          drop_oct(draw_oct(drop, b, i, j, lane + k * kGroup), line, drop.gain, v);
+          const Vals<8> x = unpack(r[k]);
 #pragma unroll
-          for (int e = 0; e < kPairs; ++e) s = __ffma2_rn(v.p[e], v.p[e], s);
+          for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
+          u[k] = pack<T, 8>(v);
         }
-        ss[f] = s.x + s.y;
+      } else {
+        const auto mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b, i, j, lane & ~31, a.octs);
+#pragma unroll
+        for (int k = 0; k < kUnits; ++k) {
+          const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
+          Vals<kU> v = unpack(u[k]);
+          v.p[0].x = bits & 1u ? v.p[0].x * drop.gain : 0.f;
+          if constexpr (kU > 1) v.p[0].y = bits & 2u ? v.p[0].y * drop.gain : 0.f;
+          const Vals<kU> x = unpack(r[k]);
+          v.p[0] = __fadd2_rn(v.p[0], x.p[0]);
+          u[k] = pack<T, kU>(v);
+        }
       }
+    } else if (has_residual) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) u[k] = add_units(u[k], r[k]);
+    }
+    const int64_t out_row = static_cast<int64_t>(row) * a.d;
+    if (a.stream != nullptr && valid) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k)
+        if (lane + k * kGroup < units) store_unit<T, kU>(a.stream + out_row + (lane + k * kGroup) * kU, u[k]);
     }
     if constexpr (kMode == kAdd) continue;
-    group_sum<kGroup, kFlight>(ss, sums, parity);
+
+    float2 s = both(0.f);
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const Vals<kU> v = unpack(u[k]);
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) s = __ffma2_rn(v.p[e], v.p[e], s);
+    }
+    float ss[1] = {s.x + s.y};
+    group_sum<kGroup, 1>(ss, sums, parity);
+    const float2 rstd = both(rsqrtf(ss[0] * a.inv_d + a.eps));
 
     if constexpr (kMode == kNorm) {
+      T* yp = static_cast<T*>(a.y) + out_row;
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        const uint32_t row = first + f * span + threadIdx.x / kGroup;
-        if (row >= a.rows) break;
-        const float2 rstd = both(rsqrtf(ss[f] * a.inv_d + a.eps));
-        T* yp = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.d;
+      for (int k = 0; k < kUnits; ++k) {
+        Vals<kU> v = unpack(u[k]);
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          Vals<kU> v = unpack(u[f][k]);
-#pragma unroll
-          for (int e = 0; e < kPairs; ++e) v.p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
-          if (lane + k * kGroup < units) store_unit<T, kU>(yp + (lane + k * kGroup) * kU, pack<T, kU>(v));
-        }
+        for (int e = 0; e < kPairs; ++e) v.p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
+        if (valid && lane + k * kGroup < units) store_unit<T, kU>(yp + (lane + k * kGroup) * kU, pack<T, kU>(v));
       }
     } else if constexpr (kMode == kNormE4m3) {
-      const bool whole = a.group == a.d;
-      const int per = a.group / 8;  // octs per scale; 4, 8 or 16 unless the whole row has one (the only form of narrow units)
-      float top[kFlight][kUnits];
-      Vals<kU> y[kFlight][kUnits];
+      const bool whole = a.scale_shift < 0;  // the only form of narrow units
+      float top[kUnits];
+      Vals<kU> y[kUnits];
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        const float2 rstd = both(rsqrtf(ss[f] * a.inv_d + a.eps));
+      for (int k = 0; k < kUnits; ++k) {
+        const Vals<kU> v = unpack(u[k]);
+        top[k] = 0.f;
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          const Vals<kU> v = unpack(u[f][k]);
-          top[f][k] = 0.f;
-#pragma unroll
-          for (int e = 0; e < kPairs; ++e) {
-            y[f][k].p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
-            top[f][k] = fmaxf(top[f][k], fmaxf(fabsf(y[f][k].p[e].x), fabsf(y[f][k].p[e].y)));
-          }
+        for (int e = 0; e < kPairs; ++e) {
+          y[k].p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
+          top[k] = fmaxf(top[k], fmaxf(fabsf(y[k].p[e].x), fabsf(y[k].p[e].y)));
         }
       }
       if (whole) {
-        float m[kFlight];
+        float m[1] = {top[0]};
 #pragma unroll
-        for (int f = 0; f < kFlight; ++f) {
-          m[f] = top[f][0];
+        for (int k = 1; k < kUnits; ++k) m[0] = fmaxf(m[0], top[k]);
+        group_max<kGroup, 1>(m, tops, parity);
 #pragma unroll
-          for (int k = 1; k < kUnits; ++k) m[f] = fmaxf(m[f], top[f][k]);
-        }
-        group_max<kGroup, kFlight>(m, tops, parity);
-#pragma unroll
-        for (int f = 0; f < kFlight; ++f)
-#pragma unroll
-          for (int k = 0; k < kUnits; ++k) top[f][k] = m[f];
+        for (int k = 0; k < kUnits; ++k) top[k] = m[0];
       } else {
         // 32, 64 or 128 channels are 4, 8 or 16 neighbouring lanes
-        for (int o = 1; o < per; o <<= 1)
+        for (int o = 1; o >> a.scale_shift == 0; o <<= 1)
 #pragma unroll
-          for (int f = 0; f < kFlight; ++f)
-#pragma unroll
-            for (int k = 0; k < kUnits; ++k) top[f][k] = fmaxf(top[f][k], __shfl_xor_sync(0xffffffffu, top[f][k], o));
+          for (int k = 0; k < kUnits; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
       }
+      if (!valid) continue;
+      uint8_t* yp = static_cast<uint8_t*>(a.y) + out_row;
+      float* sp = a.scales + static_cast<int64_t>(row) * a.scales_per_row;
 #pragma unroll
-      for (int f = 0; f < kFlight; ++f) {
-        const uint32_t row = first + f * span + threadIdx.x / kGroup;
-        if (row >= a.rows) break;
-        uint8_t* yp = static_cast<uint8_t*>(a.y) + static_cast<int64_t>(row) * a.d;
-        float* sp = a.scales + static_cast<int64_t>(row) * (whole ? 1 : a.d / a.group);
+      for (int k = 0; k < kUnits; ++k) {
+        const int n = lane + k * kGroup;
+        if (n >= units) continue;
+        const float scale = top[k] > 0.f ? fmaxf(top[k] * (1.f / kE4m3Max), 1.17549435e-38f) : 1.f;
+        if (whole ? n == 0 : (n & ((1 << a.scale_shift) - 1)) == 0) sp[whole ? 0 : n >> a.scale_shift] = scale;
+        const float2 inv = both(1.f / scale);
+        if constexpr (kU == 8) {
+          uint32_t q[4];
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          const int n = lane + k * kGroup;
-          if (n >= units) continue;
-          const float scale = top[f][k] > 0.f ? fmaxf(top[f][k] * (1.f / kE4m3Max), 1.17549435e-38f) : 1.f;
-          if (whole ? n == 0 : n % per == 0) sp[whole ? 0 : n / per] = scale;
-          const float2 inv = both(1.f / scale);
-          if constexpr (kU == 8) {
-            uint32_t q[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) q[e] = e4m3x2(__fmul2_rn(y[f][k].p[e], inv));
-            __stcs(reinterpret_cast<uint2*>(yp + n * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
-          } else {
-            const uint32_t q = e4m3x2(__fmul2_rn(y[f][k].p[0], inv));
-            if constexpr (kU == 2)
-              *reinterpret_cast<uint16_t*>(yp + n * 2) = static_cast<uint16_t>(q);
-            else
-              yp[n] = static_cast<uint8_t>(q);
-          }
+          for (int e = 0; e < 4; ++e) q[e] = e4m3x2(__fmul2_rn(y[k].p[e], inv));
+          __stcs(reinterpret_cast<uint2*>(yp + n * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
+        } else {
+          const uint32_t q = e4m3x2(__fmul2_rn(y[k].p[0], inv));
+          if constexpr (kU == 2)
+            *reinterpret_cast<uint16_t*>(yp + n * 2) = static_cast<uint16_t>(q);
+          else
+            yp[n] = static_cast<uint8_t>(q);
         }
       }
     }
@@ -302,40 +321,51 @@ cudaError_t launch_add(const NormArgs<T>& a, int sms, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-template <typename T, int kU, int kGroup, int kUnits, int kFlight, int kMode>
+template <typename T, int kU, int kGroup, int kUnits, int kMode>
 cudaError_t launch(const NormArgs<T>& a, int sms, cudaStream_t stream) {
   constexpr uint32_t kWide = threads_of(kGroup), kRows = kWide / kGroup;
+  auto kernel = add_norm_kernel<T, kU, kGroup, kUnits, kMode>;
+  const bool has_residual = a.residual.p != nullptr;
+  constexpr int kStage = kUnits * kU * static_cast<int>(sizeof(T) * kWide);
+  constexpr int kStages = kCanStage<T, kU> ? ring_of(kStage / static_cast<int>(kWide)) * kStage : 0;
+  const int smem = kStages * (has_residual ? 2 : 1);
+  if (2 * kStages > 47 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStages);
+    if (e != cudaSuccess) return e;
+  }
+  // one wave: what is resident with and without a residual's stages
+  static const int resident[2] = {resident_ctas(kernel, kWide, kStages), resident_ctas(kernel, kWide, 2 * kStages)};
   const uint32_t need = (a.rows + kRows - 1) / kRows;
-  const uint32_t most = static_cast<uint32_t>(sms) * (2048 / kWide);
-  add_norm_kernel<T, kU, kGroup, kUnits, kFlight, kMode><<<need < most ? need : most, kWide, 0, stream>>>(a);
+  const uint32_t most = static_cast<uint32_t>(sms) * resident[has_residual];
+  kernel<<<need < most ? need : most, kWide, smem, stream>>>(a);
   return cudaGetLastError();
 }
 
-// Octs: two rows in flight where a lane has one 16-byte oct of each.
+// Octs.
 template <typename T, int kMode>
 cudaError_t wide_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
-  constexpr int kTwo = sizeof(T) == 2 ? 2 : 1;
   const int o = a.octs;
-  if (o <= 8) return launch<T, 8, 8, 1, kTwo, kMode>(a, sms, s);
-  if (o <= 16) return launch<T, 8, 16, 1, kTwo, kMode>(a, sms, s);
-  if (o <= 32) return launch<T, 8, 32, 1, kTwo, kMode>(a, sms, s);
-  if (o <= 64) return launch<T, 8, 32, 2, 1, kMode>(a, sms, s);
-  if (o <= 128) return launch<T, 8, 128, 1, kTwo, kMode>(a, sms, s);
-  if (o <= 256) return launch<T, 8, 256, 1, kTwo, kMode>(a, sms, s);
-  if (o <= 512) return launch<T, 8, 512, 1, kTwo, kMode>(a, sms, s);
-  return launch<T, 8, 1024, 1, kTwo, kMode>(a, sms, s);
+  if (o <= 8) return launch<T, 8, 8, 1, kMode>(a, sms, s);
+  if (o <= 16) return launch<T, 8, 16, 1, kMode>(a, sms, s);
+  if (o <= 32) return launch<T, 8, 32, 1, kMode>(a, sms, s);
+  if (o <= 48) return launch<T, 8, 16, 3, kMode>(a, sms, s);
+  if (o <= 64) return launch<T, 8, 32, 2, kMode>(a, sms, s);
+  if (o <= 128) return launch<T, 8, 128, 1, kMode>(a, sms, s);
+  if (o <= 256) return launch<T, 8, 256, 1, kMode>(a, sms, s);
+  if (o <= 512) return launch<T, 8, 512, 1, kMode>(a, sms, s);
+  return launch<T, 8, 1024, 1, kMode>(a, sms, s);
 }
 
 // Units of one or two channels: four or eight channels per lane of a warp, then of a CTA.
 template <typename T, int kU, int kMode>
 cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
-  if (a.d <= 128) return launch<T, kU, 32, 4 / kU, 2, kMode>(a, sms, s);
-  if (a.d <= 256) return launch<T, kU, 32, 8 / kU, 1, kMode>(a, sms, s);
-  if (a.d <= 512) return launch<T, kU, 128, 4 / kU, 2, kMode>(a, sms, s);
-  if (a.d <= 1024) return launch<T, kU, 256, 4 / kU, 2, kMode>(a, sms, s);
-  if (a.d <= 2048) return launch<T, kU, 512, 4 / kU, 2, kMode>(a, sms, s);
-  if (a.d <= 4096) return launch<T, kU, 1024, 4 / kU, 2, kMode>(a, sms, s);
-  return launch<T, kU, 1024, 8 / kU, 1, kMode>(a, sms, s);
+  if (a.d <= 128) return launch<T, kU, 32, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 256) return launch<T, kU, 32, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 512) return launch<T, kU, 128, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 1024) return launch<T, kU, 256, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 2048) return launch<T, kU, 512, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 4096) return launch<T, kU, 1024, 4 / kU, kMode>(a, sms, s);
+  return launch<T, kU, 1024, 8 / kU, kMode>(a, sms, s);
 }
 
 template <typename T, int kMode>
@@ -363,7 +393,8 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* update, const pa
   a.d = d->d;
   a.octs = (d->d + 7) / 8;
   a.weight_dtype = d->weight_dtype;
-  a.group = d->group;
+  a.scales_per_row = d->group != 0 ? d->d / d->group : 0;
+  a.scale_shift = d->group == d->d ? -1 : d->group == 32 ? 2 : d->group == 64 ? 3 : 4;
   a.flat = collapses(update, d->b, d->i, d->j) && collapses(residual, d->b, d->i, d->j);
   a.eps = d->eps;
   a.inv_d = 1.f / static_cast<float>(d->d);

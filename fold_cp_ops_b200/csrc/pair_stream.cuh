@@ -52,10 +52,13 @@ template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> load_unit(const T* p) {
   Unit<T, kU> o;
   constexpr int kBytes = sizeof(T) * kU;
-  if constexpr (kBytes >= 16) {
+  if constexpr (kBytes == 32) {
+    // (the alignment of a row is 16 bytes)
     uint4* w = reinterpret_cast<uint4*>(&o);
-#pragma unroll
-    for (int k = 0; k < kBytes / 16; ++k) w[k] = __ldcs(reinterpret_cast<const uint4*>(p) + k);
+    w[0] = __ldcs(reinterpret_cast<const uint4*>(p));
+    w[1] = __ldcs(reinterpret_cast<const uint4*>(p) + 1);
+  } else if constexpr (kBytes == 16) {
+    *reinterpret_cast<uint4*>(&o) = __ldcs(reinterpret_cast<const uint4*>(p));
   } else if constexpr (kBytes == 4) {
     *reinterpret_cast<uint32_t*>(&o) = __ldcs(reinterpret_cast<const uint32_t*>(p));
   } else {
@@ -78,6 +81,30 @@ __device__ __forceinline__ void store_unit(T* p, const Unit<T, kU>& o) {
     __stcs(reinterpret_cast<uint16_t*>(p), *reinterpret_cast<const uint16_t*>(&o));
   }
 }
+
+// Asynchronous copies of a lane's own units into its own slots of shared memory, read back by the same lane: bytes in flight that
+// cost no registers, and no barrier (cp.async groups complete per thread).  Not for 2-byte units, which cp.async does not know, nor for
+// octs of fp32, whose two 16-byte halves would each touch every sector of the row: direct loads find the second half in L1.
+template <typename T, int kU>
+constexpr bool kCanStage = sizeof(T) * kU == 4 || sizeof(T) * kU == 16;
+
+template <typename T, int kU>
+__device__ __forceinline__ void stage_unit(void* slot, const T* p) {
+  constexpr int kBytes = sizeof(T) * kU;
+  const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
+  if constexpr (kBytes == 16) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
+  } else {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(p) : "memory");
+  }
+}
+template <typename T, int kU>
+__device__ __forceinline__ Unit<T, kU> staged_unit(const void* slot) {
+  return *static_cast<const Unit<T, kU>*>(slot);
+}
+__device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
 
 template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> zero_unit() {
@@ -377,6 +404,17 @@ __device__ __forceinline__ void group_sum(float (&v)[kN], float* buf, int parity
 template <int kGroup, int kN>
 __device__ __forceinline__ void group_max(float (&v)[kN], float* buf, int parity) {
   group_merge<kGroup, kN, true>(v, buf, parity);
+}
+
+// CTAs of a kernel that an SM holds at once (at least one).
+template <typename K>
+int resident_ctas(K kernel, int threads, int smem) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, smem) != cudaSuccess) {
+    cudaGetLastError();
+    n = 1;
+  }
+  return n < 1 ? 1 : n;
 }
 
 // Host-side checks shared by the entry points.

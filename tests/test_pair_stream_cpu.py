@@ -9,11 +9,37 @@ import pytest
 import torch
 
 from fold_cp_ops_b200 import _lib
-from fold_cp_ops_b200 import pair_kernels as PK
 from fold_cp_ops_b200.workflows import pair_stream as P
 from oracle.pair_oracle import keep_mask, philox4x32_10, rms_norm, rms_norm_grad
 
 INCLUDE = Path(__file__).resolve().parent.parent / "include"
+BF16 = 0
+
+
+class Dropout(C.Structure):
+    _fields_ = [("seed", C.c_uint64), ("offset", C.c_uint32), ("keep", C.c_uint32), ("device_seed", C.c_void_p),
+                ("shared", C.c_int32), ("origin_b", C.c_int32), ("origin_i", C.c_int32), ("origin_j", C.c_int32)]
+
+
+class Tensor4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride_b", C.c_int64), ("stride_i", C.c_int64), ("stride_j", C.c_int64)]
+
+
+class NormDesc(C.Structure):
+    _fields_ = [("b", C.c_int32), ("i", C.c_int32), ("j", C.c_int32), ("d", C.c_int32), ("dtype", C.c_int32),
+                ("weight_dtype", C.c_int32), ("group", C.c_int32), ("eps", C.c_float), ("dropout", Dropout)]
+
+
+class EmbedDesc(C.Structure):
+    _fields_ = [("tokens", C.c_int64), ("d", C.c_int32), ("rows", C.c_int32), ("index_bits", C.c_int32),
+                ("dtype", C.c_int32), ("table_dtype", C.c_int32), ("scale", C.c_float)]
+
+
+def refused(name, pat, *args):
+    """The C entry refuses: pointers that are no structs stand for addresses that it must not reach."""
+    args = [C.byref(a) if isinstance(a, C.Structure) else None if a is None else C.c_void_p(a) for a in args]
+    with pytest.raises(ValueError, match=pat):
+        _lib.check(getattr(_lib.load(), name)(*args), name)
 
 
 # ------------------------------------------------------------------------------------------------
@@ -77,8 +103,7 @@ def test_ctypes_mirrors_match_the_pair_headers_structs(tmp_path):
 
     if shutil.which("gcc") is None:
         pytest.skip("no C compiler")
-    mirrors = {"pair_dropout": _lib.PairDropoutDesc, "pair_tensor": _lib.PairTensor, "pair_norm_desc": _lib.PairNormDesc,
-               "pair_embed_desc": _lib.PairEmbedDesc}
+    mirrors = {"pair_dropout": Dropout, "pair_tensor": Tensor4, "pair_norm_desc": NormDesc, "pair_embed_desc": EmbedDesc}
     header = (INCLUDE / "pair_stream_sm100.h").read_text()
     assert set(re.findall(r"typedef struct (\w+) \{", header)) == set(mirrors)
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "pair_stream_sm100.h"', 'int main(void) {']
@@ -95,16 +120,25 @@ def test_ctypes_mirrors_match_the_pair_headers_structs(tmp_path):
     assert [int(v) for v in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()] == want
 
 
-def test_packed_records_have_the_headers_layout():
-    drop = (0x0123456789ABCDEF, 7, 65535, 0x1000, 2, 3, 4, 5)
-    args = (1, 2, 3, 64, 2, 1, 32, 0.5)
-    assert PK._pack_norm(*args, *drop) == bytes(_lib.PairNormDesc(*args, _lib.PairDropoutDesc(*drop)))
-    assert PK._pack_tensor(0x1000, 1 << 40, -2, 3) == bytes(_lib.PairTensor(0x1000, 1 << 40, -2, 3))
-    assert PK._pack_embed(1 << 30, 64, 9, 32, 1, 2, 0.5) == bytes(_lib.PairEmbedDesc(1 << 30, 64, 9, 32, 1, 2, 0.5))
+def test_the_packed_dropout_has_the_headers_layout():
+    drop = P.PairDropout(0.25, seed=0x8123456789ABCDEF, offset=7, shared="columns", origin=(3, 4, 5))
+    assert P._record(drop, None) == (bytes(Dropout(0x8123456789ABCDEF, 7, 49152, None, 2, 3, 4, 5)), None)
+    assert P._record(None, None) == P._record(P.PairDropout(1e-6), None) == (b"", None)
+
+
+def test_the_host_module_was_built_from_these_sources(monkeypatch):
+    from fold_cp_ops_b200 import build
+
+    host = _lib.pair_host()
+    assert host.build_id() == build.source_digest()
+    monkeypatch.setattr(_lib, "_pair", None)
+    monkeypatch.setattr(build, "source_digest", lambda: "0" * 32)
+    with pytest.raises(_lib.TrimulLibraryError, match="was not built from the sources"):
+        _lib.pair_host()
 
 
 def _norm(**kw):
-    d = _lib.PairNormDesc(1, 2, 3, 64, _lib.PAIR_BF16, _lib.PAIR_BF16, 0, 1e-5, _lib.PairDropoutDesc(*PK.NO_DROPOUT))
+    d = NormDesc(1, 2, 3, 64, BF16, BF16, 0, 1e-5, Dropout(keep=65536))
     for k, v in kw.items():
         setattr(d.dropout if k in ("keep", "shared", "origin_b", "origin_i") else d, k, v)
     return d
@@ -120,28 +154,24 @@ def _norm(**kw):
 ])
 def test_norm_refusals_of_the_c_entry(kw, pat):
     """Every refusal comes before anything is launched: the pointers are never read."""
-    d, t = _norm(**kw), _lib.PairTensor(4096, 64, 64, 64)
-    with pytest.raises(ValueError, match=pat):
-        _lib.check(_lib.load().pair_sm100_add_norm(C.byref(d), C.byref(t), None, 4096, 4096, 4096, 4096, None), "add_norm")
+    d, t = _norm(**kw), Tensor4(4096, 64, 64, 64)
+    refused("pair_sm100_add_norm", pat, d, t, None, 4096, 4096, 4096, 4096, None)
     if "group" not in kw:
-        with pytest.raises(ValueError, match=pat):
-            _lib.check(_lib.load().pair_sm100_add_norm_grad(C.byref(d), C.byref(t), None, None, 4096, 4096, None, None, None, None), "grad")
+        refused("pair_sm100_add_norm_grad", pat, d, t, None, None, 4096, 4096, None, None, None, None)
 
 
 def test_norm_refusals_of_missing_buffers():
-    lib, d, t = _lib.load(), _norm(), _lib.PairTensor(4096, 64, 64, 64)
+    d, t = _norm(), Tensor4(4096, 64, 64, 64)
     for args, pat in (((None, 4096, 4096, None, None), "come together"), ((None, None, 4096, 4096, None), "come together"),
                       ((None, None, None, None, None), "no output")):
-        with pytest.raises(ValueError, match=pat):
-            _lib.check(lib.pair_sm100_add_norm(C.byref(d), C.byref(t), *args, None), "add_norm")
-    with pytest.raises(ValueError, match="update is NULL"):
-        _lib.check(lib.pair_sm100_add_norm(C.byref(d), None, None, 4096, 4096, 4096, None, None), "add_norm")
-    with pytest.raises(ValueError, match="needs y and scales"):
-        _lib.check(lib.pair_sm100_add_norm(C.byref(_norm(group=64)), C.byref(t), None, 4096, 4096, 4096, None, None), "add_norm")
+        refused("pair_sm100_add_norm", pat, d, t, *args, None)
+    refused("pair_sm100_add_norm", "update is NULL", d, None, None, 4096, 4096, 4096, None, None)
+    refused("pair_sm100_add_norm", "needs y and scales", _norm(group=64), t, None, 4096, 4096, 4096, None, None)
+    refused("pair_sm100_add_norm", "16-byte boundaries", _norm(group=32), Tensor4(4098, 64, 64, 64), None, 4096, 4096, 4096, 4096, None)
+    refused("pair_sm100_add_norm", "16-byte boundaries", _norm(group=32), Tensor4(4096, 64, 64, 65), None, 4096, 4096, 4096, 4096, None)
     for args, pat in (((None, 4096, 4096, 4096, 4096), "weight is NULL"), ((4096, None, None, None, None), "no output"),
                       ((4096, 4096, None, 4096, None), "workspace"), ((4096, 4096, None, 4096, 4100), "workspace")):
-        with pytest.raises(ValueError, match=pat):
-            _lib.check(lib.pair_sm100_add_norm_grad(C.byref(d), C.byref(t), None, None, *args, None), "grad")
+        refused("pair_sm100_add_norm_grad", pat, d, t, None, None, *args, None)
 
 
 @pytest.mark.parametrize("kw,pat", [
@@ -150,14 +180,11 @@ def test_norm_refusals_of_missing_buffers():
     (dict(table_dtype=5), "unknown type"),
 ])
 def test_embedding_refusals_of_the_c_entry(kw, pat):
-    d = _lib.PairEmbedDesc(10, 64, 5, 64, _lib.PAIR_BF16, _lib.PAIR_BF16, 1.0)
+    d = EmbedDesc(10, 64, 5, 64, BF16, BF16, 1.0)
     for k, v in kw.items():
         setattr(d, k, v)
-    lib = _lib.load()
-    with pytest.raises(ValueError, match=pat):
-        _lib.check(lib.pair_sm100_embed(C.byref(d), 4096, 4096, None, 4096, None), "embed")
-    with pytest.raises(ValueError, match=pat):
-        _lib.check(lib.pair_sm100_embed_grad(C.byref(d), 4096, 4096, 4096, 4096, None), "embed_grad")
+    refused("pair_sm100_embed", pat, d, 4096, 4096, None, 4096, None)
+    refused("pair_sm100_embed_grad", pat, d, 4096, 4096, 4096, 4096, None)
 
 
 def test_quotients_by_multiplication_are_exact():
@@ -192,7 +219,7 @@ def test_dropout_keeps_the_nearest_of_65536():
 def test_there_is_no_cpu_path():
     x, w = torch.zeros(2, 3, 4, 8), torch.ones(8)
     for call in (lambda: P.dropout_add(x, x), lambda: P.add_rms_norm(x, None, w), lambda: P.add_rms_norm_fp8(x, x, w, group=None),
-                 lambda: P.pair_embedding(torch.zeros(3, dtype=torch.int64), w[None]), lambda: PK.add_norm(x, x, None, x, None)):
+                 lambda: P.pair_embedding(torch.zeros(3, dtype=torch.int64), w[None])):
         with pytest.raises(ValueError, match="CUDA"):
             call()
 
