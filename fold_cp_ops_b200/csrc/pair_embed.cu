@@ -6,7 +6,7 @@
 // Bound.  Forward: HBM, base read and out written once; the table (tens of rows for position bins) stays in L1 and L2.
 // Gradient: HBM, d_out read once.  Position bins give some 10^6 tokens to each of a few dozen rows, vocabularies give
 // one or two, so the sum is organised by sorted tokens: a stable counting sort of the token numbers by index (up to
-// 2048 bins a pass, no comparison, int32 numbers only), then every group of lanes sums the d_out rows of an equal share
+// 2048 bins a pass, no comparison, pairs of int32 only), then every group of lanes sums the d_out rows of an equal share
 // of the SORTED tokens.  A run of equal indices inside one share goes straight to the table; a run that crosses
 // shares leaves its pieces in the workspace, and the share in which it begins adds them up afterwards.  No atomics: the
 // same bits every time, whatever the distribution.
@@ -200,10 +200,14 @@ __global__ void __launch_bounds__(kThreads) embed_grad_few_kernel(IndexView inde
 // ---------------------------------------------------------------------------------------------
 // The tokens are cut into `tiles` equal tiles, one per warp.  Pass: count each tile's digits (counts[bin][tile]), scan
 // every bin over the tiles, then place each token behind its bin's, its tile's and its own predecessors.
+struct Entry {
+  uint32_t token, key;  // key: the token's table row, or the number of rows where it has none
+};
+
 struct SortArgs {
   IndexView index;
-  const uint32_t* in;  // token numbers in the order of the passes so far; nullptr: 0, 1, 2, ...
-  uint32_t* out;
+  const Entry* in;  // the order of the passes so far; nullptr: tokens 0, 1, 2, ...
+  Entry* out;
   uint32_t* counts;  // (bins, tiles)
   uint32_t* totals;  // (bins)
   uint32_t tokens, tiles, tile;
@@ -213,12 +217,17 @@ struct SortArgs {
 };
 
 // Tokens without an embedding sort behind all others: their key is the number of rows.
-__device__ __forceinline__ uint32_t digit_of(const SortArgs& a, uint32_t t) {
-  const uint32_t key = a.index.at(t);
-  return ((key == kNone ? a.index.rows : key) >> a.shift) & (a.bins - 1);
+__device__ __forceinline__ Entry entry_of(const SortArgs& a, uint32_t p) {
+  if (a.in != nullptr) {
+    const uint2 e = __ldg(reinterpret_cast<const uint2*>(a.in) + p);
+    return Entry{e.x, e.y};
+  }
+  const uint32_t row = a.index.at(p);
+  return Entry{p, row == kNone ? a.index.rows : row};
 }
 
 __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortArgs a) {
+  behind_previous();
   extern __shared__ uint32_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t* mine = smem + warp * a.bins;
@@ -236,7 +245,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortA
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t p = p0 + k * 32 + lane;
-      digit[k] = p < hi ? digit_of(a, a.in != nullptr ? a.in[p] : p) : kNone;
+      digit[k] = p < hi ? (entry_of(a, p).key >> a.shift) & (a.bins - 1) : kNone;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -248,37 +257,42 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortA
   for (int k = lane; k < a.bins; k += 32) a.counts[static_cast<int64_t>(k) * a.tiles + w] = mine[k];
 }
 
-// Exclusive scan of one bin's counts over the tiles; the bin's total beside it.
+// Exclusive scan of one bin's counts over the tiles, a run of neighbours per thread; the bin's total beside it.
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(uint32_t* counts, uint32_t* totals, uint32_t tiles) {
+  behind_previous();
   __shared__ uint32_t part[kThreads / 32];
   uint32_t* c = counts + static_cast<int64_t>(blockIdx.x) * tiles;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t carry = 0;
-  for (uint32_t base = 0; base < tiles; base += kThreads) {
-    const uint32_t at = base + threadIdx.x;
-    const uint32_t own = at < tiles ? c[at] : 0;
-    uint32_t x = own;
+  const uint32_t per = (tiles + kThreads - 1) / kThreads;
+  const uint32_t lo = min(tiles, threadIdx.x * per), hi = min(tiles, lo + per);
+  uint32_t own = 0;
+#pragma unroll 8
+  for (uint32_t k = lo; k < hi; ++k) own += c[k];
+  uint32_t x = own;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t up = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += up;
-    }
-    if (lane == 31) part[warp] = x;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
-#pragma unroll
-    for (int k = 0; k < kThreads / 32; ++k) {
-      if (k < warp) before += part[k];
-      all += part[k];
-    }
-    if (at < tiles) c[at] = carry + before + x - own;
-    carry += all;
-    __syncthreads();
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t up = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += up;
   }
-  if (threadIdx.x == 0) totals[blockIdx.x] = carry;
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  uint32_t before = x - own, all = 0;
+#pragma unroll
+  for (int k = 0; k < kThreads / 32; ++k) {
+    if (k < warp) before += part[k];
+    all += part[k];
+  }
+#pragma unroll 8
+  for (uint32_t k = lo; k < hi; ++k) {
+    const uint32_t n = c[k];
+    c[k] = before;
+    before += n;
+  }
+  if (threadIdx.x == 0) totals[blockIdx.x] = all;
 }
 
 __global__ void __launch_bounds__(kSortWarps * 32) sort_place_kernel(const SortArgs a) {
+  behind_previous();
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t part[kSortWarps];
   uint32_t* first = smem + kSortWarps * a.bins;  // where each bin begins
@@ -312,12 +326,16 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_place_kernel(const SortA
   __syncwarp();
   const uint32_t lo = min(a.tokens, w * a.tile), hi = min(a.tokens, lo + a.tile);
   for (uint32_t p0 = lo; p0 < hi; p0 += 128) {
-    uint32_t token[4], digit[4];
+    Entry entry[4];
+    uint32_t digit[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint32_t p = p0 + k * 32 + lane;
-      token[k] = p < hi ? (a.in != nullptr ? a.in[p] : p) : kNone;
-      digit[k] = p < hi ? digit_of(a, token[k]) : kNone;
+      digit[k] = kNone;
+      if (p < hi) {
+        entry[k] = entry_of(a, p);
+        digit[k] = (entry[k].key >> a.shift) & (a.bins - 1);
+      }
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
@@ -325,7 +343,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_place_kernel(const SortA
       const uint32_t at = digit[k] != kNone ? next[digit[k]] : 0;
       __syncwarp();
       if (digit[k] != kNone) {
-        a.out[at + __popc(same & ((1u << lane) - 1))] = token[k];
+        a.out[at + __popc(same & ((1u << lane) - 1))] = entry[k];
         if (lane == __ffs(same) - 1) next[digit[k]] = at + __popc(same);
       }
       __syncwarp();
@@ -348,27 +366,33 @@ constexpr uint32_t kFromLeft = 1, kToRight = 2, kOneRun = 4;
 
 template <typename T>
 struct SumArgs {
-  IndexView index;
-  const uint32_t* sorted;
+  const Entry* sorted;
   const T* d_out;
   void* d_table;
   float* pieces;  // (CTAs, 2, width): what crosses into the CTA, and what begins in it and crosses out
   Edge* edges;    // (CTAs)
-  uint32_t tokens, share, ctas;
+  uint32_t tokens, rows, share, ctas;
   int d, width, table_dtype;
   float scale;
-  __device__ __forceinline__ uint32_t key(uint32_t p) const { return index.at(sorted[p]); }
 };
 
+// Four entries at a time are a batch.  The rows of octs of 16-bit types travel through a ring of two batches of asynchronous
+// copies per lane; others are loaded when their batch is at hand.  Four CTAs an SM with two batches take 30 us for 768 x 768
+// positions of 128 channels, three CTAs with three 34, two with four 40 (and two waves of any more than one).
+constexpr int kBatch = 4, kSumRing = 2, kSumCtas = 4;
+template <typename T, bool kWide>
+constexpr bool kSumStaged = kWide && sizeof(T) == 2;
+
 template <typename T, int kGroup, bool kWide>
-__global__ void __launch_bounds__(kThreads, 3) sum_runs_kernel(const SumArgs<T> a) {
-  constexpr int kAhead = kWide ? 8 : 4;  // rows of d_out in flight per lane
+__global__ void __launch_bounds__(kThreads, kSumCtas) sum_runs_kernel(const SumArgs<T> a) {
+  behind_previous();
   constexpr int kGroups = kThreads / kGroup;
   constexpr int kChannels = kGroup * 8;
+  constexpr bool kStaged = kSumStaged<T, kWide>;
   __shared__ float piece[2][kGroups][kChannels];
   __shared__ Edge edge[kGroups];
+  extern __shared__ uint4 ring[];
   const int lane = threadIdx.x % kGroup, group = threadIdx.x / kGroup;
-  const uint32_t mask = kGroup == 32 ? 0xffffffffu : ((1u << (kGroup & 31)) - 1) << ((threadIdx.x & 31) / kGroup * kGroup);
   const uint32_t share = blockIdx.x * kGroups + group;
   const int slab = blockIdx.y * kSlab, left = a.d - slab;
   // 64 bits: the last CTA's shares may begin behind 2^32
@@ -376,71 +400,162 @@ __global__ void __launch_bounds__(kThreads, 3) sum_runs_kernel(const SumArgs<T> 
   const uint32_t lo = begin < a.tokens ? static_cast<uint32_t>(begin) : a.tokens;
   const uint32_t hi = min(a.tokens, lo + a.share);
 
-  if (lo < hi) {
-    float total[8], acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) total[e] = acc[e] = 0.f;
-    const uint32_t first = a.key(lo);
-    const bool crosses_in = lo > 0 && a.key(lo - 1) == first;
-    const uint32_t next = hi < a.tokens ? a.key(hi) : kNone;
-    uint32_t run = first;  // index of the run at hand
-    bool from_left = crosses_in, one = true;
-
-    for (uint32_t p0 = lo; p0 < hi; p0 += kGroup) {
-      const uint32_t p = p0 + lane;
-      const uint32_t my_token = p < hi ? a.sorted[p] : 0;
-      const uint32_t my_key = p < hi ? a.index.at(my_token) : kNone;
-      const int here = min(static_cast<uint32_t>(kGroup), hi - p0);
-      for (int e0 = 0; e0 < here; e0 += kAhead) {
-        Unit<T, 8> o[kAhead];
-        uint32_t key[kAhead];
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          const uint32_t t = __shfl_sync(mask, my_token, e0 + k, kGroup);
-          key[k] = __shfl_sync(mask, my_key, e0 + k, kGroup);
-          o[k] = key[k] != kNone ? load_eight<kWide, kGroup>(a.d_out + static_cast<int64_t>(t) * a.d + slab, lane, left)
-                                 : zero_unit<T, 8>();
-        }
-#pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-          if (e0 + k < here) {
-            if (key[k] != run) {
-              if (from_left) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) piece[0][group][channel_of<kWide, kGroup>(lane, e)] = total[e] + acc[e];
-              } else {
-                float f[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = (total[e] + acc[e]) * a.scale;
-                store_eight<kWide, kGroup>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + slab, lane, left, f);
-              }
-              run = key[k];
-              from_left = one = false;
-#pragma unroll
-              for (int e = 0; e < 8; ++e) total[e] = acc[e] = 0.f;
-            }
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += to_f32(o[k].e[e]);
-          }
-        }
+  // The groups of a warp stay together: the loop is as long for a group whose share is short or empty (its entries have no table
+  // row then), and only what a run's end writes is done by some groups alone.
+  struct Batch {
+    uint32_t token[kBatch], key[kBatch];
+  };
+  auto entries_of = [&](uint32_t q) {  // of the share's entries q .. q + 3; q, the share and its begin are multiples of 4
+    Batch b;
+    uint4 x = make_uint4(0, a.rows, 0, a.rows), y = x;
+    if (q < a.share && lo + q < hi) {  // (behind the last token there is padding)
+      x = __ldg(reinterpret_cast<const uint4*>(a.sorted + lo + q));
+      y = __ldg(reinterpret_cast<const uint4*>(a.sorted + lo + q) + 1);
+      if (hi - (lo + q) < kBatch) {
+        y.w = a.rows;
+        if (hi - (lo + q) < 3) y.y = a.rows;
+        if (hi - (lo + q) < 2) x.w = a.rows;
       }
-      // sums of at most 32 terms first: the error grows with the root of either count
-#pragma unroll
-      for (int e = 0; e < 8; ++e) total[e] += acc[e], acc[e] = 0.f;
     }
-    const bool to_right = run != kNone && next == run;
-    if (from_left || to_right) {
+    b.token[0] = x.x, b.token[1] = x.z, b.token[2] = y.x, b.token[3] = y.z;
+    b.key[0] = x.y, b.key[1] = x.w, b.key[2] = y.y, b.key[3] = y.w;
+    return b;
+  };
+  const T* const d_out = a.d_out + slab;
+  auto fetch = [&](const Batch& b, int stage) {
+    if constexpr (kStaged) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) piece[from_left ? 0 : 1][group][channel_of<kWide, kGroup>(lane, e)] = total[e];
-    } else if (run != kNone) {
+      for (int k = 0; k < kBatch; ++k)
+        if (b.key[k] != a.rows && lane * 8 < left)
+          stage_unit<T, 8>(ring + (stage * kBatch + k) * kThreads + threadIdx.x,
+                           d_out + static_cast<int64_t>(b.token[k]) * a.d + lane * 8);
+      stage_commit();
+    }
+  };
+
+  // keys of the batches whose copies are under way, the one at hand first, and the entries of the batch after them
+  constexpr int kAhead = kStaged ? kSumRing - 1 : 1;
+  uint32_t key[kAhead][kBatch];
+  Batch next;
+#pragma unroll
+  for (int k = 0; k < kAhead; ++k) {
+    next = entries_of(k * kBatch);
+    fetch(next, k);
+#pragma unroll
+    for (int e = 0; e < kBatch; ++e) key[k][e] = next.key[e];
+  }
+  if constexpr (kStaged) next = entries_of(kAhead * kBatch);
+
+  float2 total[4], acc[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) total[e] = acc[e] = both(0.f);
+  const uint32_t before = lo > 0 && lo < hi ? a.sorted[lo - 1].key : a.rows;
+  const uint32_t after = lo < hi && hi < a.tokens ? a.sorted[hi].key : a.rows;
+  const uint32_t first = key[0][0];
+  const bool crosses_in = first != a.rows && before == first;
+  uint32_t run = first;  // the run at hand
+  bool from_left = crosses_in, one = true;
+
+  auto end_run = [&] {
+    if (from_left) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        piece[0][group][channel_of<kWide, kGroup>(lane, 2 * e)] = total[e].x + acc[e].x;
+        piece[0][group][channel_of<kWide, kGroup>(lane, 2 * e + 1)] = total[e].y + acc[e].y;
+      }
+    } else {
       float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = total[e] * a.scale;
+      for (int e = 0; e < 4; ++e) {
+        f[2 * e] = (total[e].x + acc[e].x) * a.scale;
+        f[2 * e + 1] = (total[e].y + acc[e].y) * a.scale;
+      }
       store_eight<kWide, kGroup>(a.d_table, a.table_dtype, static_cast<int64_t>(run) * a.d + slab, lane, left, f);
+    }
+  };
+  auto add = [&](const Unit<T, 8>& o) {
+    const Vals<8> v = unpack(o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] = __fadd2_rn(acc[e], v.p[e]);
+  };
+
+  int stage = 0;
+#pragma unroll 1
+  for (uint32_t q = 0; q < a.share; q += kBatch) {
+    if constexpr (kStaged) {
+      fetch(next, stage == 0 ? kSumRing - 1 : stage - 1);
+      stage_wait<kSumRing - 1>();
+    }
+    const uint4* slot = ring + stage * kBatch * kThreads + threadIdx.x;
+    bool same = true;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) same = same && key[0][k] == run;
+    if (__all_sync(0xffffffffu, same)) {
+      if (run != a.rows) {
+        Unit<T, 8> o[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          if constexpr (kStaged)  // (lanes behind the row's end add what their slot holds: those sums go nowhere)
+            o[k] = staged_unit<T, 8>(slot + k * kThreads);
+          else
+            o[k] = load_eight<kWide, kGroup>(d_out + static_cast<int64_t>(next.token[k]) * a.d, lane, left);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) add(o[k]);
+      }
+    } else {
+#pragma unroll 1
+      for (uint32_t k = 0; k < kBatch && lo + q + k < hi; ++k) {
+        const Entry e = a.sorted[lo + q + k];
+        if (e.key != run) {
+          if (run != a.rows) end_run();
+          run = e.key;
+          from_left = one = false;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) total[c] = acc[c] = both(0.f);
+        }
+        if (run != a.rows) {
+          if constexpr (kStaged)
+            add(staged_unit<T, 8>(slot + k * kThreads));
+          else
+            add(load_eight<kWide, kGroup>(d_out + static_cast<int64_t>(e.token) * a.d, lane, left));
+        }
+      }
+    }
+    // sums of at most 32 terms first: the error grows with the root of either count
+    if ((q / kBatch & 7) == 7) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) total[e] = __fadd2_rn(total[e], acc[e]), acc[e] = both(0.f);
+    }
+    if constexpr (kStaged) {
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+        for (int e = 0; e < kBatch; ++e) key[k][e] = k + 1 < kAhead ? key[k + 1 < kAhead ? k + 1 : 0][e] : next.key[e];
+      next = entries_of(q + (kAhead + 1) * kBatch);
+      stage = stage == kSumRing - 1 ? 0 : stage + 1;
+    } else {
+      next = entries_of(q + kBatch);
+#pragma unroll
+      for (int e = 0; e < kBatch; ++e) key[0][e] = next.key[e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) total[e] = __fadd2_rn(total[e], acc[e]), acc[e] = both(0.f);
+  if (lo < hi) {
+    const bool to_right = run != a.rows && after == run;
+    if (to_right && !from_left) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        piece[1][group][channel_of<kWide, kGroup>(lane, 2 * e)] = total[e].x;
+        piece[1][group][channel_of<kWide, kGroup>(lane, 2 * e + 1)] = total[e].y;
+      }
+    } else if (run != a.rows) {
+      end_run();
     }
     if (lane == 0) edge[group] = Edge{first, run, (crosses_in ? kFromLeft : 0) | (to_right ? kToRight : 0) | (one ? kOneRun : 0), 0};
   } else if (lane == 0) {
-    edge[group] = Edge{kNone, kNone, kOneRun, 0};
+    edge[group] = Edge{a.rows, a.rows, kOneRun, 0};
   }
   __syncthreads();
 
@@ -452,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 3) sum_runs_kernel(const SumArgs<T> 
     bool open = false;
     for (int g = 0; g < kGroups; ++g) {
       const Edge s = edge[g];
-      if (s.first == kNone) break;  // tokens without an embedding, or behind the last one
+      if (s.first == a.rows) break;  // tokens without an embedding, or behind the last one
       if (s.bits & kFromLeft) {
         if (g == 0) before = true;
         sum += piece[0][g][c];
@@ -490,6 +605,7 @@ __global__ void __launch_bounds__(kThreads, 3) sum_runs_kernel(const SumArgs<T> 
 // The CTA in which a crossing run begins adds up its pieces: its own [1], then [0] of the CTAs that follow.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_runs_kernel(const SumArgs<T> a) {
+  behind_previous();
   __shared__ float4 sums[kThreads / 32][32];
   const uint32_t cta = blockIdx.x;
   const Edge own = a.edges[cta];
@@ -564,19 +680,20 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   if (tiles > most) tiles = most;
   p.tile = static_cast<uint32_t>(((tokens + tiles - 1) / tiles + 31) / 32 * 32);
   p.tiles = static_cast<uint32_t>((tokens + p.tile - 1) / p.tile);
-  // shares: one wave of resident groups (three CTAs an SM over all slabs), of at least 8 tokens
+  // shares: one wave of resident groups over all slabs, of at least 8 tokens, in whole batches
   p.group = d->d <= 64 ? 8 : d->d <= 128 ? 16 : 32;
   p.width = (d->d + 7) / 8 * 8;
   const int held = kThreads / p.group;
-  uint64_t ctas = static_cast<uint64_t>(sms) * 3 / p.slabs;
+  uint64_t ctas = static_cast<uint64_t>(sms) * kSumCtas / p.slabs;
   if (ctas < 1) ctas = 1;
   uint64_t share = (tokens + ctas * held - 1) / (ctas * held);
   if (share < 8) share = 8;
+  share = (share + kBatch - 1) / kBatch * kBatch;
   p.share = static_cast<uint32_t>(share);
   p.ctas = static_cast<uint32_t>((tokens + share * held - 1) / (share * held));
   uint64_t at = 0;
-  p.sorted_at[0] = at, at += up256(tokens * 4);
-  p.sorted_at[1] = at, at += p.passes > 1 ? up256(tokens * 4) : 0;
+  p.sorted_at[0] = at, at += up256(tokens * sizeof(Entry));
+  p.sorted_at[1] = at, at += p.passes > 1 ? up256(tokens * sizeof(Entry)) : 0;
   p.counts_at = at, at += up256(static_cast<uint64_t>(p.bins) * p.tiles * 4);
   p.totals_at = at, at += up256(static_cast<uint64_t>(p.bins) * 4);
   p.pieces_at = at, at += up256(static_cast<uint64_t>(p.ctas) * 2 * p.width * 4);
@@ -644,19 +761,21 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   const unsigned grid = (p.tiles + kSortWarps - 1) / kSortWarps;
   for (int pass = 0; pass < p.passes; ++pass) {
     // the last pass ends in buffer 0
-    a.out = reinterpret_cast<uint32_t*>(ws + p.sorted_at[(p.passes - 1 - pass) & 1]);
+    a.out = reinterpret_cast<Entry*>(ws + p.sorted_at[(p.passes - 1 - pass) & 1]);
     a.shift = pass * p.digit_bits;
-    sort_count_kernel<<<grid, kSortWarps * 32, count_smem, s>>>(a);
-    sort_scan_kernel<<<p.bins, kThreads, 0, s>>>(a.counts, a.totals, a.tiles);
-    sort_place_kernel<<<grid, kSortWarps * 32, place_smem, s>>>(a);
-    e = cudaGetLastError();
+    // clearing takes every SM, whatever the tiles need
+    const unsigned busy = a.clear != nullptr && grid < 4u * sms ? 4u * sms : grid;
+    e = pass == 0 ? launch(sort_count_kernel, busy, kSortWarps * 32, count_smem, s, a)
+                  : launch_behind(sort_count_kernel, busy, kSortWarps * 32, count_smem, s, a);
+    if (e == cudaSuccess) e = launch_behind(sort_scan_kernel, p.bins, kThreads, 0, s, a.counts, a.totals, a.tiles);
+    if (e == cudaSuccess) e = launch_behind(sort_place_kernel, grid, kSortWarps * 32, place_smem, s, a);
     if (e != cudaSuccess) return e;
     a.in = a.out;
     a.clear = nullptr;
   }
   SumArgs<T> m;
-  m.index = index;
   m.sorted = a.in;
+  m.rows = static_cast<uint32_t>(d->rows);
   m.d_out = static_cast<const T*>(d_out);
   m.d_table = d_table;
   m.pieces = reinterpret_cast<float*>(ws + p.pieces_at);
@@ -669,16 +788,16 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   m.table_dtype = d->table_dtype;
   m.scale = d->scale;
   const dim3 sum_grid(p.ctas, p.slabs);
-  if (p.group == 8)
-    sum_runs_kernel<T, 8, kWide><<<sum_grid, kThreads, 0, s>>>(m);
-  else if (p.group == 16)
-    sum_runs_kernel<T, 16, kWide><<<sum_grid, kThreads, 0, s>>>(m);
-  else
-    sum_runs_kernel<T, 32, kWide><<<sum_grid, kThreads, 0, s>>>(m);
-  e = cudaGetLastError();
+  const int smem = kSumStaged<T, kWide> ? kSumRing * kBatch * kThreads * 16 : 0;
+  auto kernel = p.group == 8 ? sum_runs_kernel<T, 8, kWide> : p.group == 16 ? sum_runs_kernel<T, 16, kWide> : sum_runs_kernel<T, 32, kWide>;
+  if (smem > 0) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  e = launch_behind(kernel, sum_grid, kThreads, smem, s, m);
   if (e != cudaSuccess) return e;
-  join_runs_kernel<T><<<dim3(p.ctas, (p.width + 127) / 128 < 4 ? (p.width + 127) / 128 : 4), kThreads, 0, s>>>(m);
-  return cudaGetLastError();
+  const int quads = (p.width + 127) / 128;
+  return launch_behind(join_runs_kernel<T>, dim3(p.ctas, quads < 4 ? quads : 4), kThreads, 0, s, m);
 }
 
 int check_embed_desc(const pair_embed_desc_t* d, const char* who) {

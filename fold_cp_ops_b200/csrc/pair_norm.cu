@@ -322,7 +322,7 @@ cudaError_t launch_add(const NormArgs<T>& a, int sms, cudaStream_t s) {
 }
 
 template <typename T, int kU, int kGroup, int kUnits, int kMode>
-cudaError_t launch(const NormArgs<T>& a, int sms, cudaStream_t stream) {
+cudaError_t launch_rows(const NormArgs<T>& a, int sms, cudaStream_t stream) {
   constexpr uint32_t kWide = threads_of(kGroup), kRows = kWide / kGroup;
   auto kernel = add_norm_kernel<T, kU, kGroup, kUnits, kMode>;
   const bool has_residual = a.residual.p != nullptr;
@@ -345,27 +345,27 @@ cudaError_t launch(const NormArgs<T>& a, int sms, cudaStream_t stream) {
 template <typename T, int kMode>
 cudaError_t wide_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
   const int o = a.octs;
-  if (o <= 8) return launch<T, 8, 8, 1, kMode>(a, sms, s);
-  if (o <= 16) return launch<T, 8, 16, 1, kMode>(a, sms, s);
-  if (o <= 32) return launch<T, 8, 32, 1, kMode>(a, sms, s);
-  if (o <= 48) return launch<T, 8, 16, 3, kMode>(a, sms, s);
-  if (o <= 64) return launch<T, 8, 32, 2, kMode>(a, sms, s);
-  if (o <= 128) return launch<T, 8, 128, 1, kMode>(a, sms, s);
-  if (o <= 256) return launch<T, 8, 256, 1, kMode>(a, sms, s);
-  if (o <= 512) return launch<T, 8, 512, 1, kMode>(a, sms, s);
-  return launch<T, 8, 1024, 1, kMode>(a, sms, s);
+  if (o <= 8) return launch_rows<T, 8, 8, 1, kMode>(a, sms, s);
+  if (o <= 16) return launch_rows<T, 8, 16, 1, kMode>(a, sms, s);
+  if (o <= 32) return launch_rows<T, 8, 32, 1, kMode>(a, sms, s);
+  if (o <= 48) return launch_rows<T, 8, 16, 3, kMode>(a, sms, s);
+  if (o <= 64) return launch_rows<T, 8, 32, 2, kMode>(a, sms, s);
+  if (o <= 128) return launch_rows<T, 8, 128, 1, kMode>(a, sms, s);
+  if (o <= 256) return launch_rows<T, 8, 256, 1, kMode>(a, sms, s);
+  if (o <= 512) return launch_rows<T, 8, 512, 1, kMode>(a, sms, s);
+  return launch_rows<T, 8, 1024, 1, kMode>(a, sms, s);
 }
 
 // Units of one or two channels: four or eight channels per lane of a warp, then of a CTA.
 template <typename T, int kU, int kMode>
 cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
-  if (a.d <= 128) return launch<T, kU, 32, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 256) return launch<T, kU, 32, 8 / kU, kMode>(a, sms, s);
-  if (a.d <= 512) return launch<T, kU, 128, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 1024) return launch<T, kU, 256, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 2048) return launch<T, kU, 512, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 4096) return launch<T, kU, 1024, 4 / kU, kMode>(a, sms, s);
-  return launch<T, kU, 1024, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 128) return launch_rows<T, kU, 32, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 256) return launch_rows<T, kU, 32, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 512) return launch_rows<T, kU, 128, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 1024) return launch_rows<T, kU, 256, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 2048) return launch_rows<T, kU, 512, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 4096) return launch_rows<T, kU, 1024, 4 / kU, kMode>(a, sms, s);
+  return launch_rows<T, kU, 1024, 8 / kU, kMode>(a, sms, s);
 }
 
 template <typename T, int kMode>

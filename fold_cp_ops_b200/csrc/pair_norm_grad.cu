@@ -165,6 +165,7 @@ __global__ void __launch_bounds__(threads_of(kGroup)) norm_grad_kernel(const __g
 constexpr int kJoinChannels = 16, kJoinRows = 64;
 __global__ void __launch_bounds__(kJoinChannels* kJoinRows) join_weight_kernel(const double* partial, int parts, int d,
                                                                               void* d_weight, int dtype) {
+  behind_previous();
   __shared__ double s[kJoinRows][kJoinChannels + 1];
   const int x = threadIdx.x % kJoinChannels, y = threadIdx.x / kJoinChannels;
   const int c = blockIdx.x * kJoinChannels + x;
@@ -210,7 +211,7 @@ inline uint32_t grid_of(uint32_t rows, Shape w, int sms) {
 }
 
 template <typename T, int kU, int kGroup, int kUnits>
-cudaError_t launch(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream) {
+cudaError_t launch_rows(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream) {
   constexpr int kWide = threads_of(kGroup);
   const int smem = a.partial != nullptr ? kUnits * kU * kWide * static_cast<int>(sizeof(double)) : 0;
   if (smem > 48 * 1024) {
@@ -225,22 +226,22 @@ cudaError_t launch(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream) {
 template <typename T, int kU>
 cudaError_t by_shape(const GradArgs<T>& a, Shape w, uint32_t grid, cudaStream_t s) {
   if constexpr (kU == 8) {
-    if (w.group == 8) return launch<T, 8, 8, 1>(a, grid, s);
-    if (w.group == 16) return launch<T, 8, 16, 1>(a, grid, s);
-    if (w.group == 32 && w.channels == 8) return launch<T, 8, 32, 1>(a, grid, s);
-    if (w.group == 32) return launch<T, 8, 32, 2>(a, grid, s);
-    if (w.group == 128) return launch<T, 8, 128, 1>(a, grid, s);
-    if (w.group == 256) return launch<T, 8, 256, 1>(a, grid, s);
-    if (w.group == 512) return launch<T, 8, 512, 1>(a, grid, s);
-    return launch<T, 8, 1024, 1>(a, grid, s);
+    if (w.group == 8) return launch_rows<T, 8, 8, 1>(a, grid, s);
+    if (w.group == 16) return launch_rows<T, 8, 16, 1>(a, grid, s);
+    if (w.group == 32 && w.channels == 8) return launch_rows<T, 8, 32, 1>(a, grid, s);
+    if (w.group == 32) return launch_rows<T, 8, 32, 2>(a, grid, s);
+    if (w.group == 128) return launch_rows<T, 8, 128, 1>(a, grid, s);
+    if (w.group == 256) return launch_rows<T, 8, 256, 1>(a, grid, s);
+    if (w.group == 512) return launch_rows<T, 8, 512, 1>(a, grid, s);
+    return launch_rows<T, 8, 1024, 1>(a, grid, s);
   } else {
-    if (w.group == 32 && w.channels == 4) return launch<T, kU, 32, 4 / kU>(a, grid, s);
-    if (w.group == 32) return launch<T, kU, 32, 8 / kU>(a, grid, s);
-    if (w.group == 128) return launch<T, kU, 128, 4 / kU>(a, grid, s);
-    if (w.group == 256) return launch<T, kU, 256, 4 / kU>(a, grid, s);
-    if (w.group == 512) return launch<T, kU, 512, 4 / kU>(a, grid, s);
-    if (w.channels == 4) return launch<T, kU, 1024, 4 / kU>(a, grid, s);
-    return launch<T, kU, 1024, 8 / kU>(a, grid, s);
+    if (w.group == 32 && w.channels == 4) return launch_rows<T, kU, 32, 4 / kU>(a, grid, s);
+    if (w.group == 32) return launch_rows<T, kU, 32, 8 / kU>(a, grid, s);
+    if (w.group == 128) return launch_rows<T, kU, 128, 4 / kU>(a, grid, s);
+    if (w.group == 256) return launch_rows<T, kU, 256, 4 / kU>(a, grid, s);
+    if (w.group == 512) return launch_rows<T, kU, 512, 4 / kU>(a, grid, s);
+    if (w.channels == 4) return launch_rows<T, kU, 1024, 4 / kU>(a, grid, s);
+    return launch_rows<T, kU, 1024, 8 / kU>(a, grid, s);
   }
 }
 
@@ -278,9 +279,8 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* z, const pair_te
     if (unit == 1) e = by_shape<T, 1>(a, w, grid, s);
   }
   if (e != cudaSuccess || d_weight == nullptr) return e;
-  join_weight_kernel<<<(a.d + kJoinChannels - 1) / kJoinChannels, kJoinChannels * kJoinRows, 0, s>>>(
-      a.partial, static_cast<int>(grid), a.d, d_weight, d->weight_dtype);
-  return cudaGetLastError();
+  return launch_behind(join_weight_kernel, (a.d + kJoinChannels - 1) / kJoinChannels, kJoinChannels * kJoinRows, 0, s,
+                       static_cast<const double*>(a.partial), static_cast<int>(grid), a.d, d_weight, static_cast<int>(d->weight_dtype));
 }
 
 }  // namespace

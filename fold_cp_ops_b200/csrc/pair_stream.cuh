@@ -406,6 +406,37 @@ __device__ __forceinline__ void group_max(float (&v)[kN], float* buf, int parity
   group_merge<kGroup, kN, true>(v, buf, parity);
 }
 
+// Launches.  The kernels of one call follow one another: each says at its start that the next may be set up while it runs, and waits
+// there for the one before it to end (its results included), which hides the launch of all but the first.
+__device__ __forceinline__ void behind_previous() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+template <bool kBehind, typename K, typename... A>
+cudaError_t launch_kernel(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t c = {};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  c.attrs = &early;
+  c.numAttrs = kBehind ? 1 : 0;
+  return cudaLaunchKernelEx(&c, kernel, args...);
+}
+template <typename K, typename... A>
+cudaError_t launch(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
+  return launch_kernel<false>(kernel, grid, threads, smem, stream, args...);
+}
+// Behind a kernel of the same call; the kernel begins with behind_previous().
+template <typename K, typename... A>
+cudaError_t launch_behind(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
+  return launch_kernel<true>(kernel, grid, threads, smem, stream, args...);
+}
+
 // CTAs of a kernel that an SM holds at once (at least one).
 template <typename K>
 int resident_ctas(K kernel, int threads, int smem) {
