@@ -50,17 +50,34 @@ __device__ __forceinline__ uint32_t e4m3x2(float2 v) {
 // three 44, four 51).
 __host__ __device__ constexpr int ring_of(int lane_bytes) { return lane_bytes <= 16 ? 3 : 2; }
 
+// round(r + dropout(u)) of one oct.
+template <typename T>
+__device__ __forceinline__ Unit<T, 8> drop_and_add(const Dropout& d, uint32_t line, uint32_t b, uint32_t i, uint32_t j, uint32_t oct,
+                                                   const Unit<T, 8>& u, const Unit<T, 8>& r, bool has_residual) {
+  const Unit<T, 8> in[1] = {u}, other[1] = {r};
+  Lane<8, 1> v = unpack_all<T, 8, 1>(in);
+  drop_oct(draw_oct(d, b, i, j, oct), line, d.gain, v.p);
+  if (has_residual) {
+    const Lane<8, 1> x = unpack_all<T, 8, 1>(other);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
+  }
+  Unit<T, 8> out[1];
+  pack_all<T, 8, 1>(v, out);
+  return out[0];
+}
+
 // kU channels per access, kGroup lanes per row, kUnits units per lane.
 template <typename T, int kU, int kGroup, int kUnits, int kMode>
-__global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup)) add_norm_kernel(const __grid_constant__ NormArgs<T> a) {
+__global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 1024) / threads_of(kGroup)) add_norm_kernel(const __grid_constant__ NormArgs<T> a) {
   __shared__ float sums[2 * 32];
   __shared__ float tops[2 * 32];
   extern __shared__ uint4 ring[];
   constexpr int kWide = threads_of(kGroup);
   constexpr int kRows = kWide / kGroup;  // rows a CTA holds side by side
-  constexpr int kPairs = (kU + 1) / 2;
-  constexpr int kBytes = sizeof(T) * kU;
-  constexpr int kRing = ring_of(kUnits * kBytes);
+  constexpr int kPairs = kU * kUnits / 2;
+  using In = Rows<T, kU, kGroup, kUnits>;
+  constexpr int kRing = ring_of(In::kStage / kWide);
   const int lane = threadIdx.x % kGroup;
   const int units = a.d / kU;
   const bool dropping = a.drop.keep < 65536u;
@@ -69,77 +86,73 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
   Dropout drop = a.drop;
   if (dropping) resolve_seed(drop);
 
-  Vals<kU> w[kMode == kAdd ? 1 : kUnits];
-  if constexpr (kMode != kAdd) {
-#pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      float f[kPairs * 2];
-#pragma unroll
-      for (int e = 0; e < kPairs * 2; ++e) {
-        const int n = lane + k * kGroup;
-        f[e] = n < units && e < kU ? load_any(a.weight, n * kU + e, a.weight_dtype) : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < kPairs; ++e) w[k].p[e] = make_float2(f[2 * e], f[2 * e + 1]);
-    }
-  }
+  Lane<kU, kUnits> w;
+  if constexpr (kMode != kAdd) w = load_gain<kU, kGroup, kUnits>(a.weight, a.weight_dtype, lane, units);
 
   const uint32_t span = gridDim.x * kRows;
-  auto rows_of = [&](uint32_t row, const T*& up, const T*& rp) {
+  const uint32_t mine = blockIdx.x * kRows + threadIdx.x / kGroup;  // this group's first row
+  // rows at a constant distance are reached step by step, others by their (b, i, j)
+  const T *next_u = a.update.flat(mine), *next_r = a.residual.flat(mine);
+  const int64_t step_u = span * a.update.sj, step_r = span * a.residual.sj;
+  auto next_rows = [&](uint32_t row, const T*& up, const T*& rp) {
     if (a.flat) {
-      up = a.update.flat(row);
-      rp = a.residual.flat(row);
-    } else {
+      up = next_u, rp = next_r;
+      next_u += step_u, next_r += step_r;
+    } else if (row < a.rows) {
       uint32_t b, i, j;
       a.walk.at(row, b, i, j);
       up = a.update.row(b, i, j);
       rp = a.residual.row(b, i, j);
     }
   };
-  // one stage: the update's units, then the residual's, each kWide lanes side by side
-  const int stage_bytes = kUnits * kWide * kBytes * (has_residual ? 2 : 1);
-  char* const slots = reinterpret_cast<char*>(ring) + threadIdx.x * kBytes;
-  auto fetch = [&](uint32_t row, char* slot) {
+  // one stage: the update's row of every group, then the residual's
+  const int stage_bytes = In::kStage * (has_residual ? 2 : 1);
+  char* const stages = reinterpret_cast<char*>(ring);
+  char *from = stages, *to = stages;  // the stages that are read and copied into next
+  auto advance = [&](char*& stage) {
+    stage += stage_bytes;
+    if (stage == stages + kRing * stage_bytes) stage = stages;
+  };
+  auto fetch = [&](uint32_t row) {
+    const T *up, *rp;
+    next_rows(row, up, rp);
     if (row < a.rows) {
-      const T *up, *rp;
-      rows_of(row, up, rp);
-#pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        const int n = lane + k * kGroup;
-        if (n < units) {
-          stage_unit<T, kU>(slot + k * kWide * kBytes, up + n * kU);
-          if (has_residual) stage_unit<T, kU>(slot + (kUnits + k) * kWide * kBytes, rp + n * kU);
-        }
-      }
+      In::fetch(to, up, a.d);
+      if (has_residual) In::fetch(to + In::kStage, rp, a.d);
     }
     stage_commit();
+    advance(to);
   };
 
-  const uint32_t mine = threadIdx.x / kGroup;
-  if constexpr (kCanStage<T, kU>) {
+  if constexpr (In::kStaged) {
 #pragma unroll
-    for (int s = 0; s < kRing - 1; ++s) fetch(blockIdx.x * kRows + mine + s * span, slots + s * stage_bytes);
+    for (int s = 0; s < kRing - 1; ++s) fetch(mine + s * span);
   }
-  int parity = 0, stage = 0;
+  int parity = 0;
+  const int64_t out_step = static_cast<int64_t>(span) * a.d, scale_step = static_cast<int64_t>(span) * a.scales_per_row;
+  int64_t out = static_cast<int64_t>(mine) * a.d + lane * kU;  // the lane's first channel
+  int64_t scale_row = static_cast<int64_t>(mine) * a.scales_per_row;
   // the bound is the CTA's first row: lanes whose row lies behind the end still take part in the reductions
-  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += span, parity ^= 1) {
-    const uint32_t row = first + mine;
+  uint32_t row = mine;
+  for (uint32_t first = blockIdx.x * kRows; first < a.rows;
+       first += span, row += span, parity ^= 1, out += out_step, scale_row += scale_step) {
     const bool valid = row < a.rows;
+    // octs are not cleared where a lane has none: their sums are left out instead
+    constexpr bool kClear = kU < 8 || !In::kStaged;
     Unit<T, kU> u[kUnits], r[kUnits];
-    if constexpr (kCanStage<T, kU>) {
-      fetch(row + (kRing - 1) * span, slots + ((stage + kRing - 1) % kRing) * stage_bytes);
+    if constexpr (In::kStaged) {
+      fetch(row + (kRing - 1) * span);
       stage_wait<kRing - 1>();
-      const char* slot = slots + stage * stage_bytes;
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
-        const bool on = valid && lane + k * kGroup < units;
-        u[k] = on ? staged_unit<T, kU>(slot + k * kWide * kBytes) : zero_unit<T, kU>();
-        r[k] = on && has_residual ? staged_unit<T, kU>(slot + (kUnits + k) * kWide * kBytes) : zero_unit<T, kU>();
+        const bool on = !kClear || (valid && lane + k * kGroup < units);
+        u[k] = on ? In::read(from, k) : zero_unit<T, kU>();
+        r[k] = on && has_residual ? In::read(from + In::kStage, k) : zero_unit<T, kU>();
       }
-      stage = (stage + 1) % kRing;
+      advance(from);
     } else {
       const T *up = nullptr, *rp = nullptr;
-      if (valid) rows_of(row, up, rp);
+      next_rows(row, up, rp);
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
         const int n = lane + k * kGroup;
@@ -152,74 +165,67 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
     if (dropping) {
       uint32_t b, i, j;
       a.walk.at(valid ? row : 0, b, i, j);
-      if constexpr (kU == 8) {
+      if constexpr (kU == 8) {  // oct by oct: fewer values at a time
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          Vals<8> v = unpack(u[k]);
-          drop_oct(draw_oct(drop, b, i, j, lane + k * kGroup), line, drop.gain, v);
-          const Vals<8> x = unpack(r[k]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
-          u[k] = pack<T, 8>(v);
-        }
+        for (int k = 0; k < kUnits; ++k) u[k] = drop_and_add<T>(drop, line, b, i, j, lane + k * kGroup, u[k], r[k], has_residual);
       } else {
-        const auto mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b, i, j, lane & ~31, a.octs);
+        Lane<kU, kUnits> v = unpack_all<T, kU, kUnits>(u);
+        drop_all<kU, kGroup, kUnits>(drop, line, b, i, j, lane, a.octs, v);
+        const Lane<kU, kUnits> x = unpack_all<T, kU, kUnits>(r);
 #pragma unroll
-        for (int k = 0; k < kUnits; ++k) {
-          const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
-          Vals<kU> v = unpack(u[k]);
-          v.p[0].x = bits & 1u ? v.p[0].x * drop.gain : 0.f;
-          if constexpr (kU > 1) v.p[0].y = bits & 2u ? v.p[0].y * drop.gain : 0.f;
-          const Vals<kU> x = unpack(r[k]);
-          v.p[0] = __fadd2_rn(v.p[0], x.p[0]);
-          u[k] = pack<T, kU>(v);
-        }
+        for (int n = 0; n < kPairs; ++n) v.p[n] = __fadd2_rn(v.p[n], x.p[n]);
+        pack_all<T, kU, kUnits>(v, u);
       }
     } else if (has_residual) {
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) u[k] = add_units(u[k], r[k]);
     }
-    const int64_t out_row = static_cast<int64_t>(row) * a.d;
     if (a.stream != nullptr && valid) {
 #pragma unroll
       for (int k = 0; k < kUnits; ++k)
-        if (lane + k * kGroup < units) store_unit<T, kU>(a.stream + out_row + (lane + k * kGroup) * kU, u[k]);
+        if (lane + k * kGroup < units) store_unit<T, kU>(a.stream + out + k * kGroup * kU, u[k]);
     }
     if constexpr (kMode == kAdd) continue;
 
-    float2 s = both(0.f);
+    Lane<kU, kUnits> v = unpack_all<T, kU, kUnits>(u);
+    float ss[1] = {0.f};
+    if constexpr (kClear) {
+      float2 s = both(0.f);
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const Vals<kU> v = unpack(u[k]);
-#pragma unroll
-      for (int e = 0; e < kPairs; ++e) s = __ffma2_rn(v.p[e], v.p[e], s);
-    }
-    float ss[1] = {s.x + s.y};
-    group_sum<kGroup, 1>(ss, sums, parity);
-    const float2 rstd = both(rsqrtf(ss[0] * a.inv_d + a.eps));
-
-    if constexpr (kMode == kNorm) {
-      T* yp = static_cast<T*>(a.y) + out_row;
+      for (int n = 0; n < kPairs; ++n) s = __ffma2_rn(v.p[n], v.p[n], s);
+      ss[0] = s.x + s.y;
+    } else {
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
-        Vals<kU> v = unpack(u[k]);
+        float2 s = __fmul2_rn(v.p[4 * k], v.p[4 * k]);
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) v.p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
-        if (valid && lane + k * kGroup < units) store_unit<T, kU>(yp + (lane + k * kGroup) * kU, pack<T, kU>(v));
+        for (int n = 1; n < 4; ++n) s = __ffma2_rn(v.p[4 * k + n], v.p[4 * k + n], s);
+        ss[0] += valid && lane + k * kGroup < units ? s.x + s.y : 0.f;
       }
+    }
+    group_sum<kGroup, 1>(ss, sums, parity);
+    const float2 rstd = both(rsqrtf(ss[0] * a.inv_d + a.eps));
+#pragma unroll
+    for (int n = 0; n < kPairs; ++n) v.p[n] = __fmul2_rn(__fmul2_rn(v.p[n], rstd), w.p[n]);
+
+    if constexpr (kMode == kNorm) {
+      T* yp = static_cast<T*>(a.y) + out;
+      pack_all<T, kU, kUnits>(v, u);
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k)
+        if (valid && lane + k * kGroup < units) store_unit<T, kU>(yp + k * kGroup * kU, u[k]);
     } else if constexpr (kMode == kNormE4m3) {
       const bool whole = a.scale_shift < 0;  // the only form of narrow units
       float top[kUnits];
-      Vals<kU> y[kUnits];
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
-        const Vals<kU> v = unpack(u[k]);
         top[k] = 0.f;
 #pragma unroll
-        for (int e = 0; e < kPairs; ++e) {
-          y[k].p[e] = __fmul2_rn(__fmul2_rn(v.p[e], rstd), w[k].p[e]);
-          top[k] = fmaxf(top[k], fmaxf(fabsf(y[k].p[e].x), fabsf(y[k].p[e].y)));
+        for (int e = 0; e < kU; ++e) {
+          const float2 x = v.p[(k * kU + e) / 2];
+          top[k] = fmaxf(top[k], fabsf((k * kU + e) & 1 ? x.y : x.x));
         }
+        if constexpr (!kClear) top[k] = valid && lane + k * kGroup < units ? top[k] : 0.f;
       }
       if (whole) {
         float m[1] = {top[0]};
@@ -230,13 +236,16 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
         for (int k = 0; k < kUnits; ++k) top[k] = m[0];
       } else {
         // 32, 64 or 128 channels are 4, 8 or 16 neighbouring lanes
-        for (int o = 1; o >> a.scale_shift == 0; o <<= 1)
 #pragma unroll
-          for (int k = 0; k < kUnits; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], o));
+        for (int o = 0; o < 4; ++o)
+          if (o < a.scale_shift) {
+#pragma unroll
+            for (int k = 0; k < kUnits; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1 << o));
+          }
       }
       if (!valid) continue;
-      uint8_t* yp = static_cast<uint8_t*>(a.y) + out_row;
-      float* sp = a.scales + static_cast<int64_t>(row) * a.scales_per_row;
+      uint8_t* yp = static_cast<uint8_t*>(a.y) + out;
+      float* sp = a.scales + scale_row;
 #pragma unroll
       for (int k = 0; k < kUnits; ++k) {
         const int n = lane + k * kGroup;
@@ -247,14 +256,12 @@ __global__ void __launch_bounds__(threads_of(kGroup), 1024 / threads_of(kGroup))
         if constexpr (kU == 8) {
           uint32_t q[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) q[e] = e4m3x2(__fmul2_rn(y[k].p[e], inv));
-          __stcs(reinterpret_cast<uint2*>(yp + n * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
+          for (int e = 0; e < 4; ++e) q[e] = e4m3x2(__fmul2_rn(v.p[4 * k + e], inv));
+          __stcs(reinterpret_cast<uint2*>(yp + k * kGroup * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
+        } else if constexpr (kU == 2) {
+          *reinterpret_cast<uint16_t*>(yp + k * kGroup * 2) = static_cast<uint16_t>(e4m3x2(__fmul2_rn(v.p[k], inv)));
         } else {
-          const uint32_t q = e4m3x2(__fmul2_rn(y[k].p[0], inv));
-          if constexpr (kU == 2)
-            *reinterpret_cast<uint16_t*>(yp + n * 2) = static_cast<uint16_t>(q);
-          else
-            yp[n] = static_cast<uint8_t>(q);
+          yp[k * kGroup] = static_cast<uint8_t>(e4m3x2(both((k & 1 ? v.p[k / 2].y : v.p[k / 2].x) * inv.x)));
         }
       }
     }
@@ -296,14 +303,7 @@ __global__ void __launch_bounds__(kThreads) add_octs_kernel(const __grid_constan
       const int64_t n = n0 + f * span;
       if (n >= total) break;
       if (dropping) {
-        Vals<8> v = unpack(u[f]);
-        drop_oct(draw_oct(drop, b[f], i[f], j[f], oct[f]), line, drop.gain, v);
-        if (has_residual) {
-          const Vals<8> x = unpack(r[f]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
-        }
-        u[f] = pack<T, 8>(v);
+        u[f] = drop_and_add<T>(drop, line, b[f], i[f], j[f], oct[f], u[f], r[f], has_residual);
       } else if (has_residual) {
         u[f] = add_units(u[f], r[f]);
       }
@@ -326,8 +326,8 @@ cudaError_t launch_rows(const NormArgs<T>& a, int sms, cudaStream_t stream) {
   constexpr uint32_t kWide = threads_of(kGroup), kRows = kWide / kGroup;
   auto kernel = add_norm_kernel<T, kU, kGroup, kUnits, kMode>;
   const bool has_residual = a.residual.p != nullptr;
-  constexpr int kStage = kUnits * kU * static_cast<int>(sizeof(T) * kWide);
-  constexpr int kStages = kCanStage<T, kU> ? ring_of(kStage / static_cast<int>(kWide)) * kStage : 0;
+  constexpr int kStage = Rows<T, kU, kGroup, kUnits>::kStage;
+  constexpr int kStages = ring_of(kStage / static_cast<int>(kWide)) * kStage;
   const int smem = kStages * (has_residual ? 2 : 1);
   if (2 * kStages > 47 * 1024) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStages);
@@ -360,6 +360,8 @@ cudaError_t wide_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
 template <typename T, int kU, int kMode>
 cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
   if (a.d <= 128) return launch_rows<T, kU, 32, 4 / kU, kMode>(a, sms, s);
+  if constexpr (kU == 1)
+    if (a.d <= 192) return launch_rows<T, kU, 32, 6, kMode>(a, sms, s);
   if (a.d <= 256) return launch_rows<T, kU, 32, 8 / kU, kMode>(a, sms, s);
   if (a.d <= 512) return launch_rows<T, kU, 128, 4 / kU, kMode>(a, sms, s);
   if (a.d <= 1024) return launch_rows<T, kU, 256, 4 / kU, kMode>(a, sms, s);

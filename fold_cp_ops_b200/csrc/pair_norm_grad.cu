@@ -34,14 +34,26 @@ struct GradArgs {
   float eps, inv_d;
 };
 
+// Shared memory of a CTA: the gain's sums, and the stages of three rows where both fit an SM (all but rows of 4097 to 8192 channels
+// in one-channel units of fp32, which are loaded directly).
+template <typename T, int kU, int kGroup, int kUnits>
+struct Shared {
+  using In = Rows<T, kU, kGroup, kUnits>;
+  static constexpr int kSums = kUnits * kU * In::kWide * static_cast<int>(sizeof(double));
+  static constexpr bool kStaged = In::kStaged && kSums + 2 * 3 * In::kStage <= 224 * 1024;
+  static constexpr int kStages = kStaged ? 2 * 3 * In::kStage : 0;
+};
+
 // As add_norm_kernel: kU channels per access, kGroup lanes per row, kUnits units per lane.
 template <typename T, int kU, int kGroup, int kUnits>
-__global__ void __launch_bounds__(threads_of(kGroup)) norm_grad_kernel(const __grid_constant__ GradArgs<T> a) {
+__global__ void __launch_bounds__(threads_of(kGroup), (kU * kUnits > 8 ? 512 : 1024) / threads_of(kGroup)) norm_grad_kernel(const __grid_constant__ GradArgs<T> a) {
   __shared__ float sums[2 * 32 * 2];
-  extern __shared__ double fold[];  // [unit of the lane][channel of the unit][thread]
+  extern __shared__ double fold[];  // [unit of the lane][channel of the unit][thread], then the stages of the rows
   constexpr int kWide = threads_of(kGroup);
   constexpr int kRows = kWide / kGroup;
-  constexpr int kPairs = (kU + 1) / 2;
+  using In = Rows<T, kU, kGroup, kUnits>;
+  constexpr bool kStaged = Shared<T, kU, kGroup, kUnits>::kStaged;
+  constexpr int kPairs = kU * kUnits / 2;
   const int lane = threadIdx.x % kGroup;
   const int units = a.d / kU;
   const bool dropping = a.drop.keep < 65536u && a.d_update != nullptr;
@@ -49,97 +61,112 @@ __global__ void __launch_bounds__(threads_of(kGroup)) norm_grad_kernel(const __g
   Dropout drop = a.drop;
   if (dropping) resolve_seed(drop);
 
-  Vals<kU> w[kUnits], dw[kUnits];
+  const Lane<kU, kUnits> w = load_gain<kU, kGroup, kUnits>(a.weight, a.weight_dtype, lane, units);
+  Lane<kU, kUnits> dw;
 #pragma unroll
-  for (int k = 0; k < kUnits; ++k) {
-    float f[kPairs * 2];
+  for (int n = 0; n < kPairs; ++n) dw.p[n] = both(0.f);
+  if (a.partial != nullptr)
 #pragma unroll
-    for (int e = 0; e < kPairs * 2; ++e) {
-      const int n = lane + k * kGroup;
-      f[e] = n < units && e < kU ? load_any(a.weight, n * kU + e, a.weight_dtype) : 0.f;
-      if (e < kU && a.partial != nullptr) fold[(k * kU + e) * kWide + threadIdx.x] = 0.0;
-    }
-#pragma unroll
-    for (int e = 0; e < kPairs; ++e) {
-      w[k].p[e] = make_float2(f[2 * e], f[2 * e + 1]);
-      dw[k].p[e] = both(0.f);
-    }
-  }
+    for (int c = 0; c < 2 * kPairs; ++c) fold[c * kWide + threadIdx.x] = 0.0;
   auto carry = [&] {
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k)
-#pragma unroll
-      for (int e = 0; e < kU; ++e) {
-        fold[(k * kU + e) * kWide + threadIdx.x] += e & 1 ? dw[k].p[e / 2].y : dw[k].p[e / 2].x;
-        (e & 1 ? dw[k].p[e / 2].y : dw[k].p[e / 2].x) = 0.f;
-      }
+    for (int n = 0; n < kPairs; ++n) {
+      fold[2 * n * kWide + threadIdx.x] += dw.p[n].x;
+      fold[(2 * n + 1) * kWide + threadIdx.x] += dw.p[n].y;
+      dw.p[n] = both(0.f);
+    }
   };
 
+  const uint32_t span = gridDim.x * kRows;
+  auto rows_of = [&](uint32_t row, const T*& zp, const T*& yp, const T*& gp) {
+    if (a.flat) {
+      zp = a.z.flat(row), yp = a.dy.flat(row), gp = a.dz.flat(row);
+    } else {
+      uint32_t b, i, j;
+      a.walk.at(row, b, i, j);
+      zp = a.z.row(b, i, j), yp = a.dy.row(b, i, j), gp = a.dz.row(b, i, j);
+    }
+  };
+  char* const stages = reinterpret_cast<char*>(fold + (a.partial != nullptr ? kUnits * kU * kWide : 0));
+  auto fetch = [&](uint32_t row, char* to) {
+    if (row < a.rows) {
+      const T *zp, *yp, *gp;
+      rows_of(row, zp, yp, gp);
+      In::fetch(to, zp, a.d);
+      if (a.dy.p != nullptr) In::fetch(to + In::kStage, yp, a.d);
+      if (a.dz.p != nullptr) In::fetch(to + 2 * In::kStage, gp, a.d);
+    }
+    stage_commit();
+  };
+  const uint32_t mine = threadIdx.x / kGroup;
+  if constexpr (kStaged) fetch(blockIdx.x * kRows + mine, stages);
+
   int parity = 0, held = 0;
-  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += gridDim.x * kRows, parity ^= 1) {
-    const uint32_t row = first + threadIdx.x / kGroup;
+  for (uint32_t first = blockIdx.x * kRows; first < a.rows; first += span, parity ^= 1) {
+    const uint32_t row = first + mine;
     const bool valid = row < a.rows;
     uint32_t b = 0, i = 0, j = 0;
-    if (valid && (dropping || !a.flat)) a.walk.at(row, b, i, j);
-    const T* zp = a.flat ? a.z.flat(row) : a.z.row(b, i, j);
-    const T* yp = a.flat ? a.dy.flat(row) : a.dy.row(b, i, j);
-    const T* gp = a.flat ? a.dz.flat(row) : a.dz.row(b, i, j);
+    if (valid && dropping) a.walk.at(row, b, i, j);
 
     Unit<T, kU> z[kUnits], dy[kUnits], dz[kUnits];
+    if constexpr (kStaged) {
+      // two stages: one at hand, one on its way (a third is no faster)
+      fetch(row + span, stages + (parity ^ 1) * 3 * In::kStage);
+      stage_wait<1>();
+      const char* from = stages + parity * 3 * In::kStage;
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const int n = lane + k * kGroup;
-      const bool on = valid && n < units;
-      z[k] = on ? load_unit<T, kU>(zp + n * kU) : zero_unit<T, kU>();
-      dy[k] = on && a.dy.p != nullptr ? load_unit<T, kU>(yp + n * kU) : zero_unit<T, kU>();
-      dz[k] = on && a.dz.p != nullptr ? load_unit<T, kU>(gp + n * kU) : zero_unit<T, kU>();
+      for (int k = 0; k < kUnits; ++k) {
+        const bool on = valid && lane + k * kGroup < units;
+        z[k] = on ? In::read(from, k) : zero_unit<T, kU>();
+        dy[k] = on && a.dy.p != nullptr ? In::read(from + In::kStage, k) : zero_unit<T, kU>();
+        dz[k] = on && a.dz.p != nullptr ? In::read(from + 2 * In::kStage, k) : zero_unit<T, kU>();
+      }
+    } else {
+      const T *zp = nullptr, *yp = nullptr, *gp = nullptr;
+      if (valid) rows_of(row, zp, yp, gp);
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        const int n = lane + k * kGroup;
+        const bool on = valid && n < units;
+        z[k] = on ? load_unit<T, kU>(zp + n * kU) : zero_unit<T, kU>();
+        dy[k] = on && a.dy.p != nullptr ? load_unit<T, kU>(yp + n * kU) : zero_unit<T, kU>();
+        dz[k] = on && a.dz.p != nullptr ? load_unit<T, kU>(gp + n * kU) : zero_unit<T, kU>();
+      }
     }
+    const int64_t at = static_cast<int64_t>(row) * a.d + lane * kU;  // the lane's first channel
 
+    const Lane<kU, kUnits> vz = unpack_all<T, kU, kUnits>(z), vy = unpack_all<T, kU, kUnits>(dy);
     float2 zz = both(0.f), tz = both(0.f);
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const Vals<kU> vz = unpack(z[k]), vy = unpack(dy[k]);
-#pragma unroll
-      for (int e = 0; e < kPairs; ++e) {
-        zz = __ffma2_rn(vz.p[e], vz.p[e], zz);
-        tz = __ffma2_rn(__fmul2_rn(vy.p[e], w[k].p[e]), vz.p[e], tz);
-      }
+    for (int n = 0; n < kPairs; ++n) {
+      zz = __ffma2_rn(vz.p[n], vz.p[n], zz);
+      tz = __ffma2_rn(__fmul2_rn(vy.p[n], w.p[n]), vz.p[n], tz);
     }
     float s[2] = {zz.x + zz.y, tz.x + tz.y};
     group_sum<kGroup, 2>(s, sums, parity);
     const float rstd = rsqrtf(s[0] * a.inv_d + a.eps);
     // in this order a row of zeros gives 0 even where rstd^3 would overflow
-    const float back = -rstd * (rstd * (rstd * (s[1] * a.inv_d)));
-    const int64_t out_row = static_cast<int64_t>(row) * a.d;
-    NarrowMask<kU < 8 ? kU : 1, kUnits> mask;
-    if constexpr (kU < 8)
-      if (dropping) mask = draw_narrow<kU, kUnits, kGroup>(drop, line, b, i, j, lane & ~31, a.octs);
-
+    const float2 back = both(-rstd * (rstd * (rstd * (s[1] * a.inv_d))));
+    Lane<kU, kUnits> g = unpack_all<T, kU, kUnits>(dz);
 #pragma unroll
-    for (int k = 0; k < kUnits; ++k) {
-      const int n = lane + k * kGroup;
-      const bool on = valid && n < units;
-      const Vals<kU> vz = unpack(z[k]), vy = unpack(dy[k]);
-      Vals<kU> g = unpack(dz[k]);
+    for (int n = 0; n < kPairs; ++n) {
+      const float2 y = __fmul2_rn(vy.p[n], both(rstd));
+      g.p[n] = __ffma2_rn(vz.p[n], back, __ffma2_rn(w.p[n], y, g.p[n]));
+      dw.p[n] = __ffma2_rn(vz.p[n], y, dw.p[n]);
+    }
+    Unit<T, kU> out[kUnits];
+    if (a.d_stream != nullptr) {
+      pack_all<T, kU, kUnits>(g, out);
 #pragma unroll
-      for (int e = 0; e < kPairs; ++e) {
-        const float2 y = __fmul2_rn(vy.p[e], both(rstd));
-        g.p[e] = __ffma2_rn(vz.p[e], both(back), __ffma2_rn(w[k].p[e], y, g.p[e]));
-        dw[k].p[e] = __ffma2_rn(vz.p[e], y, dw[k].p[e]);
-      }
-      if (on && a.d_stream != nullptr) store_unit<T, kU>(a.d_stream + out_row + n * kU, pack<T, kU>(g));
-      if (a.d_update != nullptr) {
-        if (dropping) {
-          if constexpr (kU == 8) {
-            drop_oct(draw_oct(drop, b, i, j, n), line, drop.gain, g);
-          } else {
-            const uint32_t bits = narrow_bits<kU, kUnits>(mask, k);
-            g.p[0].x = bits & 1u ? g.p[0].x * drop.gain : 0.f;
-            if constexpr (kU > 1) g.p[0].y = bits & 2u ? g.p[0].y * drop.gain : 0.f;
-          }
-        }
-        if (on) store_unit<T, kU>(a.d_update + out_row + n * kU, pack<T, kU>(g));
-      }
+      for (int k = 0; k < kUnits; ++k)
+        if (valid && lane + k * kGroup < units) store_unit<T, kU>(a.d_stream + at + k * kGroup * kU, out[k]);
+    }
+    if (a.d_update != nullptr) {
+      if (dropping) drop_all<kU, kGroup, kUnits>(drop, line, b, i, j, lane, a.octs, g);
+      pack_all<T, kU, kUnits>(g, out);
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k)
+        if (valid && lane + k * kGroup < units) store_unit<T, kU>(a.d_update + at + k * kGroup * kU, out[k]);
     }
     if (a.partial != nullptr && ++held == kFold) {
       held = 0;
@@ -150,7 +177,7 @@ __global__ void __launch_bounds__(threads_of(kGroup)) norm_grad_kernel(const __g
   if (a.partial == nullptr) return;
   carry();
   __syncthreads();
-  // channel c is part of unit c / kU: lane (c / kU) % kGroup, unit (c / kU) / kGroup of every row the CTA holds
+  // channel c is part of unit c / kU: lane (c / kU) % kGroup, value (c / kU) / kGroup * kU + c % kU of every row the CTA holds
   for (int c = threadIdx.x; c < a.d; c += kWide) {
     const int n = c / kU;
     const double* f = fold + (n / kGroup * kU + c % kU) * kWide + n % kGroup;
@@ -197,6 +224,7 @@ inline Shape shape_of(int unit, int d) {
     return {d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024, 8};
   }
   if (d <= 128) return {32, 4};
+  if (unit == 1 && d <= 192) return {32, 6};
   if (d <= 256) return {32, 8};
   return {d <= 512 ? 128 : d <= 1024 ? 256 : d <= 2048 ? 512 : 1024, d <= 4096 ? 4 : 8};
 }
@@ -213,13 +241,13 @@ inline uint32_t grid_of(uint32_t rows, Shape w, int sms) {
 template <typename T, int kU, int kGroup, int kUnits>
 cudaError_t launch_rows(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream) {
   constexpr int kWide = threads_of(kGroup);
-  const int smem = a.partial != nullptr ? kUnits * kU * kWide * static_cast<int>(sizeof(double)) : 0;
-  if (smem > 48 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(norm_grad_kernel<T, kU, kGroup, kUnits>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  constexpr int kSums = Shared<T, kU, kGroup, kUnits>::kSums, kStages = Shared<T, kU, kGroup, kUnits>::kStages;
+  auto kernel = norm_grad_kernel<T, kU, kGroup, kUnits>;
+  if (kSums + kStages > 47 * 1024) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSums + kStages);
     if (e != cudaSuccess) return e;
   }
-  norm_grad_kernel<T, kU, kGroup, kUnits><<<grid, kWide, smem, stream>>>(a);
+  kernel<<<grid, kWide, kStages + (a.partial != nullptr ? kSums : 0), stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -236,6 +264,8 @@ cudaError_t by_shape(const GradArgs<T>& a, Shape w, uint32_t grid, cudaStream_t 
     return launch_rows<T, 8, 1024, 1>(a, grid, s);
   } else {
     if (w.group == 32 && w.channels == 4) return launch_rows<T, kU, 32, 4 / kU>(a, grid, s);
+    if constexpr (kU == 1)
+      if (w.group == 32 && w.channels == 6) return launch_rows<T, kU, 32, 6>(a, grid, s);
     if (w.group == 32) return launch_rows<T, kU, 32, 8 / kU>(a, grid, s);
     if (w.group == 128) return launch_rows<T, kU, 128, 4 / kU>(a, grid, s);
     if (w.group == 256) return launch_rows<T, kU, 256, 4 / kU>(a, grid, s);
@@ -296,7 +326,7 @@ extern "C" int pair_sm100_add_norm_grad_workspace(const pair_norm_desc_t* desc, 
   const uint32_t rows = static_cast<uint32_t>(desc->b) * desc->i * desc->j;
   // the unit depends on addresses that are not known here: room for the largest grid
   uint32_t most = 0;
-  for (int unit : {8, 2}) {
+  for (int unit : {8, 2, 1}) {
     const uint32_t grid = grid_of(rows, shape_of(unit, desc->d), sms);
     most = grid > most ? grid : most;
   }

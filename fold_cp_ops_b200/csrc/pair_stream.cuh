@@ -83,20 +83,16 @@ __device__ __forceinline__ void store_unit(T* p, const Unit<T, kU>& o) {
 }
 
 // Asynchronous copies of a lane's own units into its own slots of shared memory, read back by the same lane: bytes in flight that
-// cost no registers, and no barrier (cp.async groups complete per thread).  Not for 2-byte units, which cp.async does not know, nor for
-// octs of fp32, whose two 16-byte halves would each touch every sector of the row: direct loads find the second half in L1.
-template <typename T, int kU>
-constexpr bool kCanStage = sizeof(T) * kU == 4 || sizeof(T) * kU == 16;
-
+// cost no registers, and no barrier (cp.async groups complete per thread).
 template <typename T, int kU>
 __device__ __forceinline__ void stage_unit(void* slot, const T* p) {
   constexpr int kBytes = sizeof(T) * kU;
+  static_assert(kBytes == 4 || kBytes == 16, "cp.async moves 4 or 16 bytes here");
   const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot));
-  if constexpr (kBytes == 16) {
+  if constexpr (kBytes == 16)
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(p) : "memory");
-  } else {
+  else
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(p) : "memory");
-  }
 }
 template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> staged_unit(const void* slot) {
@@ -105,6 +101,31 @@ __device__ __forceinline__ Unit<T, kU> staged_unit(const void* slot) {
 __device__ __forceinline__ void stage_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int kPending>
 __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory"); }
+
+// Which rows travel that way: not octs of fp32, whose two 16-byte halves would each touch every sector of the row, where direct loads
+// find the second half in L1 (131072 rows of 256 channels: 95 against 126 us), nor 2-byte units, which cp.async does not know
+// (copying the 4-byte words under them takes more instructions than the loads do: 80000 rows of 131 channels 26 against 17 us).
+template <typename T, int kU, int kGroup, int kUnits>
+struct Rows {
+  static constexpr int kWide = kGroup <= 32 ? 256 : kGroup;  // threads of the CTA
+  static constexpr int kBytes = sizeof(T) * kU;
+  static constexpr bool kStaged = kBytes == 4 || kBytes == 16;
+  static constexpr int kStage = kStaged ? kUnits * kWide * kBytes : 0;  // shared memory of one row of every group
+
+  // Begins to copy this lane's units of a row into a stage.
+  static __device__ __forceinline__ void fetch(char* stage, const T* row, int d) {
+    if constexpr (kStaged) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) {
+        const int c = (threadIdx.x % kGroup + k * kGroup) * kU;
+        if (c < d) stage_unit<T, kU>(stage + k * kWide * kBytes + threadIdx.x * kBytes, row + c);
+      }
+    }
+  }
+  static __device__ __forceinline__ Unit<T, kU> read(const char* stage, int k) {
+    return staged_unit<T, kU>(stage + k * kWide * kBytes + threadIdx.x * kBytes);
+  }
+};
 
 template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> zero_unit() {
@@ -149,6 +170,41 @@ __device__ __forceinline__ Unit<T, kU> pack(const Vals<kU>& v) {
   return o;
 }
 
+// The fp32 values of all units of a lane in pairs: channels of a unit, or, of one-channel units, two steps' units.
+template <int kU, int kUnits>
+struct Lane {
+  static constexpr int kPairs = kU * kUnits / 2;
+  static_assert(kU * kUnits % 2 == 0, "one-channel units come in even numbers");
+  float2 p[kPairs];
+};
+
+template <typename T, int kU, int kUnits>
+__device__ __forceinline__ Lane<kU, kUnits> unpack_all(const Unit<T, kU> (&u)[kUnits]) {
+  Lane<kU, kUnits> v;
+#pragma unroll
+  for (int n = 0; n < v.kPairs; ++n) {
+    v.p[n].x = to_f32(u[2 * n / kU].e[2 * n % kU]);
+    v.p[n].y = to_f32(u[(2 * n + 1) / kU].e[(2 * n + 1) % kU]);
+  }
+  return v;
+}
+
+template <typename T, int kU, int kUnits>
+__device__ __forceinline__ void pack_all(const Lane<kU, kUnits>& v, Unit<T, kU> (&u)[kUnits]) {
+#pragma unroll
+  for (int n = 0; n < v.kPairs; ++n) {
+    if constexpr (sizeof(T) == 2 && kU > 1) {
+      if constexpr (__is_same(T, __half))
+        reinterpret_cast<__half2*>(&u[2 * n / kU])[n % (kU / 2)] = __float22half2_rn(v.p[n]);
+      else
+        reinterpret_cast<__nv_bfloat162*>(&u[2 * n / kU])[n % (kU / 2)] = __float22bfloat162_rn(v.p[n]);
+    } else {
+      u[2 * n / kU].e[2 * n % kU] = from_f32<T>(v.p[n].x);
+      u[(2 * n + 1) / kU].e[(2 * n + 1) % kU] = from_f32<T>(v.p[n].y);
+    }
+  }
+}
+
 // a + b in the unit's type, rounded once: for 16-bit pairs the packed addition, which rounds the exact sum.
 template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> add_units(const Unit<T, kU>& a, const Unit<T, kU>& b) {
@@ -187,6 +243,19 @@ __device__ __forceinline__ void store_any(void* p, int64_t at, int dtype, float 
 }
 
 inline int type_bytes(int dtype) { return dtype == PAIR_FP32 ? 4 : 2; }
+
+// The gain's values of a lane's channels; 0 behind the row's end.
+template <int kU, int kGroup, int kUnits>
+__device__ __forceinline__ Lane<kU, kUnits> load_gain(const void* weight, int dtype, int lane, int units) {
+  Lane<kU, kUnits> w;
+#pragma unroll
+  for (int c = 0; c < kU * kUnits; ++c) {
+    const int n = lane + c / kU * kGroup;
+    const float f = n < units ? load_any(weight, n * kU + c % kU, dtype) : 0.f;
+    (c & 1 ? w.p[c / 2].y : w.p[c / 2].x) = f;
+  }
+  return w;
+}
 
 // ---------------------------------------------------------------------------------------------
 // rows of a strided tensor
@@ -301,16 +370,16 @@ __device__ __forceinline__ uint4 draw_oct(const Dropout& d, uint32_t b, uint32_t
   return philox(((b + d.b0) << 16) | oct, cj, ci, d.offset, d.key0, d.key1);
 }
 
-// Dropout of the eight channels of an oct.  `line` is keep << 16: the high half of a word is below keep exactly when the
-// word is below that, the low half when the word shifted up is (keep is at most 65535 here).  A dropped element becomes
+// Dropout of the eight channels of an oct, four pairs.  `line` is keep << 16: the high half of a word is below keep exactly when
+// the word is below that, the low half when the word shifted up is (keep is at most 65535 here).  A dropped element becomes
 // 0 whatever it was (an infinity or NaN included): it is selected, and what is kept is multiplied.
-__device__ __forceinline__ void drop_oct(const uint4 r, uint32_t line, float gain, Vals<8>& v) {
+__device__ __forceinline__ void drop_oct(const uint4 r, uint32_t line, float gain, float2* p) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
-    v.p[k].x = (w[k] << 16) < line ? v.p[k].x : 0.f;
-    v.p[k].y = w[k] < line ? v.p[k].y : 0.f;
-    v.p[k] = __fmul2_rn(v.p[k], both(gain));
+    p[k].x = (w[k] << 16) < line ? p[k].x : 0.f;
+    p[k].y = w[k] < line ? p[k].y : 0.f;
+    p[k] = __fmul2_rn(p[k], both(gain));
   }
 }
 
@@ -358,6 +427,25 @@ __device__ __forceinline__ uint32_t narrow_bits(const NarrowMask<kU, kUnits>& m,
   const int slot = m.kPer * k / 32;
   const uint32_t byte = (__shfl_sync(0xffffffffu, m.bits[slot / 4], q & 31) >> (8 * (slot & 3))) & 0xffu;
   return byte >> (lane * kU % 8);
+}
+
+// Dropout of all units of a lane.  `lane` is the lane of its group; every lane of the warp takes part.
+template <int kU, int kGroup, int kUnits>
+__device__ __forceinline__ void drop_all(const Dropout& d, uint32_t line, uint32_t b, uint32_t i, uint32_t j, int lane, int octs,
+                                         Lane<kU, kUnits>& v) {
+  if constexpr (kU == 8) {
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) drop_oct(draw_oct(d, b, i, j, lane + k * kGroup), line, d.gain, v.p + 4 * k);
+  } else {
+    const auto mask = draw_narrow<kU, kUnits, kGroup>(d, line, b, i, j, lane & ~31, octs);
+#pragma unroll
+    for (int n = 0; n < v.kPairs; ++n) {
+      const uint32_t x = narrow_bits<kU, kUnits>(mask, 2 * n / kU);
+      const uint32_t y = kU == 2 ? x >> 1 : narrow_bits<kU, kUnits>(mask, 2 * n + 1);
+      v.p[n].x = x & 1u ? v.p[n].x * d.gain : 0.f;
+      v.p[n].y = y & 1u ? v.p[n].y * d.gain : 0.f;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
