@@ -227,6 +227,7 @@ __device__ __forceinline__ Entry entry_of(const SortArgs& a, uint32_t p) {
 }
 
 __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortArgs a) {
+  next_may_start();
   behind_previous();
   extern __shared__ uint32_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -259,6 +260,7 @@ __global__ void __launch_bounds__(kSortWarps * 32) sort_count_kernel(const SortA
 
 // Exclusive scan of one bin's counts over the tiles, a run of neighbours per thread; the bin's total beside it.
 __global__ void __launch_bounds__(kThreads) sort_scan_kernel(uint32_t* counts, uint32_t* totals, uint32_t tiles) {
+  next_may_start();
   behind_previous();
   __shared__ uint32_t part[kThreads / 32];
   uint32_t* c = counts + static_cast<int64_t>(blockIdx.x) * tiles;
@@ -292,6 +294,7 @@ __global__ void __launch_bounds__(kThreads) sort_scan_kernel(uint32_t* counts, u
 }
 
 __global__ void __launch_bounds__(kSortWarps * 32) sort_place_kernel(const SortArgs a) {
+  next_may_start();
   behind_previous();
   extern __shared__ uint32_t smem[];
   __shared__ uint32_t part[kSortWarps];
@@ -385,6 +388,7 @@ constexpr bool kSumStaged = kWide && sizeof(T) == 2;
 
 template <typename T, int kGroup, bool kWide>
 __global__ void __launch_bounds__(kThreads, kSumCtas) sum_runs_kernel(const SumArgs<T> a) {
+  next_may_start();
   behind_previous();
   constexpr int kGroups = kThreads / kGroup;
   constexpr int kChannels = kGroup * 8;

@@ -5,9 +5,11 @@
 // the launch is native: a forward call takes about 6 us and the gradient of one runs in the autograd engine's own thread
 // without the interpreter.  (The same in Python: 14 us, and 90 to 130 us for a training step.)  The library's functions come as
 // addresses from the loader, which has checked them against the sources; nothing here links to it.
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -188,6 +190,23 @@ void check_overlap(const Tensor& out, const Tensor& t, const char* name) {
   const auto a = span(out), b = span(t);
   if (a.first < b.second && b.first < a.second && !(a.first == b.first && t.is_contiguous()))
     refuse("out overlaps ", name, " without being it");
+}
+
+// A captured backward pass may only touch the capturing stream, but the engine also waits for the streams that the leaves'
+// accumulators belong to.  An accumulator lives as long as any graph that uses the leaf: one that an eager graph on another
+// stream still holds would break the capture from inside the engine, so the call is refused while nothing is lost.
+void check_capture(std::initializer_list<const Tensor*> tensors) {
+  if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+  for (const Tensor* t : tensors) {
+    if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+    const auto accumulator = torch::autograd::impl::try_get_grad_accumulator(*t);
+    if (accumulator == nullptr) continue;
+    const auto stream = accumulator->stream();
+    if (stream.has_value() && *stream != c10::cuda::getCurrentCUDAStream(t->get_device()).unwrap())
+      throw std::runtime_error(
+          "cannot capture a gradient: an eager graph of the same leaf, made on another stream, is still alive. Drop its outputs "
+          "(and run warm-up passes on the capturing stream) before the capture");
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -379,6 +398,7 @@ Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_,
     check_overlap(out, update, "update");
     check_overlap(out, residual, "residual");
   } else if (wants_grad({&update, &residual})) {
+    check_capture({&update, &residual});
     return DropoutAdd::apply(update, residual_, seed, drop);
   }
   return run_add(update, residual, dropping(drop, or_none(seed)), out);
@@ -390,6 +410,7 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optiona
   check_pair(update, residual);
   check_weight(weight, update, eps);
   if (wants_grad({&update, &residual, &weight})) {
+    check_capture({&update, &residual, &weight});
     variable_list out = AddRmsNorm::apply(update, residual_, weight, seed, eps, drop);
     return {out[0], out[1]};
   }
@@ -447,7 +468,10 @@ Tensor pair_embedding(const Tensor& index, const Tensor& table, double scale, co
   const at::ScalarType dtype = base.defined() ? base.scalar_type() : dtype_.value_or(table.scalar_type());
   if (kind_of(dtype) < 0) refuse("the embedding's type must be bfloat16, float16 or float32; got ", dtype);
   if (!std::isfinite(scale)) refuse("scale must be finite; got ", scale);
-  if (wants_grad({&table, &base})) return PairEmbedding::apply(index, table, base_, scale, static_cast<int64_t>(dtype));
+  if (wants_grad({&table, &base})) {
+    check_capture({&table, &base});
+    return PairEmbedding::apply(index, table, base_, scale, static_cast<int64_t>(dtype));
+  }
   return run_embed(index, table, base, scale, dtype);
 }
 

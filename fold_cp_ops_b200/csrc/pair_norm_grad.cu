@@ -53,6 +53,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kU * kUnits > 8 ? 512 : 1
   constexpr int kRows = kWide / kGroup;
   using In = Rows<T, kU, kGroup, kUnits>;
   constexpr bool kStaged = Shared<T, kU, kGroup, kUnits>::kStaged;
+  if (a.partial != nullptr) next_may_start();  // the kernel that joins the sums
   constexpr int kPairs = kU * kUnits / 2;
   const int lane = threadIdx.x % kGroup;
   const int units = a.d / kU;

@@ -494,12 +494,11 @@ __device__ __forceinline__ void group_max(float (&v)[kN], float* buf, int parity
   group_merge<kGroup, kN, true>(v, buf, parity);
 }
 
-// Launches.  The kernels of one call follow one another: each says at its start that the next may be set up while it runs, and waits
-// there for the one before it to end (its results included), which hides the launch of all but the first.
-__device__ __forceinline__ void behind_previous() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
+// Launches.  The kernels of one call follow one another: each but the last says at its start that the next may be set up while it
+// runs (next_may_start), and the next waits at its start for it to end, its results included (behind_previous).  That hides the
+// launch of all but the first.  The last says nothing: what follows the call sees an ordinary kernel.
+__device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void behind_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <bool kBehind, typename K, typename... A>
 cudaError_t launch_kernel(K kernel, dim3 grid, unsigned threads, size_t smem, cudaStream_t stream, A... args) {

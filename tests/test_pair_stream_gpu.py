@@ -514,6 +514,43 @@ def test_the_operators_together_and_captured():
             assert torch.equal(gz, wz) and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+def test_a_capture_beside_a_living_eager_graph_is_refused():
+    """The engine would wait for the eager graph's stream in the middle of the capture; the call is refused before anything
+    of it is captured, and the same capture works once the graph is gone."""
+    p = P()
+    x, w = rand(1, 4, 4, 64, seed=1).requires_grad_(), torch.ones(64, device=DEV, requires_grad=True)
+    table, index = rand(9, 64, seed=2).requires_grad_(), torch.arange(16, device=DEV).reshape(1, 4, 4) % 9
+    calls = {"norm": lambda: p.add_rms_norm(x, None, w)[0], "add": lambda: p.dropout_add(x, x, p.PairDropout(0.5)),
+             "embed": lambda: p.pair_embedding(index, table)}
+    for name, call in calls.items():
+        want = torch.autograd.grad(call().sum(), table if name == "embed" else x)[0]
+        alive = call()
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph of the same leaf"):
+            with torch.cuda.graph(graph):
+                call()
+        del alive
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            (got,) = torch.autograd.grad(call().sum(), table if name == "embed" else x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), name
+
+
+def test_second_derivatives_are_refused_where_they_are_used():
+    p = P()
+    x, w = rand(1, 2, 3, 64, seed=1).requires_grad_(), torch.ones(64, device=DEV, requires_grad=True)
+    table = rand(5, 64, seed=2).requires_grad_()
+    for out, leaf in ((p.add_rms_norm(x, None, w)[0], x), (p.dropout_add(x, None, p.PairDropout(0.5)), x),
+                      (p.pair_embedding(torch.arange(5, device=DEV), table), table)):
+        (plain,) = torch.autograd.grad(out.sum(), leaf, retain_graph=True)
+        (g,) = torch.autograd.grad(out.sum(), leaf, create_graph=True)
+        assert torch.equal(g, plain)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            g.square().sum().backward()
+
+
 def test_two_streams_at_once():
     p = P()
     shape = (1, 64, 64, 128)
