@@ -41,6 +41,7 @@ _NO_DTENSOR_GRADIENT = "gradients through DTensors are not supported: pass the l
 
 #: a ``pair_dropout_t`` of include/pair_stream_sm100.h: seed, offset, keep, (device seed), shared, origin b, i, j
 _pack_dropout = struct.Struct("@QIIP4i").pack
+_NO_DROPOUT = (b"", None)
 
 
 @dataclass(frozen=True)
@@ -86,12 +87,12 @@ def _record(dropout: Optional[PairDropout], wrap: Optional["_Wrap"]) -> Tuple[by
     """The library's record of a dropout (empty where everything is kept), at the position of this rank's block, and the
     device seed."""
     if dropout is None:
-        return b"", None
+        return _NO_DROPOUT
     if not isinstance(dropout, PairDropout):
         raise TypeError(f"dropout must be a PairDropout or None; got {type(dropout).__name__}")
     keep = dropout.keep
     if keep == 65536:
-        return b"", None
+        return _NO_DROPOUT
     origin = dropout.origin
     if wrap is not None:
         origin = tuple(o + at for o, at in zip(origin, pair_block_origin(wrap.like)))
@@ -115,8 +116,6 @@ def pair_block_origin(x) -> Tuple[int, int, int]:
 # ---------------------------------------------------------------------------------------------
 def _locals_of(names: Sequence[str], tensors: Sequence[Optional[Tensor]]):
     """The ranks' local blocks of DTensors that are sharded alike, and their :class:`_Wrap` (``None`` where all are plain)."""
-    if all(type(t) in _PLAIN for t in tensors):
-        return tensors, None
     given = [(n, t) for n, t in zip(names, tensors) if t is not None]
     if not any(_is_dtensor(t) for _, t in given):
         return tensors, None
@@ -168,8 +167,9 @@ def dropout_add(update: Tensor, residual: Optional[Tensor] = None, dropout: Opti
     most 8192.  ``residual=None`` is a plain dropout.  ``out`` (contiguous; no gradients) may be ``residual`` or ``update``
     itself: the stream is then updated in place.  Dropped elements become 0 whatever they were.  Raises ``ValueError`` for
     anything else, ``TypeError`` for a ``dropout`` that is no :class:`PairDropout`."""
-    given = out
-    (update, residual, out), wrap = _locals_of(("update", "residual", "out"), (update, residual, out))
+    given, wrap = out, None
+    if type(update) not in _PLAIN or type(residual) not in _PLAIN or type(out) not in _PLAIN:
+        (update, residual, out), wrap = _locals_of(("update", "residual", "out"), (update, residual, out))
     drop, seed = _record(dropout, wrap)
     z = _lib.pair_host().dropout_add(update, residual, drop, seed, out)
     if given is not None:
@@ -183,8 +183,10 @@ def add_rms_norm(update: Tensor, residual: Optional[Tensor], weight: Tensor, *, 
 
     Tensors as in :func:`dropout_add`; ``weight`` is ``(D,)`` in any of the three types and gets its gradient in its own.
     ``residual=None`` takes the norm of ``dropout(update)``; without a dropout too, ``z`` is ``update`` itself."""
-    (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
-    _no_gradient(wrap, weight)
+    wrap = None
+    if type(update) not in _PLAIN or type(residual) not in _PLAIN:
+        (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
+        _no_gradient(wrap, weight)
     drop, seed = _record(dropout, wrap)
     y, z = _lib.pair_host().add_rms_norm(update, residual, weight, eps, drop, seed)
     return (y, z) if wrap is None else (wrap(y), wrap(z))
@@ -198,7 +200,9 @@ def add_rms_norm_fp8(update: Tensor, residual: Optional[Tensor], weight: Tensor,
     ``(..., D / group)``: the group's largest ``|y|`` / 448, and 1 for a group of zeros.  ``y`` is scaled in fp32 and rounded
     once, to e4m3.  For inference: refuses inputs that require gradients.  Scales per group need rows that start on 16-byte
     boundaries; other inputs are copied first."""
-    (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
+    wrap = None
+    if type(update) not in _PLAIN or type(residual) not in _PLAIN:
+        (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
     drop, seed = _record(dropout, wrap)
     q, scales, z = _lib.pair_host().add_rms_norm_fp8(update, residual, weight, eps, group, drop, seed)
     return (q, scales, z) if wrap is None else (wrap(q), wrap(scales), wrap(z))
@@ -213,7 +217,9 @@ def pair_embedding(index: Tensor, table: Tensor, *, scale: float = 1.0, base: Op
     least fp32 over tokens sorted by index, in a fixed order (the same bits every time).  ``base``: what the embedding is
     added to, or ``None``; the result has its type, else ``dtype``, else the table's.  ``index`` and ``base`` may be DTensors
     sharded alike.  ``index``, ``base`` and the result's gradient are copied where they are not contiguous."""
-    (index, base), wrap = _locals_of(("index", "base"), (index, base))
-    _no_gradient(wrap, table)
+    wrap = None
+    if type(index) not in _PLAIN or type(base) not in _PLAIN:
+        (index, base), wrap = _locals_of(("index", "base"), (index, base))
+        _no_gradient(wrap, table)
     out = _lib.pair_host().pair_embedding(index, table, scale, base, dtype)
     return out if wrap is None else wrap(out)

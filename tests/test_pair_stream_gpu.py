@@ -514,6 +514,7 @@ def test_the_operators_together_and_captured():
             assert torch.equal(gz, wz) and all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_a_capture_beside_a_living_eager_graph_is_refused():
     """The engine would wait for the eager graph's stream in the middle of the capture; the call is refused before anything
     of it is captured, and the same capture works once the graph is gone."""
@@ -549,6 +550,28 @@ def test_second_derivatives_are_refused_where_they_are_used():
         assert torch.equal(g, plain)
         with pytest.raises(RuntimeError, match="differentiable once"):
             g.square().sum().backward()
+
+
+def test_dtensors_on_one_rank(tmp_path):
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Shard, distribute_tensor
+
+    p, started = P(), not dist.is_initialized()
+    if started:
+        dist.init_process_group("nccl", init_method=f"file://{tmp_path}/store", rank=0, world_size=1, device_id=torch.device(DEV))
+    try:
+        mesh = init_device_mesh("cuda", (1,))
+        x, w = rand(1, 6, 8, 64, seed=1, dtype=torch.bfloat16), torch.ones(64, device=DEV)
+        dx, drop = distribute_tensor(x, mesh, (Shard(1),)), p.PairDropout(0.25, seed=3)
+        y, z = p.add_rms_norm(dx, dx, w, dropout=drop)
+        want = p.add_rms_norm(x, x, w, dropout=drop)
+        assert isinstance(y, DTensor) and torch.equal(y.full_tensor(), want[0]) and torch.equal(z.full_tensor(), want[1])
+        s = distribute_tensor(x.clone(), mesh, (Shard(1),))
+        assert p.dropout_add(dx, s, drop, out=s) is s and torch.equal(s.full_tensor(), want[1])
+    finally:
+        if started:
+            dist.destroy_process_group()
 
 
 def test_two_streams_at_once():
