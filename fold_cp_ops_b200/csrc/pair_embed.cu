@@ -150,49 +150,64 @@ __global__ void __launch_bounds__(kThreads) embed_rows_kernel(const EmbedArgs a)
 // ---------------------------------------------------------------------------------------------
 // gradient without a sort
 // ---------------------------------------------------------------------------------------------
-// One CTA per table row (x) and slab of 256 channels (y): its eight warps look through an eighth of the indices each and
-// add the rows that match, in ascending order; the warps' sums are joined in order.
-template <typename T, bool kWide>
-__global__ void __launch_bounds__(kThreads) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table,
-                                                                  int table_dtype, uint32_t tokens, int d, float scale) {
-  constexpr int kAhead = 4;
-  __shared__ float sums[kThreads / 32][kSlab];
+// One CTA per table row (x) and slab of 256 channels (y): each warp looks through its part of the indices and adds the rows that
+// match, in ascending order; the warps' sums are joined in order.  The fewer rows there are, the more warps each takes (4096 tokens
+// into 21 rows: 7.4 us with 32, 12.7 with eight; into 2048 rows 22 and 13).
+template <typename T, bool kWide, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table,
+                                                                     int table_dtype, uint32_t tokens, int d, float scale) {
+  constexpr int kAhead = 4, kLook = kWarps > 8 ? 2 : 4;  // rows of d_out and blocks of 32 indices in flight
+  __shared__ float sums[kWarps][kSlab];
   const uint32_t row = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slab = blockIdx.y * kSlab, left = d - slab;
-  const uint32_t share = ((tokens + 8 * 32 - 1) / (8 * 32)) * 32;
-  const uint32_t lo = warp * share, hi = min(tokens, lo + share);
-  float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  for (uint32_t t0 = lo; t0 < hi; t0 += 32) {
-    const uint32_t t = t0 + lane;
-    uint32_t hit = __ballot_sync(0xffffffffu, t < hi && index.at(t) == row);
-    while (hit != 0) {
-      Unit<T, 8> o[kAhead];
+  const uint32_t share = ((tokens + kWarps * 32 - 1) / (kWarps * 32)) * 32;
+  const uint32_t lo = min(tokens, warp * share), hi = min(tokens, lo + share);
+  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  for (uint32_t block = lo; block < hi; block += 32 * kLook) {
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // of a block first: at most 128 terms, then at most 32
+    uint32_t hits[kLook];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) {
-        o[k] = zero_unit<T, 8>();
-        if (hit != 0) {
-          o[k] = load_eight<kWide, 32>(d_out + static_cast<int64_t>(t0 + __ffs(hit) - 1) * d + slab, lane, left);
-          hit &= hit - 1;
-        }
-      }
-#pragma unroll
-      for (int k = 0; k < kAhead; ++k)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] += to_f32(o[k].e[e]);
+    for (int k = 0; k < kLook; ++k) {
+      const uint32_t t = block + k * 32 + lane;
+      hits[k] = t < hi && index.at(t) == row;
     }
+#pragma unroll
+    for (int k = 0; k < kLook; ++k) hits[k] = __ballot_sync(0xffffffffu, hits[k]);
+#pragma unroll 1
+    for (int look = 0; look < kLook; ++look) {
+      uint32_t hit = hits[0];
+#pragma unroll
+      for (int k = 0; k + 1 < kLook; ++k) hits[k] = hits[k + 1];
+      const uint32_t t0 = block + look * 32;
+      while (hit != 0) {
+        Unit<T, 8> o[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          o[k] = zero_unit<T, 8>();
+          if (hit != 0) {
+            o[k] = load_eight<kWide, 32>(d_out + static_cast<int64_t>(t0 + __ffs(hit) - 1) * d + slab, lane, left);
+            hit &= hit - 1;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[e] += to_f32(o[k].e[e]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) total[e] += acc[e];
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = acc[e];
+  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = total[e];
   __syncthreads();
-  if (warp != 0) return;
+  if (threadIdx.x >= kSlab) return;
+  const int c = channel_of<kWide, 32>(lane, warp);  // thread 32 e + lane joins value e of the lanes
+  float sum = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-#pragma unroll
-    for (int w = 1; w < kThreads / 32; ++w) acc[e] += sums[w][lane + e * 32];
-    acc[e] *= scale;
-  }
-  store_eight<kWide, 32>(d_table, table_dtype, static_cast<int64_t>(row) * d + slab, lane, left, acc);
+  for (int w = 0; w < kWarps; ++w) sum += sums[w][threadIdx.x];
+  if (c < left) store_any(d_table, static_cast<int64_t>(row) * d + slab + c, table_dtype, sum * scale);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -667,7 +682,11 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   Plan p = {};
   const uint64_t tokens = static_cast<uint64_t>(d->tokens);
   p.slabs = (d->d + kSlab - 1) / kSlab;
-  p.few = tokens <= 2048 && tokens * static_cast<uint64_t>(d->rows) <= (1u << 22);
+  // Few tokens: looking through all indices once per table row and slab takes about 1.3 ns + 0.8 ps a token for each of them, the
+  // sort 17 to 40 us whatever its size.  Up to 4096 tokens, so that a row that takes most of them stays short too.  (128
+  // channels, looking against sorting: 1024 tokens into 21 rows 4.3 against 18 us, 4096 into 2048 rows 15 against 39, 1024
+  // into 16384 rows 33 against 38.)
+  p.few = tokens <= 4096 && static_cast<uint64_t>(d->rows) * p.slabs * (tokens + 1600) <= (1u << 25);
   if (p.few) {
     p.bytes = 256;
     return p;
@@ -677,10 +696,10 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   p.passes = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digit_bits = (bits + p.passes - 1) / p.passes;
   p.bins = 1 << p.digit_bits;
-  // tiles of at least 256 tokens, at most 16 warps an SM, and no more counters than tokens (one SM's worth aside)
-  uint64_t most = tokens / p.bins > static_cast<uint64_t>(sms) ? tokens / p.bins : sms;
+  // tiles of at least 64 tokens, at most 16 warps an SM, and at most two counters a token (one SM's worth of tiles aside)
+  uint64_t most = 2 * tokens / p.bins > static_cast<uint64_t>(sms) ? 2 * tokens / p.bins : sms;
   if (most > static_cast<uint64_t>(sms) * 16) most = static_cast<uint64_t>(sms) * 16;
-  uint64_t tiles = (tokens + 255) / 256;
+  uint64_t tiles = (tokens + 63) / 64;
   if (tiles > most) tiles = most;
   p.tile = static_cast<uint32_t>(((tokens + tiles - 1) / tiles + 31) / 32 * 32);
   p.tiles = static_cast<uint32_t>((tokens + p.tile - 1) / p.tile);
@@ -736,9 +755,13 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   const Plan p = make_plan(d, sms);
   const uint32_t tokens = static_cast<uint32_t>(d->tokens);
   if (p.few) {
-    embed_grad_few_kernel<T, kWide><<<dim3(d->rows, p.slabs), kThreads, 0, s>>>(
-        index, static_cast<const T*>(d_out), d_table, d->table_dtype, tokens, d->d, d->scale);
-    return cudaGetLastError();
+    const int64_t ctas = static_cast<int64_t>(d->rows) * p.slabs;
+    const int warps = ctas <= 2 * sms ? 32 : ctas <= 4096 ? 16 : 8;
+    const auto kernel = warps == 32   ? embed_grad_few_kernel<T, kWide, 32>
+                        : warps == 16 ? embed_grad_few_kernel<T, kWide, 16>
+                                      : embed_grad_few_kernel<T, kWide, 8>;
+    return launch(kernel, dim3(d->rows, p.slabs), warps * 32, 0, s, index, static_cast<const T*>(d_out), d_table,
+                  static_cast<int>(d->table_dtype), tokens, static_cast<int>(d->d), d->scale);
   }
   char* ws = static_cast<char*>(workspace);
   cudaError_t e;

@@ -336,7 +336,8 @@ def indices(kind, n, rows, dtype, seed=0):
 @pytest.mark.parametrize("n,rows,d", [(1, 1, 1), (5, 3, 8), (37, 21, 131), (300, 7, 256), (2047, 66, 128), (2500, 66, 264),
                                       (6000, 3000, 64), (3000, 100000, 32), (4097, 2, 1031), (1, 5000, 8192), (40000, 139, 24)])
 def test_embedding_and_its_gradient(n, rows, d, dtype, table_dtype):
-    """Sums of d_out: fp32 over at most 256 tokens, beyond that in 64 bits: 264 x 2^-24 < 2^-15 of the absolute values."""
+    """Sums of d_out are fp32 in steps: at most 128 terms, then at most 64, then the parts of 32 warps or of the shares (in 64 bits):
+    fewer than 512 roundings of 2^-24, 2^-15 of the absolute values."""
     p = P()
     for k, kind in enumerate(("uniform", "skewed", "sorted", "holes", "one", "none")):
         index = indices(kind, n, rows, torch.int32 if k % 2 else torch.int64)
