@@ -163,7 +163,8 @@ __global__ void __launch_bounds__(kWarps * 32) embed_grad_few_kernel(IndexView i
   const int slab = blockIdx.y * kSlab, left = d - slab;
   const uint32_t share = ((tokens + kWarps * 32 - 1) / (kWarps * 32)) * 32;
   const uint32_t lo = min(tokens, warp * share), hi = min(tokens, lo + share);
-  float total[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = 0.f;
   for (uint32_t block = lo; block < hi; block += 32 * kLook) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // of a block first: at most 128 terms, then at most 32
     uint32_t hits[kLook];
@@ -197,10 +198,8 @@ __global__ void __launch_bounds__(kWarps * 32) embed_grad_few_kernel(IndexView i
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) total[e] += acc[e];
+    for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] += acc[e];
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = total[e];
   __syncthreads();
   if (threadIdx.x >= kSlab) return;
   const int c = channel_of<kWide, 32>(lane, warp);  // thread 32 e + lane joins value e of the lanes
