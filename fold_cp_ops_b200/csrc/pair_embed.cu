@@ -740,12 +740,10 @@ cudaError_t embed_run(const pair_embed_desc_t* d, const IndexView& index, const 
   const int64_t most = static_cast<int64_t>(sms) * 8;
   if (wide) {
     const int64_t need = (d->tokens * a.octs + kThreads - 1) / kThreads;
-    embed_octs_kernel<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, make_fast_div(a.octs));
-  } else {
-    const int64_t need = (d->tokens + kThreads / 32 - 1) / (kThreads / 32);
-    embed_rows_kernel<T><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a);
+    return launch(embed_octs_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
   }
-  return cudaGetLastError();
+  const int64_t need = (d->tokens + kThreads / 32 - 1) / (kThreads / 32);
+  return launch(embed_rows_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a);
 }
 
 template <typename T, bool kWide>
@@ -854,6 +852,9 @@ extern "C" int pair_sm100_embed(const pair_embed_desc_t* desc, const void* index
   if (desc->tokens == 0) return TRIMUL_OK;
   if (index == nullptr || table == nullptr || out == nullptr)
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: index, table and out must not be NULL", who);
+  if (!elements_aligned(type_bytes(desc->dtype), {}, {base, out}) || !aligned(index, desc->index_bits / 8) ||
+      !aligned(table, type_bytes(desc->table_dtype)))
+    return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", who);
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   const IndexView view{index, desc->index_bits, static_cast<uint32_t>(desc->rows)};
@@ -896,6 +897,9 @@ extern "C" int pair_sm100_embed_grad(const pair_embed_desc_t* desc, const void* 
   if (index == nullptr || d_out == nullptr) return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: index and d_out must not be NULL", who);
   if (workspace == nullptr || !aligned(workspace, 16))
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace", who);
+  if (!aligned(d_out, type_bytes(desc->dtype)) || !aligned(index, desc->index_bits / 8) ||
+      !aligned(d_table, type_bytes(desc->table_dtype)))
+    return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", who);
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   const IndexView view{index, desc->index_bits, static_cast<uint32_t>(desc->rows)};

@@ -85,10 +85,15 @@ bool same(const Tensor& a, const Tensor& b) {
 
 std::string describe(const Tensor& t) { return c10::str(t.sizes(), " ", t.scalar_type(), " on ", t.device()); }
 
+// What the memory holds is what the tensor says (no lazy negation).
+Tensor unlazy(const Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 // Contiguous channels (a copy where they are not).
 Tensor channels(const Tensor& t) {
-  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? t : t.contiguous();
+  return !t.defined() || t.size(-1) == 1 || t.stride(-1) == 1 ? unlazy(t) : unlazy(t).contiguous();
 }
+
+Tensor packed(const Tensor& t) { return t.defined() ? unlazy(t).contiguous() : t; }
 
 // The last one to four axes are (b, i, j, d).
 pair_tensor_t view(const Tensor& t) {
@@ -129,8 +134,10 @@ struct Dropping {
 
 const pair_dropout_t kNoDropout = {0, 0, 65536u, nullptr, PAIR_SHARED_NONE, 0, 0, 0};
 
-Dropping dropping(const std::string& bytes, const Tensor& seed) {
+Dropping dropping(const std::string& bytes, const Tensor& seed, const Tensor& like) {
   Dropping d{kNoDropout, seed};
+  if (seed.defined() && seed.device() != like.device())
+    refuse("the dropout's seed must be on ", like.device(), " like the tensors; it is on ", seed.device());
   if (!bytes.empty()) {
     TORCH_CHECK(bytes.size() == sizeof(pair_dropout_t), "a dropout record has ", sizeof(pair_dropout_t), " bytes");
     std::memcpy(&d.record, bytes.data(), sizeof(pair_dropout_t));
@@ -225,7 +232,7 @@ Tensor run_add(const Tensor& update, const Tensor& residual, const Dropping& dro
 std::tuple<Tensor, Tensor> run_norm(const Tensor& update, const Tensor& residual, const Tensor& weight, double eps,
                                     const Dropping& drop, int group, const Tensor& scales) {
   const c10::cuda::OptionalCUDAGuard guard(update.device());
-  const Tensor u = channels(update), r = channels(residual), w = weight.contiguous();
+  const Tensor u = channels(update), r = channels(residual), w = packed(weight);
   const Tensor z = residual.defined() || drop.on() ? fresh(update) : Tensor();
   const Tensor y = group != 0 ? at::empty(update.sizes(), update.options().dtype(at::kFloat8_e4m3fn)) : fresh(update);
   const pair_norm_desc_t d = norm_desc(u, w, eps, group, drop);
@@ -239,7 +246,7 @@ std::tuple<Tensor, Tensor> run_norm(const Tensor& update, const Tensor& residual
 std::tuple<Tensor, Tensor, Tensor> run_norm_grad(const Tensor& stream, const Tensor& dy, const Tensor& dz, const Tensor& weight,
                                                  double eps, const Dropping& drop, bool need_u, bool need_r, bool need_w) {
   const c10::cuda::OptionalCUDAGuard guard(stream.device());
-  const Tensor z = channels(stream), y = channels(dy), g = channels(dz), w = weight.contiguous();
+  const Tensor z = channels(stream), y = channels(dy), g = channels(dz), w = packed(weight);
   const bool own_u = need_u && (drop.on() || !need_r);
   const Tensor du = own_u ? fresh(stream) : Tensor(), dr = need_r ? fresh(stream) : Tensor();
   const pair_norm_desc_t d = norm_desc(z, w, eps, 0, drop);
@@ -271,7 +278,7 @@ pair_embed_desc_t embed_desc(const Tensor& index, int64_t rows, int64_t d, at::S
 
 Tensor run_embed(const Tensor& index, const Tensor& table, const Tensor& base, double scale, at::ScalarType dtype) {
   const c10::cuda::OptionalCUDAGuard guard(index.device());
-  const Tensor x = index.contiguous(), t = table.contiguous(), b = base.defined() ? base.contiguous() : base;
+  const Tensor x = index.contiguous(), t = packed(table), b = packed(base);
   std::vector<int64_t> shape(index.sizes().begin(), index.sizes().end());
   shape.push_back(table.size(1));
   const Tensor out = at::empty(shape, table.options().dtype(dtype));
@@ -282,7 +289,7 @@ Tensor run_embed(const Tensor& index, const Tensor& table, const Tensor& base, d
 
 Tensor run_embed_grad(const Tensor& index, const Tensor& d_out, int64_t rows, at::ScalarType table_dtype, double scale) {
   const c10::cuda::OptionalCUDAGuard guard(index.device());
-  const Tensor x = index.contiguous(), g = d_out.contiguous();
+  const Tensor x = index.contiguous(), g = packed(d_out);
   const Tensor d_table = at::empty({rows, g.size(-1)}, g.options().dtype(table_dtype));
   const pair_embed_desc_t d = embed_desc(x, rows, g.size(-1), g.scalar_type(), table_dtype, scale);
   uint64_t bytes = 0;
@@ -316,13 +323,13 @@ struct DropoutAdd : torch::autograd::Function<DropoutAdd> {
     ctx->saved_data["drop"] = drop;
     ctx->saved_data["residual"] = residual.has_value();
     ctx->save_for_backward({or_none(seed)});
-    return run_add(update, or_none(residual), dropping(drop, or_none(seed)), Tensor());
+    return run_add(update, or_none(residual), dropping(drop, or_none(seed), update), Tensor());
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     Tensor du, dz = grads[0];
     const variable_list saved = ctx->get_saved_variables();  // raises where the seed's values were changed
     if (dz.defined() && ctx->needs_input_grad(0)) {
-      const Dropping drop = dropping(ctx->saved_data["drop"].toStringRef(), saved[0]);
+      const Dropping drop = dropping(ctx->saved_data["drop"].toStringRef(), saved[0], dz);
       du = drop.on() ? run_add(dz, Tensor(), drop, Tensor()) : dz;
     }
     const bool need_r = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(1);
@@ -336,7 +343,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
   static variable_list forward(AutogradContext* ctx, const Tensor& update, const std::optional<Tensor>& residual, const Tensor& weight,
                                const std::optional<Tensor>& seed, double eps, const std::string& drop) {
     ctx->set_materialize_grads(false);
-    auto [y, z] = run_norm(update, or_none(residual), weight, eps, dropping(drop, or_none(seed)), 0, Tensor());
+    auto [y, z] = run_norm(update, or_none(residual), weight, eps, dropping(drop, or_none(seed), update), 0, Tensor());
     if (!z.defined()) z = update.view_as(update);
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["drop"] = drop;
@@ -351,7 +358,7 @@ struct AddRmsNorm : torch::autograd::Function<AddRmsNorm> {
       const bool residual = ctx->saved_data["residual"].toBool();
       std::tie(out[0], out[1], out[2]) =
           run_norm_grad(saved[0], grads[0], grads[1], saved[1], ctx->saved_data["eps"].toDouble(),
-                        dropping(ctx->saved_data["drop"].toStringRef(), saved[2]), ctx->needs_input_grad(0),
+                        dropping(ctx->saved_data["drop"].toStringRef(), saved[2], saved[0]), ctx->needs_input_grad(0),
                         residual && ctx->needs_input_grad(1), ctx->needs_input_grad(residual ? 2 : 1));
     }
     out = once(std::move(out));
@@ -394,14 +401,14 @@ Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_,
   check_pair(update, residual);
   if (out.defined()) {
     if (wants_grad({&update, &residual, &out})) refuse("out= has no gradient: leave it out, or run under torch.no_grad()");
-    if (!same(out, update) || !out.is_contiguous()) refuse("out must be a contiguous ", describe(update), " tensor; got ", describe(out));
+    if (!same(out, update) || !out.is_contiguous() || out.is_neg()) refuse("out must be a contiguous ", describe(update), " tensor; got ", describe(out));
     check_overlap(out, update, "update");
     check_overlap(out, residual, "residual");
   } else if (wants_grad({&update, &residual})) {
     check_capture({&update, &residual});
     return DropoutAdd::apply(update, residual_, seed, drop);
   }
-  return run_add(update, residual, dropping(drop, or_none(seed)), out);
+  return run_add(update, residual, dropping(drop, or_none(seed), update), out);
 }
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optional<Tensor>& residual_, const Tensor& weight, double eps,
@@ -414,12 +421,13 @@ std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optiona
     variable_list out = AddRmsNorm::apply(update, residual_, weight, seed, eps, drop);
     return {out[0], out[1]};
   }
-  auto [y, z] = run_norm(update, residual, weight, eps, dropping(drop, or_none(seed)), 0, Tensor());
+  auto [y, z] = run_norm(update, residual, weight, eps, dropping(drop, or_none(seed), update), 0, Tensor());
   return {y, z.defined() ? z : update};
 }
 
 // Lanes reduce a group's octs: rows have to start on 16-byte boundaries (a copy where they do not).
-Tensor aligned(const Tensor& t) {
+Tensor aligned(const Tensor& given) {
+  const Tensor t = unlazy(given);
   if (!t.defined() || t.numel() == 0) return t;
   const int64_t unit = 16 / t.element_size();
   bool fits = reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(-1) == 1 || t.stride(-1) == 1);
@@ -442,7 +450,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& update_, const
   std::vector<int64_t> shape(update.sizes().begin(), update.sizes().end());
   shape.back() = width / g;
   const Tensor scales = at::empty(shape, update.options().dtype(at::kFloat));
-  auto [q, z] = run_norm(update, residual, weight, eps, dropping(drop, or_none(seed)), static_cast<int>(g), scales);
+  auto [q, z] = run_norm(update, residual, weight, eps, dropping(drop, or_none(seed), update), static_cast<int>(g), scales);
   return {q, scales, z.defined() ? z : update_};
 }
 

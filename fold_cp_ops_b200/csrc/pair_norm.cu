@@ -305,8 +305,7 @@ cudaError_t launch_add(const NormArgs<T>& a, int sms, cudaStream_t s) {
   constexpr int kFlight = sizeof(T) == 2 ? 2 : 1;
   const int64_t total = static_cast<int64_t>(a.rows) * a.octs;
   const int64_t need = (total + kThreads - 1) / kThreads, most = static_cast<int64_t>(sms) * 8;
-  add_octs_kernel<T, kFlight><<<static_cast<unsigned>(need < most ? need : most), kThreads, 0, s>>>(a, make_fast_div(a.octs));
-  return cudaGetLastError();
+  return launch(add_octs_kernel<T, kFlight>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
 }
 
 template <typename T, int kU, int kGroup, int kUnits, int kMode>
@@ -324,8 +323,7 @@ cudaError_t launch_rows(const NormArgs<T>& a, int sms, cudaStream_t stream) {
   static const int resident[2] = {resident_ctas(kernel, kWide, kStages), resident_ctas(kernel, kWide, 2 * kStages)};
   const uint32_t need = (a.rows + kRows - 1) / kRows;
   const uint32_t most = static_cast<uint32_t>(sms) * resident[has_residual];
-  kernel<<<need < most ? need : most, kWide, smem, stream>>>(a);
-  return cudaGetLastError();
+  return pair::launch(kernel, need < most ? need : most, kWide, smem, stream, a);
 }
 
 // Octs.
@@ -449,6 +447,9 @@ extern "C" int pair_sm100_add_norm(const pair_norm_desc_t* desc, const pair_tens
   if (update == nullptr || update->data == nullptr)
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: update is NULL", who);
   const int size = type_bytes(desc->dtype);
+  if (!elements_aligned(size, {update, residual}, {stream, g == 0 ? y : nullptr}) || !aligned(scales, 4) ||
+      !aligned(weight, type_bytes(desc->weight_dtype)) || !aligned(desc->dropout.device_seed, 8))
+    return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", who);
   const int unit = unit_of(desc->d, size, {update, residual}, {stream, g == 0 ? y : nullptr});
   if (g != 0 && g != desc->d && (unit != 8 || !aligned(y, 8)))
     return report_error(TRIMUL_ERR_UNSUPPORTED_SHAPE, "%s: scales per group need rows that start on 16-byte boundaries", who);

@@ -248,8 +248,7 @@ cudaError_t launch_rows(const GradArgs<T>& a, uint32_t grid, cudaStream_t stream
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSums + kStages);
     if (e != cudaSuccess) return e;
   }
-  kernel<<<grid, kWide, kStages + (a.partial != nullptr ? kSums : 0), stream>>>(a);
-  return cudaGetLastError();
+  return pair::launch(kernel, grid, kWide, kStages + (a.partial != nullptr ? kSums : 0), stream, a);
 }
 
 template <typename T, int kU>
@@ -355,6 +354,10 @@ extern "C" int pair_sm100_add_norm_grad(const pair_norm_desc_t* desc, const pair
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: stream is NULL", who);
   if (d_weight != nullptr && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0))
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: the weight's gradient needs an 8-byte aligned workspace", who);
+  const int weight_size = type_bytes(desc->weight_dtype);
+  if (!elements_aligned(type_bytes(desc->dtype), {stream, dy, dz}, {d_stream, d_update}) || !aligned(weight, weight_size) ||
+      !aligned(d_weight, weight_size) || !aligned(desc->dropout.device_seed, 8))
+    return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", who);
   const int sms = trimul::current_device_sms();
   if (sms <= 0) return report_error(TRIMUL_ERR_CUDA, "%s: cannot query the current device", who);
   cudaError_t e;

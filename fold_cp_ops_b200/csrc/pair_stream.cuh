@@ -547,6 +547,15 @@ inline bool rows_aligned(const pair_tensor_t* t, int type_size, int bytes) {
   return aligned(t->data, bytes) && t->stride_b % m == 0 && t->stride_i % m == 0 && t->stride_j % m == 0;
 }
 
+// Whether every tensor of a call starts (and every row of a strided one) on a multiple of its elements.
+inline bool elements_aligned(int type_size, std::initializer_list<const pair_tensor_t*> strided, std::initializer_list<const void*> flat) {
+  for (const pair_tensor_t* t : strided)
+    if (t != nullptr && !aligned(t->data, type_size)) return false;
+  for (const void* p : flat)
+    if (!aligned(p, type_size)) return false;
+  return true;
+}
+
 // Channels per memory access that every tensor of a call allows: 8, 2 (16-bit types) or 1.
 inline int unit_of(int d, int type_size, std::initializer_list<const pair_tensor_t*> strided, std::initializer_list<const void*> flat) {
   auto fits = [&](int unit, int bytes) {

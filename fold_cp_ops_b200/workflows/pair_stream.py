@@ -16,7 +16,8 @@ generator of exactly that position, so the gradient draws the mask again, and ra
 context-parallel grid draw the same mask as one GPU would.
 
 Tensors may be DTensors sharded over batch and token dims, as the distributed triangle update takes them: the blocks'
-positions are then taken from the placements.  Gradients are for plain tensors only.  Inputs need contiguous channels
+positions are then taken from the placements, and gains and tables may be replicated DTensors.  Gradients are for plain
+tensors only.  Inputs need contiguous channels
 (others are copied); other strides -- a transposed view, a block of a larger tensor, a broadcast axis -- are read in place.
 There is no CPU path.
 """
@@ -31,7 +32,8 @@ import torch
 from torch import Tensor
 
 from .. import _lib
-from ..distributed.dtensor_adapter import _dtensor_mesh_placements, _is_dtensor, _rowmaj_stride, _shards
+from ..distributed.dtensor_adapter import (_dtensor_mesh_placements, _effective_placements, _is_dtensor, _rowmaj_stride,
+                                           _shards)
 
 __all__ = ["PairDropout", "dropout_add", "add_rms_norm", "add_rms_norm_fp8", "pair_embedding", "pair_block_origin"]
 
@@ -54,7 +56,7 @@ class PairDropout:
     that is read when the kernel runs (``offset`` is then ignored here); it must keep its values until the gradient is computed.
     ``shared``: ``"rows"`` -- one mask for all rows ``i``; ``"columns"`` -- one for all columns ``j``; ``None`` -- every
     element its own.  ``origin``: the ``(b, i, j)`` of the tensor's first element in the whole grid, where the tensor is one
-    rank's block (DTensors know theirs)."""
+    rank's block (DTensors know theirs).  At most 65536 batch entries."""
 
     p: float
     seed: Union[int, Tensor] = 0
@@ -151,6 +153,17 @@ class _Wrap:
         return DTensor.from_local(local, self.mesh, self.placements, run_check=False, shape=shape, stride=_rowmaj_stride(shape))
 
 
+def _whole(t, name: str):
+    """A parameter that may be a replicated DTensor, as this rank holds it."""
+    if type(t) in _PLAIN or not _is_dtensor(t):
+        return t
+    if any(not p.is_replicate() for p in _effective_placements(*_dtensor_mesh_placements(t))):
+        raise ValueError(f"{name} must be whole on every rank; got placements {_dtensor_mesh_placements(t)[1]}")
+    if torch.is_grad_enabled() and t.requires_grad:
+        raise ValueError(_NO_DTENSOR_GRADIENT)
+    return t.to_local()
+
+
 def _no_gradient(wrap: Optional[_Wrap], *parameters: Tensor) -> None:
     if wrap is not None and torch.is_grad_enabled() and any(t.requires_grad for t in parameters):
         raise ValueError(_NO_DTENSOR_GRADIENT)
@@ -188,7 +201,7 @@ def add_rms_norm(update: Tensor, residual: Optional[Tensor], weight: Tensor, *, 
         (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
         _no_gradient(wrap, weight)
     drop, seed = _record(dropout, wrap)
-    y, z = _lib.pair_host().add_rms_norm(update, residual, weight, eps, drop, seed)
+    y, z = _lib.pair_host().add_rms_norm(update, residual, _whole(weight, "weight"), eps, drop, seed)
     return (y, z) if wrap is None else (wrap(y), wrap(z))
 
 
@@ -204,7 +217,7 @@ def add_rms_norm_fp8(update: Tensor, residual: Optional[Tensor], weight: Tensor,
     if type(update) not in _PLAIN or type(residual) not in _PLAIN:
         (update, residual), wrap = _locals_of(("update", "residual"), (update, residual))
     drop, seed = _record(dropout, wrap)
-    q, scales, z = _lib.pair_host().add_rms_norm_fp8(update, residual, weight, eps, group, drop, seed)
+    q, scales, z = _lib.pair_host().add_rms_norm_fp8(update, residual, _whole(weight, "weight"), eps, group, drop, seed)
     return (q, scales, z) if wrap is None else (wrap(q), wrap(scales), wrap(z))
 
 
@@ -221,5 +234,5 @@ def pair_embedding(index: Tensor, table: Tensor, *, scale: float = 1.0, base: Op
     if type(index) not in _PLAIN or type(base) not in _PLAIN:
         (index, base), wrap = _locals_of(("index", "base"), (index, base))
         _no_gradient(wrap, table)
-    out = _lib.pair_host().pair_embedding(index, table, scale, base, dtype)
+    out = _lib.pair_host().pair_embedding(index, _whole(table, "table"), scale, base, dtype)
     return out if wrap is None else wrap(out)

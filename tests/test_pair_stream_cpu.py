@@ -160,6 +160,20 @@ def test_norm_refusals_of_the_c_entry(kw, pat):
         refused("pair_sm100_add_norm_grad", pat, d, t, None, None, 4096, 4096, None, None, None, None)
 
 
+def test_refusals_of_buffers_that_their_elements_do_not_fit():
+    t = Tensor4(4096, 64, 64, 64)
+    for args in ((Tensor4(4097, 64, 64, 64), None, 4096, 4096, 4096, None), (t, Tensor4(4097, 64, 64, 64), 4096, 4096, 4096, None),
+                 (t, None, 4097, 4096, 4096, None), (t, None, 4096, 4097, 4096, None), (t, None, 4096, 4096, 4097, None)):
+        refused("pair_sm100_add_norm", "not aligned", _norm(), *args, None)
+    refused("pair_sm100_add_norm", "not aligned", _norm(dtype=2), Tensor4(4098, 64, 64, 64), None, 4096, 4096, 4096, None, None)
+    refused("pair_sm100_add_norm_grad", "not aligned", _norm(), t, Tensor4(4097, 64, 64, 64), None, 4096, 4096, None, None, None, None)
+    refused("pair_sm100_add_norm_grad", "not aligned", _norm(), t, None, None, 4096, 4096, None, 4097, 4096, None)
+    d = EmbedDesc(10, 64, 5, 64, BF16, BF16, 1.0)
+    refused("pair_sm100_embed", "not aligned", d, 4100, 4096, None, 4096, None)
+    refused("pair_sm100_embed", "not aligned", d, 4096, 4096, 4097, 4096, None)
+    refused("pair_sm100_embed_grad", "not aligned", d, 4096, 4096, 4097, 4096, None)
+
+
 def test_norm_refusals_of_missing_buffers():
     d, t = _norm(), Tensor4(4096, 64, 64, 64)
     for args, pat in (((None, 4096, 4096, None, None), "come together"), ((None, None, 4096, 4096, None), "come together"),

@@ -78,6 +78,8 @@ def _ranks(rank, world):
                 q, scales, z = P.add_rms_norm_fp8(dx, dr, w, group=32, dropout=drop)
                 assert q.full_tensor().shape == x.shape and scales.full_tensor().shape == (2, 12, 10, 1)
             assert torch.equal(P.pair_embedding(di, table, base=dx).full_tensor(), host.pair_embedding(index, table, 1.0, x, None))
+            whole = distribute_tensor(w, mesh, [Replicate()] * mesh.ndim)
+            assert torch.equal(P.add_rms_norm(dx, None, whole)[0].full_tensor(), P.add_rms_norm(dx, None, w)[0].full_tensor())
         mesh, placements = meshes[0]
         dx = distribute_tensor(x, mesh, placements)
         bad = [lambda: P.dropout_add(dx, r), lambda: P.dropout_add(dx, distribute_tensor(r, mesh, (Shard(2), Shard(1)))),
@@ -85,7 +87,9 @@ def _ranks(rank, world):
                lambda: P.dropout_add(DTensor.from_local(x, mesh, (Replicate(), Partial()))),
                lambda: P.dropout_add(distribute_tensor(x[0], mesh, (Shard(0), Shard(1)))),
                lambda: P.dropout_add(dx.detach().requires_grad_()), lambda: P.add_rms_norm(dx, None, w.clone().requires_grad_()),
-               lambda: P.pair_embedding(distribute_tensor(index, mesh, placements), table.clone().requires_grad_())]
+               lambda: P.pair_embedding(distribute_tensor(index, mesh, placements), table.clone().requires_grad_()),
+               lambda: P.add_rms_norm(dx, None, distribute_tensor(w, mesh, (Shard(0), Replicate()))),
+               lambda: P.add_rms_norm(dx, None, distribute_tensor(w, mesh, (Replicate(), Replicate())).requires_grad_())]
         for k, call in enumerate(bad):
             try:
                 call()

@@ -450,6 +450,46 @@ def test_refusals():
             call()
 
 
+@pytest.mark.parametrize("needs", [(1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 0, 1), (0, 1, 1)])
+def test_gradients_of_some_inputs_only(needs):
+    p = P()
+    ts = [rand(1, 3, 4, 72, seed=k) for k in (1, 2)] + [1 + rand(72, seed=3, scale=0.1)]
+    for drop in (None, p.PairDropout(0.25, seed=5)):
+        every = [t.clone().requires_grad_() for t in ts]
+        g = rand(1, 3, 4, 72, seed=4)
+        want = torch.autograd.grad(p.add_rms_norm(*every, dropout=drop)[0], every, g)
+        some = [t.clone().requires_grad_(bool(n)) for t, n in zip(ts, needs)]
+        got = torch.autograd.grad(p.add_rms_norm(*some, dropout=drop)[0], [t for t in some if t.requires_grad], g)
+        assert all(torch.equal(a, b) for a, b in zip(got, [w for w, n in zip(want, needs) if n]))
+        if not needs[2]:
+            some = some[:2]
+            z = p.dropout_add(*some, drop)
+            got = torch.autograd.grad(z, [t for t in some if t.requires_grad], g)
+            assert torch.equal(got[0], p.dropout_add(g, None, drop) if needs[0] else g)
+
+
+def test_lazily_negated_inputs():
+    p = P()
+    x = torch.view_as_complex(rand(1, 3, 4, 64, 2, seed=1)).conj().imag
+    assert x.is_neg()
+    w = torch.ones(64, device=DEV)
+    assert torch.equal(p.dropout_add(x, x), 2 * x.clone()) and torch.equal(p.add_rms_norm(x, x, w)[0], p.add_rms_norm(x.clone(), x.clone(), w)[0])
+    assert torch.equal(p.pair_embedding(torch.arange(3, device=DEV), x[0, :, 0]), x[0, :, 0].clone())
+
+
+def test_more_octs_than_32_bits_count():
+    """2^34 elements and some: the quotients of a 64-bit unit number."""
+    if torch.cuda.mem_get_info()[0] < 50 << 30:
+        pytest.skip("needs 50 GB of device memory")
+    p, d = P(), 8192
+    n = (1 << 34) // d + 5
+    row = rand(1, 1, 1, d, dtype=torch.bfloat16, seed=1).expand(1, 1, n, d)
+    drop, tail = p.PairDropout(0.25, seed=5), p.PairDropout(0.25, seed=5, origin=(0, 0, n - 9))
+    assert torch.equal(p.dropout_add(row, None, drop)[:, :, -9:], p.dropout_add(row[:, :, -9:], None, tail))
+    index, table = torch.arange(n, device=DEV) % 7, rand(7, d, dtype=torch.bfloat16, seed=6)
+    assert torch.equal(p.pair_embedding(index, table)[-9:], table[index[-9:]])
+
+
 def test_a_changed_device_seed_is_an_error_in_the_gradient():
     p = P()
     seed = torch.tensor([5, 1], device=DEV)
