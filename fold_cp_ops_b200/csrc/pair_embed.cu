@@ -126,24 +126,49 @@ __global__ void __launch_bounds__(kThreads) embed_octs_kernel(const EmbedArgs a,
   }
 }
 
-// Other rows: a warp per token, channels 32 apart.
+// Other rows: a warp takes 256 channels of a token at a time, 32 apart.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) embed_rows_kernel(const EmbedArgs a) {
+__global__ void __launch_bounds__(kThreads) embed_pieces_kernel(const EmbedArgs a, const FastDiv by_pieces) {
   const int lane = threadIdx.x & 31;
-  const uint32_t span = gridDim.x * (kThreads / 32);
-  for (uint32_t t = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); t < a.tokens; t += span) {
-    const uint32_t row = a.index.at(t);
-    const T* base = a.base != nullptr ? static_cast<const T*>(a.base) + static_cast<int64_t>(t) * a.d : nullptr;
-    T* out = static_cast<T*>(a.out) + static_cast<int64_t>(t) * a.d;
-    const int64_t at = static_cast<int64_t>(row) * a.d;
-#pragma unroll 8
-    for (int c = lane; c < a.d; c += 32) {
-      float f = row != kNone ? load_any(a.table, at + c, a.table_dtype) * a.scale : 0.f;
-      if (base != nullptr) f += to_f32(load_unit<T, 1>(base + c).e[0]);
-      Unit<T, 1> o;
-      o.e[0] = from_f32<T>(f);
-      store_unit<T, 1>(out + c, o);
+  const int64_t total = static_cast<int64_t>(a.tokens) * by_pieces.d;
+  const int64_t span = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t n = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); n < total; n += span) {
+    uint32_t t, piece;
+    if (total <= 0x7fffffff) {
+      t = by_pieces.div(static_cast<uint32_t>(n));
+      piece = static_cast<uint32_t>(n) - t * by_pieces.d;
+    } else {
+      t = static_cast<uint32_t>(n / by_pieces.d);
+      piece = static_cast<uint32_t>(n - static_cast<int64_t>(t) * by_pieces.d);
     }
+    const uint32_t row = a.index.at(t);
+    const int c0 = piece * 256 + lane;
+    const int64_t at = static_cast<int64_t>(t) * a.d + c0, from = static_cast<int64_t>(row) * a.d + c0;
+    const int left = a.d - c0;  // channels from the lane's first one on
+    Unit<T, 1> b[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      b[k] = zero_unit<T, 1>();
+      if (a.base != nullptr && k * 32 < left) b[k] = load_unit<T, 1>(static_cast<const T*>(a.base) + at + k * 32);
+    }
+    auto add = [&](const auto* table) {
+      float f[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = k * 32 < left ? to_f32(table[from + k * 32]) : 0.f;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) b[k].e[0] = from_f32<T>(f[k] * a.scale + to_f32(b[k].e[0]));
+    };
+    if (row != kNone) {
+      if (a.table_dtype == PAIR_FP32)
+        add(static_cast<const float*>(a.table));
+      else if (a.table_dtype == PAIR_FP16)
+        add(static_cast<const __half*>(a.table));
+      else
+        add(static_cast<const __nv_bfloat16*>(a.table));
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k * 32 < left) store_unit<T, 1>(static_cast<T*>(a.out) + at + k * 32, b[k]);
   }
 }
 
@@ -152,19 +177,29 @@ __global__ void __launch_bounds__(kThreads) embed_rows_kernel(const EmbedArgs a)
 // ---------------------------------------------------------------------------------------------
 // One CTA per table row (x) and slab of 256 channels (y): each warp looks through its part of the indices and adds the rows that
 // match, in ascending order; the warps' sums are joined in order.  The fewer rows there are, the more warps each takes (4096 tokens
-// into 21 rows: 7.4 us with 32, 12.7 with eight; into 2048 rows 22 and 13).
-template <typename T, bool kWide, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table,
-                                                                     int table_dtype, uint32_t tokens, int d, float scale) {
-  constexpr int kAhead = 4, kLook = kWarps > 8 ? 2 : 4;  // rows of d_out and blocks of 32 indices in flight
-  __shared__ float sums[kWarps][kSlab];
-  const uint32_t row = blockIdx.x;
+// into 21 rows: 7.4 us with 32, 12.7 with eight; into 2048 rows 22 and 13).  Of a table with more rows than there are tokens
+// (kByToken), each token's CTA takes the token's row, unless an earlier token has named it; the other rows are cleared before.
+template <typename T, bool kWide, bool kByToken>
+__global__ void __launch_bounds__(1024) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table, int table_dtype,
+                                                              uint32_t tokens, int d, float scale) {
+  constexpr int kAhead = 4, kLook = 4;  // rows of d_out and blocks of 32 indices in flight
+  extern __shared__ float sums[];       // (warps, kSlab)
+  const int threads = blockDim.x;
+  uint32_t row = blockIdx.x;
+  if constexpr (kByToken) {
+    row = index.at(blockIdx.x);
+    if (row == kNone) return;
+    int named = 0;
+    for (uint32_t t = threadIdx.x; t < blockIdx.x; t += threads) named |= index.at(t) == row;
+    if (__syncthreads_or(named)) return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slab = blockIdx.y * kSlab, left = d - slab;
-  const uint32_t share = ((tokens + kWarps * 32 - 1) / (kWarps * 32)) * 32;
+  const uint32_t share = ((tokens + threads - 1) / threads) * 32;
+  float* mine = sums + warp * kSlab + lane;
   const uint32_t lo = min(tokens, warp * share), hi = min(tokens, lo + share);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] = 0.f;
+  for (int e = 0; e < 8; ++e) mine[e * 32] = 0.f;
   for (uint32_t block = lo; block < hi; block += 32 * kLook) {
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // of a block first: at most 128 terms, then at most 32
     uint32_t hits[kLook];
@@ -198,14 +233,14 @@ __global__ void __launch_bounds__(kWarps * 32) embed_grad_few_kernel(IndexView i
       }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sums[warp][lane + e * 32] += acc[e];
+    for (int e = 0; e < 8; ++e) mine[e * 32] += acc[e];
   }
   __syncthreads();
   if (threadIdx.x >= kSlab) return;
   const int c = channel_of<kWide, 32>(lane, warp);  // thread 32 e + lane joins value e of the lanes
   float sum = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) sum += sums[w][threadIdx.x];
+#pragma unroll 8
+  for (int w = 0; w < threads / 32; ++w) sum += sums[w * kSlab + threadIdx.x];
   if (c < left) store_any(d_table, static_cast<int64_t>(row) * d + slab + c, table_dtype, sum * scale);
 }
 
@@ -669,7 +704,7 @@ __global__ void __launch_bounds__(kThreads) join_runs_kernel(const SumArgs<T> a)
 // host
 // ---------------------------------------------------------------------------------------------
 struct Plan {
-  bool few;
+  bool few, by_token;
   int passes, digit_bits, bins, group, slabs, width;
   uint32_t tiles, tile, share, ctas;
   uint64_t sorted_at[2], counts_at, totals_at, pieces_at, edges_at, bytes;
@@ -681,11 +716,13 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   Plan p = {};
   const uint64_t tokens = static_cast<uint64_t>(d->tokens);
   p.slabs = (d->d + kSlab - 1) / kSlab;
-  // Few tokens: looking through all indices once per table row and slab takes about 1.3 ns + 0.8 ps a token for each of them, the
-  // sort 17 to 40 us whatever its size.  Up to 4096 tokens, so that a row that takes most of them stays short too.  (128
-  // channels, looking against sorting: 1024 tokens into 21 rows 4.3 against 18 us, 4096 into 2048 rows 15 against 39, 1024
-  // into 16384 rows 33 against 38.)
-  p.few = tokens <= 4096 && static_cast<uint64_t>(d->rows) * p.slabs * (tokens + 1600) <= (1u << 25);
+  // Few tokens: looking through all indices once per table row (or, of a larger table, per token) and slab takes about 1.3 ns +
+  // 0.8 ps a token for each of them, the sort 17 to 40 us whatever its size.  Up to 4096 tokens, so that a row that takes most
+  // of them stays short too.  (128 channels, looking against sorting: 1024 tokens into 21 rows 4.3 against 18 us, 4096 into
+  // 2048 rows 15 against 39, 1024 into 16384 rows 11 by token against 38.)
+  // By token of tables with more rows than that, where clearing the table is worth its launch; a token's look costs about two rows'.
+  p.by_token = static_cast<uint64_t>(d->rows) > tokens && static_cast<uint64_t>(d->rows) * p.slabs > 1024;
+  p.few = tokens <= 4096 && (p.by_token ? 2 * tokens : d->rows) * p.slabs * (tokens + 1600) <= (1u << 25);
   if (p.few) {
     p.bytes = 256;
     return p;
@@ -742,8 +779,9 @@ cudaError_t embed_run(const pair_embed_desc_t* d, const IndexView& index, const 
     const int64_t need = (d->tokens * a.octs + kThreads - 1) / kThreads;
     return launch(embed_octs_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
   }
-  const int64_t need = (d->tokens + kThreads / 32 - 1) / (kThreads / 32);
-  return launch(embed_rows_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a);
+  const uint32_t pieces = (a.d + 255) / 256;
+  const int64_t need = (d->tokens * pieces + kThreads / 32 - 1) / (kThreads / 32);
+  return launch(embed_pieces_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(pieces));
 }
 
 template <typename T, bool kWide>
@@ -752,13 +790,16 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
   const Plan p = make_plan(d, sms);
   const uint32_t tokens = static_cast<uint32_t>(d->tokens);
   if (p.few) {
-    const int64_t ctas = static_cast<int64_t>(d->rows) * p.slabs;
+    const int64_t ctas = (p.by_token ? d->tokens : d->rows) * p.slabs;
     const int warps = ctas <= 2 * sms ? 32 : ctas <= 4096 ? 16 : 8;
-    const auto kernel = warps == 32   ? embed_grad_few_kernel<T, kWide, 32>
-                        : warps == 16 ? embed_grad_few_kernel<T, kWide, 16>
-                                      : embed_grad_few_kernel<T, kWide, 8>;
-    return launch(kernel, dim3(d->rows, p.slabs), warps * 32, 0, s, index, static_cast<const T*>(d_out), d_table,
-                  static_cast<int>(d->table_dtype), tokens, static_cast<int>(d->d), d->scale);
+    if (p.by_token) {
+      const cudaError_t e = cudaMemsetAsync(d_table, 0, static_cast<size_t>(d->rows) * d->d * type_bytes(d->table_dtype), s);
+      if (e != cudaSuccess) return e;
+    }
+    return launch(p.by_token ? embed_grad_few_kernel<T, kWide, true> : embed_grad_few_kernel<T, kWide, false>,
+                  dim3(static_cast<unsigned>(p.by_token ? d->tokens : d->rows), p.slabs), warps * 32, warps * kSlab * sizeof(float), s,
+                  index, static_cast<const T*>(d_out), d_table, static_cast<int>(d->table_dtype), tokens, static_cast<int>(d->d),
+                  d->scale);
   }
   char* ws = static_cast<char*>(workspace);
   cudaError_t e;

@@ -21,7 +21,7 @@ namespace {
 
 constexpr float kE4m3Max = 448.f;
 
-enum Mode { kNorm = 0, kNormE4m3 = 1, kAdd = 2 };
+enum Mode { kNorm = 0, kNormE4m3 = 1 };
 
 template <typename T>
 struct NormArgs {
@@ -82,8 +82,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
   Dropout drop = a.drop;
   if (dropping) resolve_seed(drop);
 
-  Lane<kU, kUnits> w;
-  if constexpr (kMode != kAdd) w = load_gain<kU, kGroup, kUnits>(a.weight, a.weight_dtype, lane, units);
+  const Lane<kU, kUnits> w = load_gain<kU, kGroup, kUnits>(a.weight, a.weight_dtype, lane, units);
 
   const uint32_t span = gridDim.x * kRows;
   const uint32_t mine = blockIdx.x * kRows + threadIdx.x / kGroup;  // this group's first row
@@ -173,8 +172,6 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
       for (int k = 0; k < kUnits; ++k)
         if (lane + k * kGroup < units) store_unit<T, kU>(a.stream + out + k * kGroup * kU, u[k]);
     }
-    if constexpr (kMode == kAdd) continue;
-
     Lane<kU, kUnits> v = unpack_all<T, kU, kUnits>(u);
     float ss[1] = {0.f};
     if constexpr (kClear) {
@@ -300,12 +297,73 @@ __global__ void __launch_bounds__(kThreads) add_octs_kernel(const __grid_constan
   }
 }
 
+// The addition alone, of other rows: a warp takes 256 channels of a row at a time, in units of kU channels per access.  Each
+// lane draws one of the piece's octs.
+template <typename T, int kU>
+__global__ void __launch_bounds__(kThreads) add_pieces_kernel(const __grid_constant__ NormArgs<T> a, const FastDiv by_pieces) {
+  constexpr int kUnits = 8 / kU;  // units of a lane
+  Dropout drop = a.drop;
+  const bool dropping = drop.keep < 65536u;
+  const bool has_residual = a.residual.p != nullptr;
+  const uint32_t line = drop.keep << 16;
+  if (dropping) resolve_seed(drop);
+  const int lane = threadIdx.x & 31;
+  const int64_t total = static_cast<int64_t>(a.rows) * by_pieces.d;
+  const int64_t span = static_cast<int64_t>(gridDim.x) * (kThreads / 32);
+  for (int64_t n = static_cast<int64_t>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5); n < total; n += span) {
+    uint32_t row, piece, b = 0, i = 0, j = 0;
+    if (total <= 0x7fffffff) {
+      row = by_pieces.div(static_cast<uint32_t>(n));
+      piece = static_cast<uint32_t>(n) - row * by_pieces.d;
+    } else {
+      row = static_cast<uint32_t>(n / by_pieces.d);
+      piece = static_cast<uint32_t>(n - static_cast<int64_t>(row) * by_pieces.d);
+    }
+    if (dropping || !a.flat) a.walk.at(row, b, i, j);
+    const int c0 = piece * 256 + lane * kU;  // the lane's first channel
+    const T* up = (a.flat ? a.update.flat(row) : a.update.row(b, i, j)) + c0;
+    const T* rp = (a.flat ? a.residual.flat(row) : a.residual.row(b, i, j)) + c0;
+    Unit<T, kU> u[kUnits], r[kUnits];
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k) {
+      const bool on = c0 + k * 32 * kU < a.d;
+      u[k] = on ? load_unit<T, kU>(up + k * 32 * kU) : zero_unit<T, kU>();
+      r[k] = on && has_residual ? load_unit<T, kU>(rp + k * 32 * kU) : zero_unit<T, kU>();
+    }
+    if (dropping) {
+      Lane<kU, kUnits> v = unpack_all<T, kU, kUnits>(u);
+      drop_all<kU, 32, kUnits>(drop, line, b, i, j, piece * (256 / kU) + lane, a.octs, v);
+      const Lane<kU, kUnits> x = unpack_all<T, kU, kUnits>(r);
+#pragma unroll
+      for (int k = 0; k < v.kPairs; ++k) v.p[k] = __fadd2_rn(v.p[k], x.p[k]);
+      pack_all<T, kU, kUnits>(v, u);
+    } else if (has_residual) {
+#pragma unroll
+      for (int k = 0; k < kUnits; ++k) u[k] = add_units(u[k], r[k]);
+    }
+    T* zp = a.stream + static_cast<int64_t>(row) * a.d + c0;
+#pragma unroll
+    for (int k = 0; k < kUnits; ++k)
+      if (c0 + k * 32 * kU < a.d) store_unit<T, kU>(zp + k * 32 * kU, u[k]);
+  }
+}
+
 template <typename T>
-cudaError_t launch_add(const NormArgs<T>& a, int sms, cudaStream_t s) {
-  constexpr int kFlight = sizeof(T) == 2 ? 2 : 1;
-  const int64_t total = static_cast<int64_t>(a.rows) * a.octs;
-  const int64_t need = (total + kThreads - 1) / kThreads, most = static_cast<int64_t>(sms) * 8;
-  return launch(add_octs_kernel<T, kFlight>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
+cudaError_t launch_add(const NormArgs<T>& a, int unit, int sms, cudaStream_t s) {
+  const int64_t most = static_cast<int64_t>(sms) * 8;
+  if (unit == 8) {
+    constexpr int kFlight = sizeof(T) == 2 ? 2 : 1;
+    const int64_t need = (static_cast<int64_t>(a.rows) * a.octs + kThreads - 1) / kThreads;
+    return launch(add_octs_kernel<T, kFlight>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
+  }
+  const uint32_t pieces = (a.d + 255) / 256;
+  const int64_t need = (static_cast<int64_t>(a.rows) * pieces + kThreads / 32 - 1) / (kThreads / 32);
+  const unsigned grid = static_cast<unsigned>(need < most ? need : most);
+  if constexpr (sizeof(T) == 2)
+    if (unit == 2) return launch(add_pieces_kernel<T, 2>, grid, kThreads, 0, s, a, make_fast_div(pieces));
+  if constexpr (sizeof(T) == 4)
+    if (unit == 4) return launch(add_pieces_kernel<T, 4>, grid, kThreads, 0, s, a, make_fast_div(pieces));
+  return launch(add_pieces_kernel<T, 1>, grid, kThreads, 0, s, a, make_fast_div(pieces));
 }
 
 template <typename T, int kU, int kGroup, int kUnits, int kMode>
@@ -357,8 +415,7 @@ cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
 
 template <typename T, int kMode>
 cudaError_t by_unit(const NormArgs<T>& a, int unit, int sms, cudaStream_t s) {
-  if constexpr (kMode != kAdd)
-    if (unit == 8) return wide_rows<T, kMode>(a, sms, s);
+  if (unit == 8) return wide_rows<T, kMode>(a, sms, s);
   if constexpr (sizeof(T) == 2)
     if (unit == 2) return narrow_rows<T, 2, kMode>(a, sms, s);
   return narrow_rows<T, 1, kMode>(a, sms, s);
@@ -385,8 +442,7 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* update, const pa
   a.flat = collapses(update, d->b, d->i, d->j) && collapses(residual, d->b, d->i, d->j);
   a.eps = d->eps;
   a.inv_d = 1.f / static_cast<float>(d->d);
-  if (y == nullptr && unit == 8) return launch_add<T>(a, sms, s);
-  if (y == nullptr) return by_unit<T, kAdd>(a, unit, sms, s);
+  if (y == nullptr) return launch_add<T>(a, unit, sms, s);
   return d->group != 0 ? by_unit<T, kNormE4m3>(a, unit, sms, s) : by_unit<T, kNorm>(a, unit, sms, s);
 }
 
@@ -450,7 +506,8 @@ extern "C" int pair_sm100_add_norm(const pair_norm_desc_t* desc, const pair_tens
   if (!elements_aligned(size, {update, residual}, {stream, g == 0 ? y : nullptr}) || !aligned(scales, 4) ||
       !aligned(weight, type_bytes(desc->weight_dtype)) || !aligned(desc->dropout.device_seed, 8))
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: a buffer is not aligned to its elements", who);
-  const int unit = unit_of(desc->d, size, {update, residual}, {stream, g == 0 ? y : nullptr});
+  int unit = unit_of(desc->d, size, {update, residual}, {stream, g == 0 ? y : nullptr});
+  if (y == nullptr && unit == 1 && size == 4 && units_fit(4, desc->d, size, {update, residual}, {stream})) unit = 4;
   if (g != 0 && g != desc->d && (unit != 8 || !aligned(y, 8)))
     return report_error(TRIMUL_ERR_UNSUPPORTED_SHAPE, "%s: scales per group need rows that start on 16-byte boundaries", who);
   if (g != 0 && !aligned(y, unit)) return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: an e4m3 output starts on an 8-byte boundary", who);

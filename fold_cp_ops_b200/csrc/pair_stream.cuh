@@ -423,7 +423,7 @@ __device__ __forceinline__ NarrowMask<kU, kUnits> draw_narrow(const Dropout& d, 
 template <int kU, int kUnits>
 __device__ __forceinline__ uint32_t narrow_bits(const NarrowMask<kU, kUnits>& m, int k) {
   const int lane = threadIdx.x & 31;
-  const int q = m.kPer * k + lane * kU / 8;  // kPer is 4 or 8, so all lanes share the slot q / 32
+  const int q = m.kPer * k + lane * kU / 8;  // kPer is 4, 8 or 16, so all lanes share the slot q / 32
   const int slot = m.kPer * k / 32;
   const uint32_t byte = (__shfl_sync(0xffffffffu, m.bits[slot / 4], q & 31) >> (8 * (slot & 3))) & 0xffu;
   return byte >> (lane * kU % 8);
@@ -440,8 +440,8 @@ __device__ __forceinline__ void drop_all(const Dropout& d, uint32_t line, uint32
     const auto mask = draw_narrow<kU, kUnits, kGroup>(d, line, b, i, j, lane & ~31, octs);
 #pragma unroll
     for (int n = 0; n < v.kPairs; ++n) {
-      const uint32_t x = narrow_bits<kU, kUnits>(mask, 2 * n / kU);
-      const uint32_t y = kU == 2 ? x >> 1 : narrow_bits<kU, kUnits>(mask, 2 * n + 1);
+      const uint32_t x = narrow_bits<kU, kUnits>(mask, 2 * n / kU) >> (2 * n % kU);
+      const uint32_t y = kU > 1 ? x >> 1 : narrow_bits<kU, kUnits>(mask, 2 * n + 1);
       v.p[n].x = x & 1u ? v.p[n].x * d.gain : 0.f;
       v.p[n].y = y & 1u ? v.p[n].y * d.gain : 0.f;
     }
@@ -556,18 +556,22 @@ inline bool elements_aligned(int type_size, std::initializer_list<const pair_ten
   return true;
 }
 
+// Whether every row of a call's tensors can be moved in units of so many channels.
+inline bool units_fit(int unit, int d, int type_size, std::initializer_list<const pair_tensor_t*> strided,
+                      std::initializer_list<const void*> flat) {
+  const int bytes = unit * type_size < 16 ? unit * type_size : 16;
+  if (d % unit != 0) return false;
+  for (const pair_tensor_t* t : strided)
+    if (!rows_aligned(t, type_size, bytes)) return false;
+  for (const void* p : flat)
+    if (!aligned(p, bytes)) return false;
+  return true;
+}
+
 // Channels per memory access that every tensor of a call allows: 8, 2 (16-bit types) or 1.
 inline int unit_of(int d, int type_size, std::initializer_list<const pair_tensor_t*> strided, std::initializer_list<const void*> flat) {
-  auto fits = [&](int unit, int bytes) {
-    if (d % unit != 0) return false;
-    for (const pair_tensor_t* t : strided)
-      if (!rows_aligned(t, type_size, bytes)) return false;
-    for (const void* p : flat)
-      if (!aligned(p, bytes)) return false;
-    return true;
-  };
-  if (fits(8, 16)) return 8;
-  return type_size == 2 && fits(2, 4) ? 2 : 1;
+  if (units_fit(8, d, type_size, strided, flat)) return 8;
+  return type_size == 2 && units_fit(2, d, type_size, strided, flat) ? 2 : 1;
 }
 
 }  // namespace pair
