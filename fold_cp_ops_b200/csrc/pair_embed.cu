@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads) embed_pieces_kernel(const EmbedArgs 
 // (kByToken), each token's CTA takes the token's row, unless an earlier token has named it; the other rows are cleared before.
 template <typename T, bool kWide, bool kByToken>
 __global__ void __launch_bounds__(1024) embed_grad_few_kernel(IndexView index, const T* d_out, void* d_table, int table_dtype,
-                                                              uint32_t tokens, int d, float scale) {
+                                                              uint32_t tokens, uint32_t share, int d, float scale) {
   constexpr int kAhead = 4, kLook = 4;  // rows of d_out and blocks of 32 indices in flight
   extern __shared__ float sums[];       // (warps, kSlab)
   const int threads = blockDim.x;
@@ -195,7 +195,6 @@ __global__ void __launch_bounds__(1024) embed_grad_few_kernel(IndexView index, c
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int slab = blockIdx.y * kSlab, left = d - slab;
-  const uint32_t share = ((tokens + threads - 1) / threads) * 32;
   float* mine = sums + warp * kSlab + lane;
   const uint32_t lo = min(tokens, warp * share), hi = min(tokens, lo + share);
 #pragma unroll
@@ -211,7 +210,7 @@ __global__ void __launch_bounds__(1024) embed_grad_few_kernel(IndexView index, c
 #pragma unroll
     for (int k = 0; k < kLook; ++k) hits[k] = __ballot_sync(0xffffffffu, hits[k]);
 #pragma unroll 1
-    for (int look = 0; look < kLook; ++look) {
+    for (int look = 0; look < kLook && block + look * 32 < hi; ++look) {
       uint32_t hit = hits[0];
 #pragma unroll
       for (int k = 0; k + 1 < kLook; ++k) hits[k] = hits[k + 1];
@@ -798,8 +797,8 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
     }
     return launch(p.by_token ? embed_grad_few_kernel<T, kWide, true> : embed_grad_few_kernel<T, kWide, false>,
                   dim3(static_cast<unsigned>(p.by_token ? d->tokens : d->rows), p.slabs), warps * 32, warps * kSlab * sizeof(float), s,
-                  index, static_cast<const T*>(d_out), d_table, static_cast<int>(d->table_dtype), tokens, static_cast<int>(d->d),
-                  d->scale);
+                  index, static_cast<const T*>(d_out), d_table, static_cast<int>(d->table_dtype), tokens,
+                  (tokens + warps * 32 - 1) / (warps * 32) * 32, static_cast<int>(d->d), d->scale);
   }
   char* ws = static_cast<char*>(workspace);
   cudaError_t e;
