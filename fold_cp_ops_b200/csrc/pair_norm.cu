@@ -399,17 +399,18 @@ cudaError_t wide_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
   return launch_rows<T, 8, 1024, 1, kMode>(a, sms, s);
 }
 
-// Units of one or two channels: four or eight channels per lane of a warp, then of a CTA.
+// Units of one or two channels: four to eight channels per lane of a warp, then eight per thread of a CTA (four of twice the threads
+// take up to 1.5 times as long: fewer rows are at hand on an SM).
 template <typename T, int kU, int kMode>
 cudaError_t narrow_rows(const NormArgs<T>& a, int sms, cudaStream_t s) {
   if (a.d <= 128) return launch_rows<T, kU, 32, 4 / kU, kMode>(a, sms, s);
   if constexpr (kU == 1)
     if (a.d <= 192) return launch_rows<T, kU, 32, 6, kMode>(a, sms, s);
   if (a.d <= 256) return launch_rows<T, kU, 32, 8 / kU, kMode>(a, sms, s);
-  if (a.d <= 512) return launch_rows<T, kU, 128, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 1024) return launch_rows<T, kU, 256, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 2048) return launch_rows<T, kU, 512, 4 / kU, kMode>(a, sms, s);
-  if (a.d <= 4096) return launch_rows<T, kU, 1024, 4 / kU, kMode>(a, sms, s);
+  if (a.d <= 512) return launch_rows<T, kU, 64, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 1024) return launch_rows<T, kU, 128, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 2048) return launch_rows<T, kU, 256, 8 / kU, kMode>(a, sms, s);
+  if (a.d <= 4096) return launch_rows<T, kU, 512, 8 / kU, kMode>(a, sms, s);
   return launch_rows<T, kU, 1024, 8 / kU, kMode>(a, sms, s);
 }
 

@@ -227,7 +227,7 @@ inline Shape shape_of(int unit, int d) {
   if (d <= 128) return {32, 4};
   if (unit == 1 && d <= 192) return {32, 6};
   if (d <= 256) return {32, 8};
-  return {d <= 512 ? 128 : d <= 1024 ? 256 : d <= 2048 ? 512 : 1024, d <= 4096 ? 4 : 8};
+  return {d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024, 8};
 }
 
 // CTAs of the gradient kernel: what 64 registers a thread let be resident (half of that for 16 channels a lane), or one
@@ -267,10 +267,10 @@ cudaError_t by_shape(const GradArgs<T>& a, Shape w, uint32_t grid, cudaStream_t 
     if constexpr (kU == 1)
       if (w.group == 32 && w.channels == 6) return launch_rows<T, kU, 32, 6>(a, grid, s);
     if (w.group == 32) return launch_rows<T, kU, 32, 8 / kU>(a, grid, s);
-    if (w.group == 128) return launch_rows<T, kU, 128, 4 / kU>(a, grid, s);
-    if (w.group == 256) return launch_rows<T, kU, 256, 4 / kU>(a, grid, s);
-    if (w.group == 512) return launch_rows<T, kU, 512, 4 / kU>(a, grid, s);
-    if (w.channels == 4) return launch_rows<T, kU, 1024, 4 / kU>(a, grid, s);
+    if (w.group == 64) return launch_rows<T, kU, 64, 8 / kU>(a, grid, s);
+    if (w.group == 128) return launch_rows<T, kU, 128, 8 / kU>(a, grid, s);
+    if (w.group == 256) return launch_rows<T, kU, 256, 8 / kU>(a, grid, s);
+    if (w.group == 512) return launch_rows<T, kU, 512, 8 / kU>(a, grid, s);
     return launch_rows<T, kU, 1024, 8 / kU>(a, grid, s);
   }
 }

@@ -451,7 +451,7 @@ __device__ __forceinline__ void drop_all(const Dropout& d, uint32_t line, uint32
 // ---------------------------------------------------------------------------------------------
 // sums over the lanes that share a row
 // ---------------------------------------------------------------------------------------------
-// A row has kGroup lanes: 8, 16 or 32 of a warp, or a CTA of its own of 128 to 1024 threads.
+// A row has kGroup lanes: 8, 16 or 32 of a warp, or a CTA of its own of 64 to 1024 threads.
 constexpr int kThreads = 256;
 __host__ __device__ constexpr int threads_of(int group) { return group <= 32 ? kThreads : group; }
 
