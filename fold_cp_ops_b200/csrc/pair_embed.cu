@@ -57,16 +57,16 @@ template <bool kWide, int kGroup>
 __device__ __forceinline__ void store_eight(void* table, int dtype, int64_t at, int lane, int left, const float (&f)[8]) {
   if constexpr (kWide) {
     if (lane * 8 >= left) return;
-    Vals<8> v;
+    Lane<8, 1> v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v.p[e] = make_float2(f[2 * e], f[2 * e + 1]);
     at += lane * 8;
     if (dtype == PAIR_FP32)
-      store_unit<float, 8>(static_cast<float*>(table) + at, pack<float, 8>(v));
+      store_unit<float, 8>(static_cast<float*>(table) + at, pack<float>(v));
     else if (dtype == PAIR_FP16)
-      store_unit<__half, 8>(static_cast<__half*>(table) + at, pack<__half, 8>(v));
+      store_unit<__half, 8>(static_cast<__half*>(table) + at, pack<__half>(v));
     else
-      store_unit<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(table) + at, pack<__nv_bfloat16, 8>(v));
+      store_unit<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(table) + at, pack<__nv_bfloat16>(v));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -87,7 +87,7 @@ struct EmbedArgs {
   float scale;
 };
 
-__device__ __forceinline__ Vals<8> table_oct(const void* table, int dtype, int64_t at) {
+__device__ __forceinline__ Lane<8, 1> table_oct(const void* table, int dtype, int64_t at) {
   if (dtype == PAIR_FP32) {
     Unit<float, 8> x;
     reinterpret_cast<uint4*>(&x)[0] = __ldg(reinterpret_cast<const uint4*>(static_cast<const float*>(table) + at));
@@ -116,13 +116,13 @@ __global__ void __launch_bounds__(kThreads) embed_octs_kernel(const EmbedArgs a,
     const uint32_t row = a.index.at(t);
     Unit<T, 8> b = zero_unit<T, 8>();
     if (base != nullptr) b = load_unit<T, 8>(base + n * 8);
-    Vals<8> f = unpack(b);
+    Lane<8, 1> f = unpack(b);
     if (row != kNone) {
-      const Vals<8> x = table_oct(a.table, a.table_dtype, static_cast<int64_t>(row) * a.d + v * 8);
+      const Lane<8, 1> x = table_oct(a.table, a.table_dtype, static_cast<int64_t>(row) * a.d + v * 8);
 #pragma unroll
       for (int e = 0; e < 4; ++e) f.p[e] = __ffma2_rn(x.p[e], both(a.scale), f.p[e]);
     }
-    store_unit<T, 8>(static_cast<T*>(a.out) + n * 8, pack<T, 8>(f));
+    store_unit<T, 8>(static_cast<T*>(a.out) + n * 8, pack<T>(f));
   }
 }
 
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, kSumCtas) sum_runs_kernel(const SumA
     }
   };
   auto add = [&](const Unit<T, 8>& o) {
-    const Vals<8> v = unpack(o);
+    const Lane<8, 1> v = unpack(o);
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[e] = __fadd2_rn(acc[e], v.p[e]);
   };

@@ -408,7 +408,9 @@ Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_,
     check_capture({&update, &residual});
     return DropoutAdd::apply(update, residual_, seed, drop);
   }
-  return run_add(update, residual, dropping(drop, or_none(seed), update), out);
+  const Tensor z = run_add(update, residual, dropping(drop, or_none(seed), update), out);
+  if (out.defined() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();  // graphs that saved out's old values notice
+  return z;
 }
 
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optional<Tensor>& residual_, const Tensor& weight, double eps,

@@ -51,17 +51,14 @@ __device__ __forceinline__ uint32_t e4m3x2(float2 v) {
 template <typename T>
 __device__ __forceinline__ Unit<T, 8> drop_and_add(const Dropout& d, uint32_t line, uint32_t b, uint32_t i, uint32_t j, uint32_t oct,
                                                    const Unit<T, 8>& u, const Unit<T, 8>& r, bool has_residual) {
-  const Unit<T, 8> in[1] = {u}, other[1] = {r};
-  Lane<8, 1> v = unpack_all<T, 8, 1>(in);
+  Lane<8, 1> v = unpack(u);
   drop_oct(draw_oct(d, b, i, j, oct), line, d.gain, v.p);
   if (has_residual) {
-    const Lane<8, 1> x = unpack_all<T, 8, 1>(other);
+    const Lane<8, 1> x = unpack(r);
 #pragma unroll
     for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
   }
-  Unit<T, 8> out[1];
-  pack_all<T, 8, 1>(v, out);
-  return out[0];
+  return pack<T>(v);
 }
 
 // kU channels per access, kGroup lanes per row, kUnits units per lane.

@@ -135,42 +135,8 @@ __device__ __forceinline__ Unit<T, kU> zero_unit() {
   return o;
 }
 
-// The fp32 values of a unit, in pairs for the packed fp32 instructions (one issue slot for two operations).
-template <int kU>
-struct Vals {
-  float2 p[(kU + 1) / 2];  // of a single channel, .y is 0
-};
-
-template <typename T, int kU>
-__device__ __forceinline__ Vals<kU> unpack(const Unit<T, kU>& o) {
-  Vals<kU> v;
-#pragma unroll
-  for (int k = 0; k < (kU + 1) / 2; ++k) {
-    v.p[k].x = to_f32(o.e[2 * k]);
-    v.p[k].y = 2 * k + 1 < kU ? to_f32(o.e[2 * k + 1 < kU ? 2 * k + 1 : 0]) : 0.f;
-  }
-  return v;
-}
-
-template <typename T, int kU>
-__device__ __forceinline__ Unit<T, kU> pack(const Vals<kU>& v) {
-  Unit<T, kU> o;
-  if constexpr (sizeof(T) == 2 && kU > 1) {
-#pragma unroll
-    for (int k = 0; k < kU / 2; ++k) {
-      if constexpr (__is_same(T, __half))
-        reinterpret_cast<__half2*>(&o)[k] = __float22half2_rn(v.p[k]);
-      else
-        reinterpret_cast<__nv_bfloat162*>(&o)[k] = __float22bfloat162_rn(v.p[k]);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(k & 1 ? v.p[k / 2].y : v.p[k / 2].x);
-  }
-  return o;
-}
-
-// The fp32 values of all units of a lane in pairs: channels of a unit, or, of one-channel units, two steps' units.
+// The fp32 values of all units of a lane in pairs, for the packed fp32 instructions (one issue slot for two operations): channels
+// of a unit, or, of one-channel units, two steps' units.
 template <int kU, int kUnits>
 struct Lane {
   static constexpr int kPairs = kU * kUnits / 2;
@@ -203,6 +169,19 @@ __device__ __forceinline__ void pack_all(const Lane<kU, kUnits>& v, Unit<T, kU> 
       u[(2 * n + 1) / kU].e[(2 * n + 1) % kU] = from_f32<T>(v.p[n].y);
     }
   }
+}
+
+// One oct.
+template <typename T>
+__device__ __forceinline__ Lane<8, 1> unpack(const Unit<T, 8>& o) {
+  const Unit<T, 8> u[1] = {o};
+  return unpack_all<T, 8, 1>(u);
+}
+template <typename T>
+__device__ __forceinline__ Unit<T, 8> pack(const Lane<8, 1>& v) {
+  Unit<T, 8> u[1];
+  pack_all<T, 8, 1>(v, u);
+  return u[0];
 }
 
 // a + b in the unit's type, rounded once: for 16-bit pairs the packed addition, which rounds the exact sum.

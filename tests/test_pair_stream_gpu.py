@@ -132,6 +132,21 @@ def test_in_place_and_refused_overlaps():
             p.dropout_add(x, None, drop, out=out)
 
 
+def test_out_counts_as_a_change_of_its_tensor():
+    p = P()
+    u, z = rand(2, 3, 16, seed=9), rand(2, 3, 16, seed=10)
+    w = torch.ones(16, device=DEV, requires_grad=True)
+    y = (z * w).sum()  # saves z
+    with torch.no_grad():
+        p.dropout_add(u, z, out=z)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        x = z + 0
+        assert torch.equal(p.dropout_add(u, x, out=x), u + z)
+    assert torch.equal(p.dropout_add(u, x, out=x), u + (u + z))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_dropout_gradient(dtype):
     p, shape = P(), (2, 5, 6, 72)
