@@ -773,14 +773,15 @@ cudaError_t embed_run(const pair_embed_desc_t* d, const IndexView& index, const 
   a.octs = (d->d + 7) / 8;
   a.table_dtype = d->table_dtype;
   a.scale = d->scale;
-  const int64_t most = static_cast<int64_t>(sms) * 8;
   if (wide) {
-    const int64_t need = (d->tokens * a.octs + kThreads - 1) / kThreads;
-    return launch(embed_octs_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
+    static const int resident = resident_ctas(embed_octs_kernel<T>, kThreads, 0);
+    const uint64_t need = (static_cast<uint64_t>(d->tokens) * a.octs + kThreads - 1) / kThreads;
+    return launch(embed_octs_kernel<T>, walk_grid(need, sms, resident, 4), kThreads, 0, s, a, make_fast_div(a.octs));
   }
+  static const int resident = resident_ctas(embed_pieces_kernel<T>, kThreads, 0);
   const uint32_t pieces = (a.d + 255) / 256;
-  const int64_t need = (d->tokens * pieces + kThreads / 32 - 1) / (kThreads / 32);
-  return launch(embed_pieces_kernel<T>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(pieces));
+  const uint64_t need = (static_cast<uint64_t>(d->tokens) * pieces + kThreads / 32 - 1) / (kThreads / 32);
+  return launch(embed_pieces_kernel<T>, walk_grid(need, sms, resident, 4), kThreads, 0, s, a, make_fast_div(pieces));
 }
 
 template <typename T, bool kWide>

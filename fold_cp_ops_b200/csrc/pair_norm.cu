@@ -10,16 +10,18 @@
 // fp32 pairs (and in packed 16-bit additions where there is no dropout).
 // Split.  A row of up to 256 channels is one oct (eight channels, 16 bytes of a 16-bit type) per lane of 8, 16 or 32 lanes, so
 // that the reductions stay inside a warp; up to 384 it is three octs of 16 lanes, up to 512 two of 32; wider rows take a CTA with
-// one oct per thread.  The grid is one wave of CTAs that walk over the rows; while one row of a lane is at hand the next is on its
-// way through shared memory.
-// Measured (of the 6457 GB/s of a copy): 1024 x 1024 rows of 256 bf16 channels to e4m3 333 us, 88 %; the addition alone with an
-// elementwise dropout 282 us, 88 %; 131072 fp32 rows of 256 94 us, 89 %; 384 x 384 rows of 128 with dropout 28 us, 82 %.
+// one oct per thread.  CTAs walk over the rows, eight rows a lane or one wave of CTAs (walk_grid); while one row of a lane is at hand
+// the next is on its way through shared memory.
+// Measured (of the 6457 GB/s of a copy): 1024 x 1024 rows of 256 bf16 channels to e4m3 293 us, 100 % (333 with one wave of CTAs); the
+// addition alone with an elementwise dropout 267 us, 93 % (282); 512 x 512 fp32 rows of 256 169 us, 98 % (193); 384 x 384
+// rows of 128 with dropout 31 us, 75 %: there the tensors are small and the fill and drain of the one wave or two show.
 #include "pair_stream.cuh"
 
 namespace pair {
 namespace {
 
 constexpr float kE4m3Max = 448.f;
+constexpr uint32_t kSteps = 8;  // rows that a lane of the norm takes, where there are enough for several waves
 
 enum Mode { kNorm = 0, kNormE4m3 = 1 };
 
@@ -98,7 +100,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
     }
   };
   // Two stages, one at hand and one on its way; each holds the update's row of every group, then the residual's.  (More are slower:
-  // 1024 x 1024 rows of 256 to e4m3 take 334 us with two, 357 with three or four.)
+  // with one wave of CTAs 1024 x 1024 rows of 256 to e4m3 take 334 us with two, 357 with three or four.)
   const int stage_bytes = In::kStage * (has_residual ? 2 : 1);
   auto fetch = [&](uint32_t row, int stage) {
     const T *up, *rp;
@@ -345,22 +347,29 @@ __global__ void __launch_bounds__(kThreads) add_pieces_kernel(const __grid_const
   }
 }
 
+template <typename T, int kU>
+cudaError_t launch_pieces(const NormArgs<T>& a, int sms, cudaStream_t s) {
+  auto kernel = add_pieces_kernel<T, kU>;
+  static const int resident = resident_ctas(kernel, kThreads, 0);
+  const uint32_t pieces = (a.d + 255) / 256;
+  const uint64_t need = (static_cast<uint64_t>(a.rows) * pieces + kThreads / 32 - 1) / (kThreads / 32);
+  return launch(kernel, walk_grid(need, sms, resident, 4), kThreads, 0, s, a, make_fast_div(pieces));
+}
+
 template <typename T>
 cudaError_t launch_add(const NormArgs<T>& a, int unit, int sms, cudaStream_t s) {
-  const int64_t most = static_cast<int64_t>(sms) * 8;
   if (unit == 8) {
     constexpr int kFlight = sizeof(T) == 2 ? 2 : 1;
-    const int64_t need = (static_cast<int64_t>(a.rows) * a.octs + kThreads - 1) / kThreads;
-    return launch(add_octs_kernel<T, kFlight>, static_cast<unsigned>(need < most ? need : most), kThreads, 0, s, a, make_fast_div(a.octs));
+    auto kernel = add_octs_kernel<T, kFlight>;
+    static const int resident = resident_ctas(kernel, kThreads, 0);
+    const uint64_t need = (static_cast<uint64_t>(a.rows) * a.octs + kThreads - 1) / kThreads;
+    return launch(kernel, walk_grid(need, sms, resident, 4 * kFlight), kThreads, 0, s, a, make_fast_div(a.octs));
   }
-  const uint32_t pieces = (a.d + 255) / 256;
-  const int64_t need = (static_cast<int64_t>(a.rows) * pieces + kThreads / 32 - 1) / (kThreads / 32);
-  const unsigned grid = static_cast<unsigned>(need < most ? need : most);
   if constexpr (sizeof(T) == 2)
-    if (unit == 2) return launch(add_pieces_kernel<T, 2>, grid, kThreads, 0, s, a, make_fast_div(pieces));
+    if (unit == 2) return launch_pieces<T, 2>(a, sms, s);
   if constexpr (sizeof(T) == 4)
-    if (unit == 4) return launch(add_pieces_kernel<T, 4>, grid, kThreads, 0, s, a, make_fast_div(pieces));
-  return launch(add_pieces_kernel<T, 1>, grid, kThreads, 0, s, a, make_fast_div(pieces));
+    if (unit == 4) return launch_pieces<T, 4>(a, sms, s);
+  return launch_pieces<T, 1>(a, sms, s);
 }
 
 template <typename T, int kU, int kGroup, int kUnits, int kMode>
@@ -374,11 +383,10 @@ cudaError_t launch_rows(const NormArgs<T>& a, int sms, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * kStages);
     if (e != cudaSuccess) return e;
   }
-  // one wave: what is resident with and without a residual's stages
+  // what is resident without and with a residual's stages
   static const int resident[2] = {resident_ctas(kernel, kWide, kStages), resident_ctas(kernel, kWide, 2 * kStages)};
   const uint32_t need = (a.rows + kRows - 1) / kRows;
-  const uint32_t most = static_cast<uint32_t>(sms) * resident[has_residual];
-  return pair::launch(kernel, need < most ? need : most, kWide, smem, stream, a);
+  return pair::launch(kernel, walk_grid(need, sms, resident[has_residual], kSteps), kWide, smem, stream, a);
 }
 
 // Octs.

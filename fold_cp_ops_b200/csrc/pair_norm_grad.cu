@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kU * kUnits > 8 ? 512 : 1
   }
 }
 
-// d_w[c] = sum over the CTAs' sums: 16 channels and 64 rows of sums per CTA, four rows of a thread in flight.
+// d_w[c] = sum over the CTAs' sums: 16 channels and 64 rows of sums per CTA, eight rows of a thread in flight.
 constexpr int kJoinChannels = 16, kJoinRows = 64;
 __global__ void __launch_bounds__(kJoinChannels* kJoinRows) join_weight_kernel(const double* partial, int parts, int d,
                                                                               void* d_weight, int dtype) {
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kJoinChannels* kJoinRows) join_weight_kernel(c
   double sum = 0.0;
   if (c < d) {
     const double* p = partial + c;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = y; r < parts; r += kJoinRows) sum += p[static_cast<int64_t>(r) * d];
   }
   s[y][x] = sum;
@@ -230,13 +230,12 @@ inline Shape shape_of(int unit, int d) {
   return {d <= 512 ? 64 : d <= 1024 ? 128 : d <= 2048 ? 256 : d <= 4096 ? 512 : 1024, 8};
 }
 
-// CTAs of the gradient kernel: what 64 registers a thread let be resident (half of that for 16 channels a lane), or one
-// per group of rows.
+// CTAs of the gradient kernel, from the sizes alone: what 64 registers a thread let be resident (half of that for 16 channels a lane),
+// or more where each still has 32 rows a lane and 256 rows in all: a CTA costs a row of sums.
 inline uint32_t grid_of(uint32_t rows, Shape w, int sms) {
   const uint32_t threads = threads_of(w.group), held = threads / w.group;
   const uint32_t need = (rows + held - 1) / held;
-  const uint32_t most = static_cast<uint32_t>(sms) * ((w.channels == 16 ? 512 : 1024) / threads);
-  return need < most ? need : most;
+  return walk_grid(need, sms, (w.channels == 16 ? 512 : 1024) / threads, held < 8 ? 256 / held : 32);
 }
 
 template <typename T, int kU, int kGroup, int kUnits>

@@ -514,6 +514,16 @@ int resident_ctas(K kernel, int threads, int smem) {
   return n < 1 ? 1 : n;
 }
 
+// The grid of a kernel whose CTAs walk over `need` steps in all: one wave of the `resident` CTAs an SM that fit, or as many whole waves
+// as leave each CTA about `steps` steps.  A single wave of equal shares ends with its slowest SM (a profile of one showed the others
+// idle for a fifth of the time); CTAs of a later wave go where one is done.
+inline unsigned walk_grid(uint64_t need, int sms, int resident, uint32_t steps) {
+  const uint64_t wave = static_cast<uint64_t>(sms) * resident;
+  if (need <= wave) return static_cast<unsigned>(need);
+  const uint64_t waves = (need / steps + wave / 2) / wave;
+  return static_cast<unsigned>(waves > 1 ? waves * wave : wave);
+}
+
 // Host-side checks shared by the entry points.
 int check_norm_desc(const pair_norm_desc_t* d, const char* who);
 int check_dtype(int dtype, const char* what, const char* who);
