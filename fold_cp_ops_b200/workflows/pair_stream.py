@@ -227,7 +227,7 @@ def pair_embedding(index: Tensor, table: Tensor, *, scale: float = 1.0, base: Op
 
     ``index``: int32 or int64, any shape; an entry outside ``[0, V)`` (``-1`` for padding) adds nothing and gets no gradient.
     ``table``: ``(V, D)`` in bfloat16, float16 or float32, ``D`` at most 8192; its gradient comes in its type, summed in at
-    least fp32 over tokens sorted by index, in a fixed order (the same bits every time).  ``base``: what the embedding is
+    least fp32 and in a fixed order (the same bits every time).  ``base``: what the embedding is
     added to, or ``None``; the result has its type, else ``dtype``, else the table's.  ``index`` and ``base`` may be DTensors
     sharded alike.  ``index``, ``base`` and the result's gradient are copied where they are not contiguous."""
     wrap = None

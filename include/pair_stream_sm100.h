@@ -6,7 +6,7 @@
  *                              or in e4m3 with fp32 scales
  *   pair_sm100_add_norm_grad   its gradients
  *   pair_sm100_embed           out = base + scale * table[index]
- *   pair_sm100_embed_grad      the table's gradient, summed over sorted tokens
+ *   pair_sm100_embed_grad      the table's gradient
  *
  * The conventions of trimul_sm100.h hold: 0 or a negative TRIMUL_ERR_* code with a message in
  * trimul_sm100_last_error(), caller-owned device memory, no allocation, no hidden stream, nothing throws.
@@ -109,7 +109,7 @@ int pair_sm100_embed(const pair_embed_desc_t* desc, const void* index, const voi
 
 int pair_sm100_embed_grad_workspace(const pair_embed_desc_t* desc, uint64_t* bytes);
 
-/* d_table[v] = scale * sum of d_out[t] over the tokens with index v, in ascending order of t (the same bits every
+/* d_table[v] = scale * sum of d_out[t] over the tokens with index v, in a fixed order (the same bits every
  * time); rows that no token names become 0. */
 int pair_sm100_embed_grad(const pair_embed_desc_t* desc, const void* index, const void* d_out, void* d_table,
                           void* workspace, trimul_stream_t cuda_stream);

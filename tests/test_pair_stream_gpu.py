@@ -384,6 +384,26 @@ def test_embedding_gradient_of_many_tokens(rows, kind):
     assert torch.equal(got[0], got[1])
 
 
+@pytest.mark.parametrize("kind", ["uniform", "sorted", "skewed", "holes", "one", "none"])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,rows,d", [(1025, 1, 1), (1025, 2, 8), (1400, 21, 131), (5000, 74, 66), (5000, 75, 66), (4800, 73, 200), (1700000, 2, 8),
+                                      (90001, 66, 64)])
+def test_embedding_gradient_of_small_tables(n, rows, d, dtype, kind):
+    """The tables that every warp has to itself, and the sizes next to them.  fp32 sums of at most 1024 terms per warp, joined in 64 bits
+    and rounded twice: fewer than 2048 roundings of 2^-24, 2^-13 of the absolute values.  Rows of d_out on odd boundaries as well, and
+    values at tokens without an embedding that no row may take."""
+    p = P()
+    index, table = indices(kind, n, rows, torch.int32), rand(rows, d, seed=1, dtype=dtype).requires_grad_()
+    for first in (0, 1):
+        d_out = rand(n * d + 1, seed=3, dtype=dtype)[first:n * d + first].view(n, d)
+        d_out[(index < 0) | (index >= rows)] = float("nan")
+        (got,) = torch.autograd.grad(p.pair_embedding(index, table, scale=-0.5), table, d_out)
+        want, terms = embedding_grad(index, rows, d_out.nan_to_num(0.0), -0.5)
+        near(got, want, terms, kind, 2.0 ** -13)
+        (again,) = torch.autograd.grad(p.pair_embedding(index, table, scale=-0.5), table, d_out)
+        assert torch.equal(got, again)
+
+
 def test_embedding_shapes_and_strides():
     p = P()
     table = rand(10, 48, seed=1, dtype=torch.bfloat16)
