@@ -11,6 +11,9 @@
 // sums of 32 terms lose about 2^-23, where sums of thousands would lose ten times that), the CTA's rows are
 // joined there and each CTA leaves one row of sums in the workspace.  A second kernel adds those in a fixed order:
 // no atomics, the same bits every time.
+// Measured (of the 6457 GB/s of a copy; with gradients of both outputs and of the gain): 1024 x 1024 rows of 256 bf16 channels 328 us, 101 %,
+// with dropout 440, 95 % (346 and 452 with one wave of CTAs); 700 x 700 fp32 rows of 256 303 and 405 us, 102 and 96 %; 384 x 384 bf16
+// rows of 128 29 and 39 us, 81 and 74 %: one wave, whose fill, drain and joining kernel show.
 #include "pair_stream.cuh"
 
 namespace pair {
