@@ -6,7 +6,7 @@
 // Bound.  Forward: HBM, base read and out written once; the table (tens of rows for position bins) stays in L1 and L2.
 // Gradient: HBM, d_out read once.  Position bins give some 10^6 tokens to each of a few dozen rows, vocabularies give
 // one or two, so the sum is organised by sorted tokens: a stable counting sort of the token numbers by index (up to
-// 2048 bins a pass, no comparison, pairs of int32 only), then every group of lanes sums the d_out rows of an equal share
+// 256 bins a pass, no comparison, pairs of int32 only), then every group of lanes sums the d_out rows of an equal share
 // of the SORTED tokens.  A run of equal indices inside one share goes straight to the table; a run that crosses
 // shares leaves its pieces in the workspace, and the share in which it begins adds them up afterwards.  No atomics: the
 // same bits every time, whatever the distribution.
@@ -19,7 +19,9 @@ namespace {
 
 constexpr int kSlab = 256;               // channels of a row that one warp covers
 constexpr int kSortWarps = 4;            // warps per CTA of the sorting kernels
-constexpr int kMaxDigitBits = 11;        // bins of one sorting pass: 2^11 counters of 4 bytes per warp
+// Bits of one sorting pass: 2^8 counters of 4 bytes per warp.  (More bits save passes and cost more than that in counters: 16384 tokens into
+// 1024 rows take 28 us with 8 bits, 41 with 11; into 100000 rows 39 against 73; with 5 bits 33 and 45.)
+constexpr int kMaxDigitBits = 8;
 constexpr uint32_t kNone = 0xffffffffu;  // key of a token without an embedding
 
 struct IndexView {
@@ -870,12 +872,12 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   const uint64_t tokens = static_cast<uint64_t>(d->tokens);
   p.slabs = (d->d + kSlab - 1) / kSlab;
   // Few tokens: looking through all indices once per table row (or, of a larger table, per token) and slab takes about 1.3 ns +
-  // 0.8 ps a token for each of them, the sort 17 to 40 us whatever its size.  Up to 4096 tokens, so that a row that takes most
-  // of them stays short too.  (128 channels, looking against sorting: 1024 tokens into 21 rows 4.3 against 18 us, 4096 into
-  // 2048 rows 15 against 39, 1024 into 16384 rows 11 by token against 38.)
+  // 0.8 ps a token for each of them, the sort 15 to 30 us whatever its size.  Up to 4096 tokens, so that a row that takes most
+  // of them stays short too.  (Looking against sorting: 128 channels, 1024 tokens into 100 rows 2.4 against 15 us, 4096 into
+  // 2048 rows 19 against 23, 2048 into 16384 rows 19 by token against 31; 512 channels, 4096 into 2048 rows 37 against 27.)
   // By token of tables with more rows than that, where clearing the table is worth its launch; a token's look costs about two rows'.
   p.by_token = static_cast<uint64_t>(d->rows) > tokens && static_cast<uint64_t>(d->rows) * p.slabs > 1024;
-  p.few = tokens <= 4096 && (p.by_token ? 2 * tokens : d->rows) * p.slabs * (tokens + 1600) <= (1u << 25);
+  p.few = tokens <= 4096 && (p.by_token ? 2 * tokens : d->rows) * p.slabs * (tokens + 1600) <= (1u << 24);
   // A small table takes longer by row than by a walk where most tokens share a row: 2304 tokens into 21 rows 23 us against 8.
   p.small = d->rows <= kTableRows && !(p.few && (tokens <= 1024 || tokens <= 64ull * d->rows));
   if (p.few && !p.small) {
