@@ -238,7 +238,9 @@ inline Shape shape_of(int unit, int d) {
 inline uint32_t grid_of(uint32_t rows, Shape w, int sms) {
   const uint32_t threads = threads_of(w.group), held = threads / w.group;
   const uint32_t need = (rows + held - 1) / held;
-  return walk_grid(need, sms, (w.channels == 16 ? 512 : 1024) / threads, held < 8 ? 256 / held : 32);
+  const uint32_t resident = (w.channels == 16 ? 512 : 1024) / threads, least = held < 8 ? 256 / held : 32;
+  const uint32_t eighth = need / (8 * static_cast<uint32_t>(sms) * resident);  // at most eight waves: one thread adds up every 64th CTA's sums
+  return walk_grid(need, sms, resident, least > eighth ? least : eighth);
 }
 
 template <typename T, int kU, int kGroup, int kUnits>
