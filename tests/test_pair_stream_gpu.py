@@ -404,6 +404,41 @@ def test_embedding_gradient_of_small_tables(n, rows, d, dtype, kind):
         assert torch.equal(got, again)
 
 
+@pytest.mark.parametrize("rows", [21, 66, 300, 70000])
+def test_embedding_gradient_captured_and_beside_another(rows):
+    """Each form of the gradient: two graphs replayed on new indices, one behind the other and on two streams."""
+    p, n, d = P(), 5000, 72
+    table, d_out = rand(rows, d, seed=1).requires_grad_(), rand(n, d, seed=2)
+    index = [indices("uniform", n, rows, torch.int64, seed=k) for k in range(2)]
+
+    def step(x):
+        return torch.autograd.grad(p.pair_embedding(x, table), table, d_out)[0]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(index[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in index], []
+    for graph, x in zip(graphs, index):
+        with torch.cuda.graph(graph):
+            outs.append(step(x))
+    for seed in (5, 9):
+        for k, x in enumerate(index):
+            x.copy_(indices("holes", n, rows, torch.int64, seed=seed + k))
+        want = [step(x) for x in index]
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for _ in range(3):
+            for graph, stream in zip(graphs, streams):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+        terms = embedding_grad(index[0], rows, d_out, 1.0)
+        near(outs[0], *terms, "replayed", 2.0 ** -13)
+
+
 def test_embedding_shapes_and_strides():
     p = P()
     table = rand(10, 48, seed=1, dtype=torch.bfloat16)
