@@ -10,7 +10,7 @@
 // fp32 pairs (and in packed 16-bit additions where there is no dropout).
 // Split.  A row of up to 256 channels is one oct (eight channels, 16 bytes of a 16-bit type) per lane of 8, 16 or 32 lanes, so
 // that the reductions stay inside a warp; up to 384 it is three octs of 16 lanes, up to 512 two of 32; wider rows take a CTA with
-// one oct per thread.  CTAs walk over the rows, eight rows a lane or one wave of CTAs (walk_grid); while one row of a lane is at hand
+// one oct per thread.  CTAs walk over the rows, 64 channels a lane or one wave of CTAs (walk_grid); while one row of a lane is at hand
 // the next is on its way through shared memory.
 // Measured (of the 6457 GB/s of a copy): 1024 x 1024 rows of 256 bf16 channels to e4m3 293 us, 100 % (333 with one wave of CTAs); the
 // addition alone with an elementwise dropout 267 us, 93 % (282); 512 x 512 fp32 rows of 256 169 us, 98 % (193); 384 x 384
@@ -21,7 +21,9 @@ namespace pair {
 namespace {
 
 constexpr float kE4m3Max = 448.f;
-constexpr uint32_t kSteps = 8;  // rows that a lane of the norm takes, where there are enough for several waves
+// Channels that a lane of the norm takes, where there are enough for several waves: eight rows of an oct, three of three octs.  (To e4m3, 96 x 768
+// rows of 384 take 37 us with two to four rows a lane and 40 with eight; 256 x 512 rows of 256 45 with three, 42 with eight.)
+constexpr uint32_t kLaneChannels = 64;
 
 enum Mode { kNorm = 0, kNormE4m3 = 1 };
 
@@ -386,7 +388,7 @@ cudaError_t launch_rows(const NormArgs<T>& a, int sms, cudaStream_t stream) {
   // what is resident without and with a residual's stages
   static const int resident[2] = {resident_ctas(kernel, kWide, kStages), resident_ctas(kernel, kWide, 2 * kStages)};
   const uint32_t need = (a.rows + kRows - 1) / kRows;
-  return pair::launch(kernel, walk_grid(need, sms, resident[has_residual], kSteps), kWide, smem, stream, a);
+  return pair::launch(kernel, walk_grid(need, sms, resident[has_residual], (kLaneChannels + kU * kUnits / 2) / (kU * kUnits)), kWide, smem, stream, a);
 }
 
 // Octs.
