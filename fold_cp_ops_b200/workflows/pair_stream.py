@@ -210,8 +210,9 @@ def add_rms_norm_fp8(update: Tensor, residual: Optional[Tensor], weight: Tensor,
     """``(q, scales, z)``: :func:`add_rms_norm` with ``y`` in ``float8_e4m3fn``, ``y ~ q * scales`` per ``group`` channels.
 
     ``group`` is 32, 64 or 128 (dividing ``D``), or ``None`` for one scale per row; ``scales`` is fp32,
-    ``(..., D / group)``: the group's largest ``|y|`` / 448, and 1 for a group of zeros.  ``y`` is scaled in fp32 and rounded
-    once, to e4m3.  For inference: refuses inputs that require gradients.  Scales per group need rows that start on 16-byte
+    ``(..., D / group)``: the group's largest ``|y|`` / 448, at least 2^-126, and 1 for a group of zeros.  ``q`` is the quotient
+    ``y / scale`` rounded once, ties to even: of 16-bit tensors with a 16-bit ``weight`` the exact quotient to within 2^-24 of it (a tie
+    stays a tie), of others to within a few 2^-24.  For inference: refuses inputs that require gradients.  Scales per group need rows that start on 16-byte
     boundaries; other inputs are copied first."""
     wrap = None
     if type(update) not in _PLAIN or type(residual) not in _PLAIN:

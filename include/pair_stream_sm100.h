@@ -78,7 +78,8 @@ typedef struct pair_norm_desc {
 /* z = round(residual + dropout(update)), y = z / sqrt(mean(z^2) + eps) * weight of the stored z.
  * residual.data may be NULL (z = dropout(update)); stream (contiguous) may be NULL when z is not wanted, and may be
  * the residual's or the update's own memory where that is contiguous; weight and y are both NULL for the addition alone.
- * scales: (b, i, j, d / group) fp32 for an e4m3 output: max|y| of the group / 448, 1 where that is 0. */
+ * scales: (b, i, j, d / group) fp32 for an e4m3 output: max|y| of the group / 448, at least 2^-126, 1 where that is 0;
+ * y is then the quotient y / scale rounded once, ties to even. */
 int pair_sm100_add_norm(const pair_norm_desc_t* desc, const pair_tensor_t* update, const pair_tensor_t* residual,
                         const void* weight, void* stream, void* y, float* scales, trimul_stream_t cuda_stream);
 
