@@ -421,7 +421,7 @@ struct SortArgs {
 // Tokens without an embedding sort behind all others: their key is the number of rows.
 __device__ __forceinline__ Entry entry_of(const SortArgs& a, uint32_t p) {
   if (a.in != nullptr) {
-    const uint2 e = __ldg(reinterpret_cast<const uint2*>(a.in) + p);
+    const uint2 e = __ldcg(reinterpret_cast<const uint2*>(a.in) + p);
     return Entry{e.x, e.y};
   }
   const uint32_t row = a.index.at(p);
@@ -615,8 +615,8 @@ __global__ void __launch_bounds__(kThreads, kSumCtas) sum_runs_kernel(const SumA
     Batch b;
     uint4 x = make_uint4(0, a.rows, 0, a.rows), y = x;
     if (q < a.share && lo + q < hi) {  // (behind the last token there is padding)
-      x = __ldg(reinterpret_cast<const uint4*>(a.sorted + lo + q));
-      y = __ldg(reinterpret_cast<const uint4*>(a.sorted + lo + q) + 1);
+      x = __ldcg(reinterpret_cast<const uint4*>(a.sorted + lo + q));
+      y = __ldcg(reinterpret_cast<const uint4*>(a.sorted + lo + q) + 1);
       if (hi - (lo + q) < kBatch) {
         y.w = a.rows;
         if (hi - (lo + q) < 3) y.y = a.rows;

@@ -477,6 +477,9 @@ __device__ __forceinline__ void group_max(float (&v)[kN], float* buf, int parity
 // Launches.  The kernels of one call follow one another: each but the last says at its start that the next may be set up while it
 // runs (next_may_start), and the next waits at its start for it to end, its results included (behind_previous).  That hides the
 // launch of all but the first.  The last says nothing: what follows the call sees an ordinary kernel.
+// A kernel that waits here may be running while the kernels before it still write, and a chain may write a buffer twice: what they write is
+// read by ordinary loads (or __ldcg) behind the wait, never by __ldg, which is for memory that nobody writes while the kernel lives
+// and which the compiler may move above the wait.
 __device__ __forceinline__ void next_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void behind_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
