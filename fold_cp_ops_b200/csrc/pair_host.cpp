@@ -6,11 +6,13 @@
 // without the interpreter.  A training step takes 55 to 80 us, some 45 of them the engine's own for a function that does nothing.  (The
 // same in Python: 14 us, and 90 to 130.)  The library's functions come as addresses from the loader, which has checked them against
 // the sources; nothing here links to it.
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <cmath>
@@ -165,6 +167,17 @@ pair_norm_desc_t norm_desc(const Tensor& x, const Tensor& weight, double eps, in
 // ---------------------------------------------------------------------------------------------
 // checks
 // ---------------------------------------------------------------------------------------------
+// The kernels run on memory and show themselves to no dispatcher: a tangent would be lost without a word, which reads as zero, and a trace would
+// keep the empty outputs and not what fills them.
+void check_visible(std::initializer_list<const Tensor*> tensors) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  if (torch::jit::tracer::isTracing() || (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value()))
+    refuse("the pair-stream operators cannot be traced");
+  for (const Tensor* t : tensors)
+    if (t->defined() && t->_fw_grad(0).defined()) refuse("the pair-stream operators have no forward-mode derivative; an input has a tangent");
+}
+
 void check_pair(const Tensor& update, const Tensor& residual) {
   if (!update.is_cuda()) refuse("update must be a CUDA tensor; the pair-stream kernels have no CPU path");
   if (kind_of(update.scalar_type()) < 0) refuse("update must be bfloat16, float16 or float32; got ", update.scalar_type());
@@ -399,6 +412,7 @@ struct PairEmbedding : torch::autograd::Function<PairEmbedding> {
 Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_, const std::string& drop,
                    const std::optional<Tensor>& seed, const std::optional<Tensor>& out_) {
   const Tensor residual = or_none(residual_), out = or_none(out_);
+  check_visible({&update, &residual, &out});
   check_pair(update, residual);
   if (out.defined()) {
     if (wants_grad({&update, &residual, &out})) refuse("out= has no gradient: leave it out, or run under torch.no_grad()");
@@ -417,6 +431,7 @@ Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_,
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optional<Tensor>& residual_, const Tensor& weight, double eps,
                                         const std::string& drop, const std::optional<Tensor>& seed) {
   const Tensor residual = or_none(residual_);
+  check_visible({&update, &residual, &weight});
   check_pair(update, residual);
   check_weight(weight, update, eps);
   if (wants_grad({&update, &residual, &weight})) {
@@ -442,6 +457,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& update_, const
                                                     double eps, const std::optional<int64_t>& group, const std::string& drop,
                                                     const std::optional<Tensor>& seed) {
   Tensor update = update_, residual = or_none(residual_);
+  check_visible({&update, &residual, &weight});
   check_pair(update, residual);
   check_weight(weight, update, eps);
   const int64_t width = update.size(-1);
@@ -460,6 +476,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& update_, const
 Tensor pair_embedding(const Tensor& index, const Tensor& table, double scale, const std::optional<Tensor>& base_,
                       const std::optional<at::ScalarType>& dtype_) {
   const Tensor base = or_none(base_);
+  check_visible({&table, &base});
   if (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong)
     refuse("index must be an int32 or int64 tensor; got ", index.scalar_type());
   if (!index.is_cuda()) refuse("index must be a CUDA tensor; the pair-stream kernels have no CPU path");

@@ -8,7 +8,7 @@ operators) computes an update of it; the functions here are the rest of the stre
 * :func:`add_rms_norm_fp8` -- the same with the norm in e4m3 and fp32 scales, for an 8-bit product;
 * :func:`pair_embedding` -- ``base + scale * table[index]``: position or distance bins, residue types.
 
-All but the e4m3 form have gradients (once).  Statistics and sums are fp32 or wider whatever the tensors'
+All but the e4m3 form have gradients (once; backwards only: inputs with forward-mode tangents, and calls under a tracer, are refused).  Statistics and sums are fp32 or wider whatever the tensors'
 type; ``z`` is rounded once, to the activations' type, and the norm reads ``z`` as it is stored.
 
 Dropout (:class:`PairDropout`) stores no mask: element ``(b, i, j, c)`` of the WHOLE grid is kept by a counter-based

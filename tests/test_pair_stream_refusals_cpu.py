@@ -1,0 +1,45 @@
+"""Calls that the pair-stream operators must not answer, refused before they look for a device."""
+import pytest
+import torch
+
+from fold_cp_ops_b200.workflows import pair_stream as P
+
+X, W = torch.zeros(2, 3, 4, 32), torch.ones(32)
+INDEX = torch.zeros(3, dtype=torch.int64)
+#: every call with one of its tensors replaced
+CALLS = {
+    "dropout_add update": lambda t: P.dropout_add(t(X), X),
+    "dropout_add residual": lambda t: P.dropout_add(X, t(X), P.PairDropout(0.5)),
+    "dropout_add out": lambda t: P.dropout_add(X, X, out=t(X)),
+    "add_rms_norm update": lambda t: P.add_rms_norm(t(X), None, W),
+    "add_rms_norm residual": lambda t: P.add_rms_norm(X, t(X), W),
+    "add_rms_norm weight": lambda t: P.add_rms_norm(X, X, t(W)),
+    "add_rms_norm_fp8 update": lambda t: P.add_rms_norm_fp8(t(X), None, W, group=32),
+    "add_rms_norm_fp8 residual": lambda t: P.add_rms_norm_fp8(X, t(X), W, group=32),
+    "add_rms_norm_fp8 weight": lambda t: P.add_rms_norm_fp8(X, X, t(W), group=32),
+    "pair_embedding table": lambda t: P.pair_embedding(INDEX, t(W[None])),
+    "pair_embedding base": lambda t: P.pair_embedding(INDEX, W[None], base=t(X[0, :, 0])),
+}
+
+
+@pytest.mark.parametrize("requires_grad", [False, True])
+@pytest.mark.parametrize("call", CALLS)
+def test_tangents_are_refused(call, requires_grad):
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        with pytest.raises(ValueError, match="forward-mode"):
+            CALLS[call](lambda t: forward_ad.make_dual(t.clone().requires_grad_(requires_grad), torch.ones_like(t)))
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            CALLS[call](lambda t: forward_ad.make_dual(t.clone(), torch.ones_like(t)))
+
+
+@pytest.mark.parametrize("call", ["dropout_add update", "add_rms_norm update", "add_rms_norm_fp8 update", "pair_embedding table"])
+def test_tracers_are_refused(call):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    x = W[None] if "table" in call else X
+    with pytest.raises(ValueError, match="cannot be traced"):
+        torch.jit.trace(lambda a: CALLS[call](lambda t: a), x)
+    with pytest.raises(ValueError, match="cannot be traced"):
+        make_fx(lambda a: CALLS[call](lambda t: a))(x)
