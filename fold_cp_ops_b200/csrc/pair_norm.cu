@@ -478,7 +478,7 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* update, const pa
   a.weight_dtype = d->weight_dtype;
   a.scales_per_row = d->group != 0 ? d->d / d->group : 0;
   a.scale_shift = d->group == d->d ? -1 : d->group == 32 ? 2 : d->group == 64 ? 3 : 4;
-  a.flat = collapses(update, d->b, d->i, d->j) && collapses(residual, d->b, d->i, d->j);
+  a.flat = collapses(update, d->i, d->j) && collapses(residual, d->i, d->j);
   a.eps = d->eps;
   a.inv_d = 1.f / static_cast<float>(d->d);
   if (y == nullptr) return launch_add<T>(a, unit, sms, s);
@@ -541,6 +541,8 @@ extern "C" int pair_sm100_add_norm(const pair_norm_desc_t* desc, const pair_tens
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: an e4m3 output needs y and scales", who);
   if (update == nullptr || update->data == nullptr)
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: update is NULL", who);
+  const pair_tensor_t u = canonical(update, desc->b, desc->i, desc->j), r = canonical(residual, desc->b, desc->i, desc->j);
+  update = &u, residual = &r;
   const int size = type_bytes(desc->dtype);
   if (!elements_aligned(size, {update, residual}, {stream, g == 0 ? y : nullptr}) || !aligned(scales, 4) ||
       !aligned(weight, type_bytes(desc->weight_dtype)) || !aligned(desc->dropout.device_seed, 8))

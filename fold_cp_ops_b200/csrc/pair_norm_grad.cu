@@ -297,7 +297,7 @@ cudaError_t run(const pair_norm_desc_t* d, const pair_tensor_t* z, const pair_te
   a.d = d->d;
   a.octs = (d->d + 7) / 8;
   a.weight_dtype = d->weight_dtype;
-  a.flat = collapses(z, d->b, d->i, d->j) && collapses(dy, d->b, d->i, d->j) && collapses(dz, d->b, d->i, d->j);
+  a.flat = collapses(z, d->i, d->j) && collapses(dy, d->i, d->j) && collapses(dz, d->i, d->j);
   a.eps = d->eps;
   a.inv_d = 1.f / static_cast<float>(d->d);
   const int unit = unit_of(d->d, sizeof(T), {z, dy, dz}, {d_stream, d_update});
@@ -358,6 +358,9 @@ extern "C" int pair_sm100_add_norm_grad(const pair_norm_desc_t* desc, const pair
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: stream is NULL", who);
   if (d_weight != nullptr && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 7) != 0))
     return report_error(TRIMUL_ERR_INVALID_ARGUMENT, "%s: the weight's gradient needs an 8-byte aligned workspace", who);
+  const pair_tensor_t z = canonical(stream, desc->b, desc->i, desc->j), y = canonical(dy, desc->b, desc->i, desc->j),
+                      g = canonical(dz, desc->b, desc->i, desc->j);
+  stream = &z, dy = &y, dz = &g;
   const int weight_size = type_bytes(desc->weight_dtype);
   if (!elements_aligned(type_bytes(desc->dtype), {stream, dy, dz}, {d_stream, d_update}) || !aligned(weight, weight_size) ||
       !aligned(d_weight, weight_size) || !aligned(desc->dropout.device_seed, 8))

@@ -283,10 +283,20 @@ inline Strided<T> strided(const pair_tensor_t* t) {
   return Strided<T>{static_cast<const T*>(t->data), t->stride_b, t->stride_i, t->stride_j};
 }
 
-// Whether row * stride_j reaches every row.
-inline bool collapses(const pair_tensor_t* t, int bb, int ii, int jj) {
-  if (t == nullptr || t->data == nullptr) return true;
-  return (ii == 1 || t->stride_i == t->stride_j * jj) && (bb == 1 || t->stride_b == t->stride_j * jj * ii);
+// A tensor as the kernels and the rules below take it.  An axis of one entry is never stepped along, and what its stride holds (a slice
+// keeps that of the whole tensor) says nothing about alignment: it becomes the stride that lets rows lie one behind another.
+inline pair_tensor_t canonical(const pair_tensor_t* t, int bb, int ii, int jj) {
+  if (t == nullptr || t->data == nullptr) return pair_tensor_t{nullptr, 0, 0, 0};
+  pair_tensor_t c = *t;
+  if (jj == 1) c.stride_j = ii != 1 ? c.stride_i : bb != 1 ? c.stride_b : 0;
+  if (ii == 1) c.stride_i = c.stride_j * jj;
+  if (bb == 1) c.stride_b = c.stride_i * ii;
+  return c;
+}
+
+// Whether row * stride_j reaches every row of a canonical tensor.
+inline bool collapses(const pair_tensor_t* t, int ii, int jj) {
+  return t->data == nullptr || (t->stride_i == t->stride_j * jj && t->stride_b == t->stride_i * ii);
 }
 
 // ---------------------------------------------------------------------------------------------
