@@ -167,16 +167,23 @@ pair_norm_desc_t norm_desc(const Tensor& x, const Tensor& weight, double eps, in
 // ---------------------------------------------------------------------------------------------
 // checks
 // ---------------------------------------------------------------------------------------------
-// The kernels run on memory and show themselves to no dispatcher: a tangent would be lost without a word, which reads as zero, and a trace would
+// The kernels run on memory and show themselves to no dispatcher: a wrapper's memory is not found, a tangent would be lost without a word, which reads as zero, and a trace would
 // keep the empty outputs and not what fills them.
 void check_visible(std::initializer_list<const Tensor*> tensors) {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
   if (torch::jit::tracer::isTracing() || (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value()))
     refuse("the pair-stream operators cannot be traced");
-  for (const Tensor* t : tensors)
-    if (t->defined() && t->_fw_grad(0).defined()) refuse("the pair-stream operators have no forward-mode derivative; an input has a tangent");
+  for (const Tensor* t : tensors) {
+    if (!t->defined()) continue;
+    if (t->_fw_grad(0).defined()) refuse("the pair-stream operators have no forward-mode derivative; an input has a tangent");
+    // subclasses that only wrap another tensor; to the library a null pointer is an absent tensor
+    if (t->numel() > 0 && t->const_data_ptr() == nullptr) refuse("the pair-stream operators need tensors with memory of their own; got one without");
+  }
 }
+
+const Tensor kAbsent;
+const Tensor* seed_of(const std::optional<Tensor>& seed) { return seed.has_value() ? &*seed : &kAbsent; }
 
 void check_pair(const Tensor& update, const Tensor& residual) {
   if (!update.is_cuda()) refuse("update must be a CUDA tensor; the pair-stream kernels have no CPU path");
@@ -412,7 +419,7 @@ struct PairEmbedding : torch::autograd::Function<PairEmbedding> {
 Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_, const std::string& drop,
                    const std::optional<Tensor>& seed, const std::optional<Tensor>& out_) {
   const Tensor residual = or_none(residual_), out = or_none(out_);
-  check_visible({&update, &residual, &out});
+  check_visible({&update, &residual, &out, seed_of(seed)});
   check_pair(update, residual);
   if (out.defined()) {
     if (wants_grad({&update, &residual, &out})) refuse("out= has no gradient: leave it out, or run under torch.no_grad()");
@@ -431,7 +438,7 @@ Tensor dropout_add(const Tensor& update, const std::optional<Tensor>& residual_,
 std::tuple<Tensor, Tensor> add_rms_norm(const Tensor& update, const std::optional<Tensor>& residual_, const Tensor& weight, double eps,
                                         const std::string& drop, const std::optional<Tensor>& seed) {
   const Tensor residual = or_none(residual_);
-  check_visible({&update, &residual, &weight});
+  check_visible({&update, &residual, &weight, seed_of(seed)});
   check_pair(update, residual);
   check_weight(weight, update, eps);
   if (wants_grad({&update, &residual, &weight})) {
@@ -457,7 +464,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& update_, const
                                                     double eps, const std::optional<int64_t>& group, const std::string& drop,
                                                     const std::optional<Tensor>& seed) {
   Tensor update = update_, residual = or_none(residual_);
-  check_visible({&update, &residual, &weight});
+  check_visible({&update, &residual, &weight, seed_of(seed)});
   check_pair(update, residual);
   check_weight(weight, update, eps);
   const int64_t width = update.size(-1);
@@ -476,7 +483,7 @@ std::tuple<Tensor, Tensor, Tensor> add_rms_norm_fp8(const Tensor& update_, const
 Tensor pair_embedding(const Tensor& index, const Tensor& table, double scale, const std::optional<Tensor>& base_,
                       const std::optional<at::ScalarType>& dtype_) {
   const Tensor base = or_none(base_);
-  check_visible({&table, &base});
+  check_visible({&index, &table, &base});
   if (index.scalar_type() != at::kInt && index.scalar_type() != at::kLong)
     refuse("index must be an int32 or int64 tensor; got ", index.scalar_type());
   if (!index.is_cuda()) refuse("index must be a CUDA tensor; the pair-stream kernels have no CPU path");

@@ -116,6 +116,12 @@ def pair_block_origin(x) -> Tuple[int, int, int]:
 # ---------------------------------------------------------------------------------------------
 # DTensors
 # ---------------------------------------------------------------------------------------------
+def _local(t) -> Tensor:
+    """This rank's block, waited for where the collective that makes it is still under way."""
+    local = t.to_local()
+    return local.trigger_wait() if hasattr(local, "trigger_wait") else local
+
+
 def _locals_of(names: Sequence[str], tensors: Sequence[Optional[Tensor]]):
     """The ranks' local blocks of DTensors that are sharded alike, and their :class:`_Wrap` (``None`` where all are plain)."""
     given = [(n, t) for n, t in zip(names, tensors) if t is not None]
@@ -137,7 +143,7 @@ def _locals_of(names: Sequence[str], tensors: Sequence[Optional[Tensor]]):
         raise ValueError(f"the channels must be whole on every rank, but {placements} shard them")
     if any(p.is_partial() for p in placements):
         raise ValueError(f"{first} holds partial sums ({placements}): reduce it first")
-    return [None if t is None else t.to_local() for t in tensors], _Wrap(mesh, placements, x, tokens)
+    return [None if t is None else _local(t) for t in tensors], _Wrap(mesh, placements, x, tokens)
 
 
 class _Wrap:
@@ -161,7 +167,7 @@ def _whole(t, name: str):
         raise ValueError(f"{name} must be whole on every rank; got placements {_dtensor_mesh_placements(t)[1]}")
     if torch.is_grad_enabled() and t.requires_grad:
         raise ValueError(_NO_DTENSOR_GRADIENT)
-    return t.to_local()
+    return _local(t)
 
 
 def _no_gradient(wrap: Optional[_Wrap], *parameters: Tensor) -> None:

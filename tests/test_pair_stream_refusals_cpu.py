@@ -43,3 +43,30 @@ def test_tracers_are_refused(call):
         torch.jit.trace(lambda a: CALLS[call](lambda t: a), x)
     with pytest.raises(ValueError, match="cannot be traced"):
         make_fx(lambda a: CALLS[call](lambda t: a))(x)
+
+
+class Wrapper(torch.Tensor):
+    """A subclass that holds another tensor and has no memory itself."""
+
+    @staticmethod
+    def __new__(cls, elem):
+        out = torch.Tensor._make_wrapper_subclass(cls, elem.shape, dtype=elem.dtype, device=elem.device)
+        out.elem = elem
+        return out
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        args = [a.elem if isinstance(a, cls) else a for a in args]
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("call", CALLS)
+def test_tensors_without_memory_are_refused(call):
+    """The library takes a null pointer for an absent tensor: a wrapped residual would be left out without a word."""
+    with pytest.raises(ValueError, match="memory of their own"):
+        CALLS[call](Wrapper)
+
+
+def test_an_index_without_memory_is_refused():
+    with pytest.raises(ValueError, match="memory of their own"):
+        P.pair_embedding(Wrapper(INDEX), W[None])
