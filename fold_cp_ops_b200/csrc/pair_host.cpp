@@ -502,7 +502,7 @@ Tensor pair_embedding(const Tensor& index, const Tensor& table, double scale, co
   }
   const at::ScalarType dtype = base.defined() ? base.scalar_type() : dtype_.value_or(table.scalar_type());
   if (kind_of(dtype) < 0) refuse("the embedding's type must be bfloat16, float16 or float32; got ", dtype);
-  if (!std::isfinite(scale)) refuse("scale must be finite; got ", scale);
+  if (!std::isfinite(static_cast<float>(scale))) refuse("scale must be finite in float32; got ", scale);
   if (wants_grad({&table, &base})) {
     check_capture({&table, &base});
     return PairEmbedding::apply(index, table, base_, scale, static_cast<int64_t>(dtype));
