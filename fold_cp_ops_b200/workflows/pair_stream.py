@@ -24,6 +24,7 @@ There is no CPU path.
 from __future__ import annotations
 
 import math
+import operator
 import struct
 from dataclasses import dataclass
 from typing import Optional, Sequence, Tuple, Union
@@ -44,6 +45,13 @@ _NO_DTENSOR_GRADIENT = "gradients through DTensors are not supported: pass the l
 #: a ``pair_dropout_t`` of include/pair_stream_sm100.h: seed, offset, keep, (device seed), shared, origin b, i, j
 _pack_dropout = struct.Struct("@QIIP4i").pack
 _NO_DROPOUT = (b"", None)
+
+
+def _fits(value, bits: int) -> bool:
+    try:
+        return 0 <= operator.index(value) < 1 << bits
+    except TypeError:
+        return False
 
 
 @dataclass(frozen=True)
@@ -72,12 +80,12 @@ class PairDropout:
         if isinstance(self.seed, Tensor):
             if self.seed.dtype is not torch.int64 or self.seed.numel() != 2 or not self.seed.is_cuda or not self.seed.is_contiguous():
                 raise ValueError("seed must be an int or a contiguous int64 CUDA tensor of two values [seed, offset]")
-        elif not 0 <= self.seed < 1 << 64:
-            raise ValueError(f"seed must fit 64 bits unsigned; got {self.seed}")
-        if not 0 <= self.offset < 1 << 32:
-            raise ValueError(f"offset must fit 32 bits unsigned; got {self.offset}")
-        if len(self.origin) != 3 or not all(0 <= o < 1 << 31 for o in self.origin):
-            raise ValueError(f"origin must be three coordinates (b, i, j) >= 0; got {self.origin}")
+        elif not _fits(self.seed, 64):
+            raise ValueError(f"seed must be an integer of 64 bits, unsigned; got {self.seed!r}")
+        if not _fits(self.offset, 32):
+            raise ValueError(f"offset must be an integer of 32 bits, unsigned; got {self.offset!r}")
+        if len(self.origin) != 3 or not all(_fits(o, 31) for o in self.origin):
+            raise ValueError(f"origin must be three integers (b, i, j), >= 0 and below 2^31; got {self.origin!r}")
 
     @property
     def keep(self) -> int:
@@ -98,6 +106,8 @@ def _record(dropout: Optional[PairDropout], wrap: Optional["_Wrap"]) -> Tuple[by
     origin = dropout.origin
     if wrap is not None:
         origin = tuple(o + at for o, at in zip(origin, pair_block_origin(wrap.like)))
+        if not all(_fits(o, 31) for o in origin):
+            raise ValueError(f"the dropout's origin {dropout.origin} puts this block at {origin}, behind 2^31 - 1")
     seed, offset, device_seed = dropout.seed, dropout.offset, None
     if isinstance(seed, Tensor):
         seed, offset, device_seed = 0, 0, seed

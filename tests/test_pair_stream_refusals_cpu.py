@@ -70,3 +70,28 @@ def test_tensors_without_memory_are_refused(call):
 def test_an_index_without_memory_is_refused():
     with pytest.raises(ValueError, match="memory of their own"):
         P.pair_embedding(Wrapper(INDEX), W[None])
+
+
+@pytest.mark.parametrize("kw", [dict(seed=3.0), dict(seed="3"), dict(seed=None), dict(offset=1.5), dict(origin=(0, 0.0, 0)), dict(origin=(0, 0, None)),
+                                dict(origin=(0, 0, 1 << 31))])
+def test_dropouts_that_are_no_integers_are_refused_where_they_are_made(kw):
+    with pytest.raises(ValueError, match="integer"):
+        P.PairDropout(0.5, **kw)
+
+
+def test_integers_of_other_kinds_are_taken():
+    import numpy as np
+
+    plain = P._record(P.PairDropout(0.5, seed=7, offset=2, origin=(1, 2, 3)), None)
+    other = P.PairDropout(0.5, seed=np.uint64(7), offset=np.int32(2), origin=tuple(torch.tensor([1, 2, 3])))
+    assert P._record(other, None) == plain
+
+
+def test_a_block_behind_the_last_coordinate_is_refused(monkeypatch):
+    class Wrap:
+        like = None
+
+    monkeypatch.setattr(P, "pair_block_origin", lambda x: (0, 1 << 30, 0))
+    assert P._record(P.PairDropout(0.5, origin=(0, (1 << 30) - 1, 0)), Wrap())
+    with pytest.raises(ValueError, match="behind"):
+        P._record(P.PairDropout(0.5, origin=(0, 1 << 30, 0)), Wrap())
