@@ -256,6 +256,7 @@ __global__ void __launch_bounds__(1024) embed_grad_few_kernel(IndexView index, c
 // against 63, 21 rows 39 and 45 against 60; 64 x 64 positions into 21 rows 8 against 15.  110 rows (eight warps' tables): 67 against 63.
 // (Four channels per lane take as long: 47 and 60 us.)
 constexpr int kTableSlab = 64, kTableWarps = 16, kTableRows = 74;
+constexpr int kTableSmem = 227 * 1024;
 constexpr uint32_t kTableShare = 1024;  // most tokens of a warp: the terms of an fp32 sum
 
 template <int kBytes>
@@ -886,7 +887,7 @@ Plan make_plan(const pair_embed_desc_t* d, int sms) {
   }
   p.few = false;
   if (p.small) {
-    p.warps = 227 * 1024 / ((d->rows + 1) * kTableSlab * 4);
+    p.warps = kTableSmem / ((d->rows + 1) * kTableSlab * 4);
     if (p.warps > kTableWarps) p.warps = kTableWarps;
     const int slabs = (d->d + kTableSlab - 1) / kTableSlab;
     const uint64_t ctas = sms > slabs ? sms / slabs : 1;  // one CTA an SM
@@ -977,7 +978,8 @@ cudaError_t grad_run(const pair_embed_desc_t* d, const IndexView& index, const v
     const bool pairs = d->d % 2 == 0 && aligned(d_out, 2 * sizeof(T));
     auto kernel = pairs ? embed_grad_table_kernel<T, 2> : embed_grad_table_kernel<T, 1>;
     const int smem = p.warps * (d->rows + 1) * kTableSlab * 4;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    // all that any table takes: the attribute is the kernel's, and another thread's smaller table must not lower it before this launch
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTableSmem);
     if (e == cudaSuccess) e = launch(kernel, dim3(p.parts, (d->d + kTableSlab - 1) / kTableSlab), p.warps * 32, smem, s, a);
     if (e != cudaSuccess) return e;
     const int64_t size = static_cast<int64_t>(d->rows) * d->d;
