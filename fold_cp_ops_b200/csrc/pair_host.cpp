@@ -152,9 +152,10 @@ Dropping dropping(const std::string& bytes, const Tensor& seed, const Tensor& li
 pair_norm_desc_t norm_desc(const Tensor& x, const Tensor& weight, double eps, int group, const Dropping& drop) {
   const int64_t n = x.dim();
   pair_norm_desc_t d;
-  d.b = n >= 4 ? static_cast<int32_t>(x.size(n - 4)) : 1;
-  d.i = n >= 3 ? static_cast<int32_t>(x.size(n - 3)) : 1;
-  d.j = n >= 2 ? static_cast<int32_t>(x.size(n - 2)) : 1;
+  const bool empty = x.numel() == 0;  // its other axes may be of any length
+  d.b = empty ? 0 : n >= 4 ? static_cast<int32_t>(x.size(n - 4)) : 1;
+  d.i = empty ? 0 : n >= 3 ? static_cast<int32_t>(x.size(n - 3)) : 1;
+  d.j = empty ? 0 : n >= 2 ? static_cast<int32_t>(x.size(n - 2)) : 1;
   d.d = static_cast<int32_t>(x.size(n - 1));
   d.dtype = kind_of(x.scalar_type());
   d.weight_dtype = weight.defined() ? kind_of(weight.scalar_type()) : d.dtype;
