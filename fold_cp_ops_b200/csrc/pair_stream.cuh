@@ -245,7 +245,7 @@ __device__ __forceinline__ Lane<kU, kUnits> load_gain(const void* weight, int dt
 // 0 <= n < 2^31.
 struct FastDiv {
   uint32_t m, shift, d;
-  __device__ __forceinline__ uint32_t div(uint32_t n) const {
+  __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
     return static_cast<uint32_t>((static_cast<uint64_t>(n) * m) >> shift);
   }
 };
