@@ -225,6 +225,7 @@ void check_overlap(const Tensor& out, const Tensor& t, const char* name) {
 // accumulators belong to.  An accumulator lives as long as any graph that uses the leaf: one that an eager graph on another
 // stream still holds would break the capture from inside the engine, so the call is refused while nothing is lost.
 void check_capture(std::initializer_list<const Tensor*> tensors) {
+  const c10::cuda::OptionalCUDAGuard guard((*tensors.begin())->device());  // all are on one device, which need not be the current one
   if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
   for (const Tensor* t : tensors) {
     if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
