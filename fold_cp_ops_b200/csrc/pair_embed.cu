@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads) embed_octs_kernel(const EmbedArgs a,
     if (row != kNone) {
       const Lane<8, 1> x = table_oct(a.table, a.table_dtype, static_cast<int64_t>(row) * a.d + v * 8);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) f.p[e] = __ffma2_rn(x.p[e], both(a.scale), f.p[e]);
+      for (int e = 0; e < 4; ++e) f.p[e] = fma_whole(x.p[e], both(a.scale), f.p[e]);
     }
     store_unit<T, 8>(static_cast<T*>(a.out) + n * 8, pack<T>(f));
   }
@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(kThreads) embed_pieces_kernel(const EmbedArgs 
 #pragma unroll
       for (int k = 0; k < 8; ++k) f[k] = k * 32 < left ? to_f32(table[from + k * 32]) : 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) b[k].e[0] = from_f32<T>(f[k] * a.scale + to_f32(b[k].e[0]));
+      for (int k = 0; k < 8; ++k) b[k].e[0] = from_f32<T>(fma_whole(f[k], a.scale, to_f32(b[k].e[0])));
     };
     if (row != kNone) {
       if (a.table_dtype == PAIR_FP32)

@@ -91,7 +91,7 @@ __device__ __forceinline__ Unit<T, 8> drop_and_add(const Dropout& d, uint32_t li
   if (has_residual) {
     const Lane<8, 1> x = unpack(r);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v.p[e] = __fadd2_rn(v.p[e], x.p[e]);
+    for (int e = 0; e < 4; ++e) v.p[e] = add_whole(v.p[e], x.p[e]);
   }
   return pack<T>(v);
 }
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
         drop_all<kU, kGroup, kUnits>(drop, line, b, i, j, lane, a.octs, v);
         const Lane<kU, kUnits> x = unpack_all<T, kU, kUnits>(r);
 #pragma unroll
-        for (int n = 0; n < kPairs; ++n) v.p[n] = __fadd2_rn(v.p[n], x.p[n]);
+        for (int n = 0; n < kPairs; ++n) v.p[n] = add_whole(v.p[n], x.p[n]);
         pack_all<T, kU, kUnits>(v, u);
       }
     } else if (has_residual) {
@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) add_pieces_kernel(const __grid_const
       drop_all<kU, 32, kUnits>(drop, line, b, i, j, piece * (256 / kU) + lane, a.octs, v);
       const Lane<kU, kUnits> x = unpack_all<T, kU, kUnits>(r);
 #pragma unroll
-      for (int k = 0; k < v.kPairs; ++k) v.p[k] = __fadd2_rn(v.p[k], x.p[k]);
+      for (int k = 0; k < v.kPairs; ++k) v.p[k] = add_whole(v.p[k], x.p[k]);
       pack_all<T, kU, kUnits>(v, u);
     } else if (has_residual) {
 #pragma unroll

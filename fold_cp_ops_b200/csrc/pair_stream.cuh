@@ -185,6 +185,45 @@ __device__ __forceinline__ Unit<T, 8> pack(const Lane<8, 1>& v) {
   return u[0];
 }
 
+// The library is built to flush fp32 subnormals.  What becomes the stream (sums, kept elements, embeddings) keeps them, in packed
+// pairs like the rest; what is computed from it (statistics, norms, gradients' sums) does not.
+__device__ __forceinline__ float2 add_whole(float2 a, float2 b) {
+  float2 r;
+  asm("add.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 mul_whole(float2 a, float2 b) {
+  float2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)));
+  return r;
+}
+__device__ __forceinline__ float2 fma_whole(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;"
+      : "=l"(reinterpret_cast<uint64_t&>(r))
+      : "l"(reinterpret_cast<const uint64_t&>(a)), "l"(reinterpret_cast<const uint64_t&>(b)), "l"(reinterpret_cast<const uint64_t&>(c)));
+  return r;
+}
+__device__ __forceinline__ float add_whole(float a, float b) {
+  float r;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float mul_whole(float a, float b) {
+  float r;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float fma_whole(float a, float b, float c) {
+  float r;
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // a + b in the unit's type, rounded once: for 16-bit pairs the packed addition, which rounds the exact sum.
 template <typename T, int kU>
 __device__ __forceinline__ Unit<T, kU> add_units(const Unit<T, kU>& a, const Unit<T, kU>& b) {
@@ -200,7 +239,7 @@ __device__ __forceinline__ Unit<T, kU> add_units(const Unit<T, kU>& a, const Uni
     }
   } else {
 #pragma unroll
-    for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(to_f32(a.e[k]) + to_f32(b.e[k]));
+    for (int k = 0; k < kU; ++k) o.e[k] = from_f32<T>(add_whole(to_f32(a.e[k]), to_f32(b.e[k])));
   }
   return o;
 }
@@ -369,7 +408,7 @@ __device__ __forceinline__ void drop_oct(const uint4 r, uint32_t line, float gai
   for (int k = 0; k < 4; ++k) {
     p[k].x = (w[k] << 16) < line ? p[k].x : 0.f;
     p[k].y = w[k] < line ? p[k].y : 0.f;
-    p[k] = __fmul2_rn(p[k], both(gain));
+    p[k] = mul_whole(p[k], both(gain));
   }
 }
 
@@ -432,8 +471,8 @@ __device__ __forceinline__ void drop_all(const Dropout& d, uint32_t line, uint32
     for (int n = 0; n < v.kPairs; ++n) {
       const uint32_t x = narrow_bits<kU, kUnits>(mask, 2 * n / kU) >> (2 * n % kU);
       const uint32_t y = kU > 1 ? x >> 1 : narrow_bits<kU, kUnits>(mask, 2 * n + 1);
-      v.p[n].x = x & 1u ? v.p[n].x * d.gain : 0.f;
-      v.p[n].y = y & 1u ? v.p[n].y * d.gain : 0.f;
+      v.p[n].x = x & 1u ? mul_whole(v.p[n].x, d.gain) : 0.f;
+      v.p[n].y = y & 1u ? mul_whole(v.p[n].y, d.gain) : 0.f;
     }
   }
 }

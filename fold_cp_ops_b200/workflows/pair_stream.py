@@ -9,7 +9,7 @@ operators) computes an update of it; the functions here are the rest of the stre
 * :func:`pair_embedding` -- ``base + scale * table[index]``: position or distance bins, residue types.
 
 All but the e4m3 form have gradients (once; backwards only: inputs with forward-mode tangents, and calls under a tracer, are refused).  Statistics and sums are fp32 or wider whatever the tensors'
-type; ``z`` is rounded once, to the activations' type, and the norm reads ``z`` as it is stored.
+type, and there values below 2^-126 count as 0; ``z`` is rounded once, to the activations' type and its subnormals, and the norm reads ``z`` as it is stored.
 
 Dropout (:class:`PairDropout`) stores no mask: element ``(b, i, j, c)`` of the WHOLE grid is kept by a counter-based
 generator of exactly that position, so the gradient draws the mask again, and ranks that hold different blocks of a

@@ -32,3 +32,23 @@ def test_empty_tensors_with_long_axes(shape):
     assert g.shape == shape and torch.equal(gw, torch.zeros_like(w))
     q, scales, z = p.add_rms_norm_fp8(x.detach(), None, w.detach(), group=None)
     assert q.shape == shape and scales.shape == (*shape[:3], 1) and z.shape == shape
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 66, 67, 68])
+def test_the_addition_keeps_subnormals(d, dtype):
+    """Multiples of the smallest subnormal add up, and double where half of them are kept, without rounding."""
+    p = P()
+    step = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24, torch.float32: 2.0 ** -149}[dtype]
+    u, r = ((torch.randint(-40, 41, (1, 3, 5, d), device=DEV).double() * step).to(dtype) for _ in range(2))
+    assert torch.equal(p.dropout_add(u, r), (u.double() + r.double()).to(dtype)) and (u != 0).any()
+    drop = p.PairDropout(0.5, seed=3)
+    kept = p.dropout_add(torch.ones_like(u), None, drop) != 0
+    want = torch.where(kept, u.double() * 2, 0.0)
+    assert torch.equal(p.dropout_add(u, None, drop), want.to(dtype))
+    assert torch.equal(p.dropout_add(u, r, drop), (want + r.double()).to(dtype))
+    w = torch.ones(d, device=DEV)
+    assert torch.equal(p.add_rms_norm(u, r, w, dropout=drop)[1], (want + r.double()).to(dtype))
+    table, index = u[0, :, 0].contiguous(), torch.tensor([2, -1, 0, 1, 2], device=DEV)
+    want = torch.where((index >= 0)[:, None], table.double()[index.clamp(min=0)], 0.0) * 2 + r[0, 0].double()
+    assert torch.equal(p.pair_embedding(index, table, scale=2.0, base=r[0, 0]), want.to(dtype))
