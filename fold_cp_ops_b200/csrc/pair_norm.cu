@@ -51,9 +51,24 @@ __device__ __forceinline__ uint32_t e4m3x2(float2 v) {
   return r;
 }
 
-// The e4m3 output.  With s = 2^k rest (1/2 <= rest < 1: p is not flushed before y is) the channels become p = (z 2^k) w, exact for 16-bit
-// z and w, and y = p rest; so scale = max|p| rest / 448 and y / scale = p (448 / max|p|), from which rest has gone.  Random bf16
-// rows have one quotient in some 2500 that lies exactly between two e4m3 values, and roundings before it would send it to either side.
+// The e4m3 output.  With p = z w, exact for 16-bit z and w, y = p s; so scale = max|p| s / 448 and y / scale = p (448 / max|p|), from
+// which s has gone.  Random bf16 rows have one quotient in some 2500 that lies exactly between two e4m3 values, and roundings
+// before it would send it to either side.  448 / max|p| is held as the sum of an approximation and of what a fused product shows it to lack, good to
+// 2^-44: a quotient that fp32 holds, as every tie is, then comes out exactly, every other within 2^-24 of it.  (1024 x 1024 rows of 256
+// take 324 us, 321 with a product by an approximate 1 / scale, which misses ties, and 365 with divisions.)
+struct Quotient {
+  float scale, factor, lack;
+  __device__ __forceinline__ float2 operator()(float2 p) const { return __ffma2_rn(p, both(factor), __fmul2_rn(p, both(lack))); }
+};
+__device__ __forceinline__ Quotient quotient_near(float top, float rstd) {
+  const float inverse = 1.f / (top * (1.f / kE4m3Max));
+  return Quotient{top * rstd * (1.f / kE4m3Max), inverse, __fmaf_rn(-inverse, top, kE4m3Max) * (inverse * (1.f / kE4m3Max))};
+}
+// Not for sizes far from 1, rows of zeros and rows without a norm.  (What is below 2^-126 beside a largest |p| of 2^-90 is 0 in e4m3.)
+__device__ __forceinline__ bool is_near(float top, float rstd) { return top >= 0x1p-90f && top <= 3.4e38f && top * rstd >= 0x1p-100f; }
+
+// The same for every size, from p = (z 2^k) w with s = 2^k rest, 1/2 <= rest < 1 (p is not flushed before y is): y / scale = p rest / scale,
+// within 2^-21.
 struct Parts {
   float power, rest;
 };
@@ -62,24 +77,10 @@ __device__ __forceinline__ Parts parts_of(float rstd) {
   const uint32_t bits = __float_as_uint(rstd);  // normal: eps is
   return Parts{__uint_as_float((bits & 0x7f800000u) + 0x00800000u), __uint_as_float((bits & 0x007fffffu) | 0x3f000000u)};
 }
-
-// The scale of a group whose largest |p| is `top`, and what takes p to its quotient: 448 / top as the sum of an approximation and of what a
-// fused product shows it to lack, good to 2^-44.  A quotient that fp32 holds, as every tie is, then comes out exactly, every other
-// within 2^-24 of it.  Where the second part could over- or underflow, far from 1, it is left out: 2^-21.  (1024 x 1024 rows of 256 take
-// 338 us, 326 with a product by an approximate 1 / scale, which misses ties, and 365 with divisions.)
-struct Quotient {
-  float scale, factor, lack;
-  __device__ __forceinline__ float2 operator()(float2 p) const { return __ffma2_rn(p, both(factor), __fmul2_rn(p, both(lack))); }
-};
-__device__ __forceinline__ Quotient quotient_of(float top, float rest) {
-  Quotient q;
+__device__ __forceinline__ Quotient quotient_far(float top, float rest) {
   const float most = top * rest;
-  q.scale = most > 0.f ? fmaxf(most * (1.f / kE4m3Max), 1.17549435e-38f) : 1.f;
-  const bool near = top >= 0x1p-90f && top <= 0x1p120f;  // what is below 2^-126 here is 0 in e4m3
-  const float inverse = 1.f / (near ? top * (1.f / kE4m3Max) : q.scale);
-  q.factor = near ? inverse : inverse * rest;
-  q.lack = near ? __fmaf_rn(-inverse, top, kE4m3Max) * (inverse * (1.f / kE4m3Max)) : 0.f;
-  return q;
+  const float scale = most > 0.f ? fmaxf(most * (1.f / kE4m3Max), 1.17549435e-38f) : 1.f;
+  return Quotient{scale, 1.f / scale * rest, 0.f};
 }
 
 // round(r + dropout(u)) of one oct.
@@ -222,11 +223,13 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
     }
     group_sum<kGroup, 1>(ss, sums, parity);
     const float rstd = rsqrtf(ss[0] * a.inv_d + a.eps);
-    const Parts parts = kMode == kNormE4m3 ? parts_of(rstd) : Parts{rstd, 1.f};
+    const auto gain = [&](float by) {
 #pragma unroll
-    for (int n = 0; n < kPairs; ++n) v.p[n] = __fmul2_rn(__fmul2_rn(v.p[n], both(parts.power)), w.p[n]);
+      for (int n = 0; n < kPairs; ++n) v.p[n] = __fmul2_rn(__fmul2_rn(v.p[n], both(by)), w.p[n]);
+    };
 
     if constexpr (kMode == kNorm) {
+      gain(rstd);
       T* yp = static_cast<T*>(a.y) + out;
       pack_all<T, kU, kUnits>(v, u);
 #pragma unroll
@@ -235,31 +238,53 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
     } else if constexpr (kMode == kNormE4m3) {
       const bool whole = a.scale_shift < 0;  // the only form of narrow units
       float top[kUnits];
+      const auto find_top = [&] {
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        top[k] = 0.f;
+        for (int k = 0; k < kUnits; ++k) {
+          top[k] = 0.f;
 #pragma unroll
-        for (int e = 0; e < kU; ++e) {
-          const float2 x = v.p[(k * kU + e) / 2];
-          top[k] = fmaxf(top[k], fabsf((k * kU + e) & 1 ? x.y : x.x));
-        }
-        if constexpr (!kClear) top[k] = valid && lane + k * kGroup < units ? top[k] : 0.f;
-      }
-      if (whole) {
-        float m[1] = {top[0]};
-#pragma unroll
-        for (int k = 1; k < kUnits; ++k) m[0] = fmaxf(m[0], top[k]);
-        group_max<kGroup, 1>(m, tops, parity);
-#pragma unroll
-        for (int k = 0; k < kUnits; ++k) top[k] = m[0];
-      } else {
-        // 32, 64 or 128 channels are 4, 8 or 16 neighbouring lanes
-#pragma unroll
-        for (int o = 0; o < 4; ++o)
-          if (o < a.scale_shift) {
-#pragma unroll
-            for (int k = 0; k < kUnits; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1 << o));
+          for (int e = 0; e < kU; ++e) {
+            const float2 x = v.p[(k * kU + e) / 2];
+            top[k] = fmaxf(top[k], fabsf((k * kU + e) & 1 ? x.y : x.x));
           }
+          if constexpr (!kClear) top[k] = valid && lane + k * kGroup < units ? top[k] : 0.f;
+        }
+        if (whole) {
+          float m[1] = {top[0]};
+#pragma unroll
+          for (int k = 1; k < kUnits; ++k) m[0] = fmaxf(m[0], top[k]);
+          group_max<kGroup, 1>(m, tops, parity);
+#pragma unroll
+          for (int k = 0; k < kUnits; ++k) top[k] = m[0];
+        } else {
+          // 32, 64 or 128 channels are 4, 8 or 16 neighbouring lanes
+#pragma unroll
+          for (int o = 0; o < 4; ++o)
+            if (o < a.scale_shift) {
+#pragma unroll
+              for (int k = 0; k < kUnits; ++k) top[k] = fmaxf(top[k], __shfl_xor_sync(0xffffffffu, top[k], 1 << o));
+            }
+        }
+      };
+      // One oct a lane: p = z w, and the long way, a warp or all that share one scale together, where that will not do.  More channels a
+      // lane have no registers for both ways and take the long one (96 x 768 rows of 384: 38.7 us, with both 40.9).
+      bool far = true;
+      if constexpr (kU == 8 && kUnits == 1) {
+#pragma unroll
+        for (int n = 0; n < kPairs; ++n) v.p[n] = __fmul2_rn(v.p[n], w.p[n]);
+        find_top();
+        far = __any_sync(0xffffffffu, !is_near(top[0], rstd) && (whole || lane < units));
+        if (far) {
+          v = unpack_all<T, kU, kUnits>(u);
+          if (kGroup > 32 && whole) __syncthreads();  // the first maxima have been read
+        }
+      }
+      float rest = rstd;
+      if (far) {
+        const Parts parts = parts_of(rstd);
+        rest = parts.rest;
+        gain(parts.power);
+        find_top();
       }
       if (!valid) continue;
       uint8_t* yp = static_cast<uint8_t*>(a.y) + out;
@@ -268,7 +293,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
       for (int k = 0; k < kUnits; ++k) {
         const int n = lane + k * kGroup;
         if (n >= units) continue;
-        const Quotient by = quotient_of(top[k], parts.rest);
+        const Quotient by = !far || is_near(top[k], rest) ? quotient_near(top[k], rest) : quotient_far(top[k], rest);
         if (whole ? n == 0 : (n & ((1 << a.scale_shift) - 1)) == 0) sp[whole ? 0 : n >> a.scale_shift] = by.scale;
         if constexpr (kU == 8) {
           uint32_t q[4];

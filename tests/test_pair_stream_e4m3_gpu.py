@@ -47,6 +47,33 @@ def test_e4m3_of_bf16_rows_is_that_of_the_exact_quotient(shape):
     assert ties > 0 or u.numel() < 100000
 
 
+@pytest.mark.parametrize("d", [64, 96, 128, 256, 384, 1024, 4096, 67, 130])
+def test_neighbours_of_rows_without_a_norm(d):
+    """Rows of zeros, of tiny values and with a NaN or an infinity change nothing in the rows beside them."""
+    p = P()
+    g = torch.Generator(device=DEV).manual_seed(d)
+    z = torch.randn((1, 12, 97, d), generator=g, device=DEV).bfloat16()
+    w = (1 + 0.1 * torch.randn(d, generator=g, device=DEV)).bfloat16()
+    kind = torch.randint(0, 12, z.shape[:3], generator=g, device=DEV)
+    z[kind == 0] = 0
+    z[kind == 1] *= 2.0 ** -100
+    z[..., 5][kind == 2] = float("nan")
+    z[..., 7][kind == 3] = float("inf")
+    for group in (None, 32, 64, 128):
+        if group is not None and d % group:
+            continue
+        q, scales, _ = p.add_rms_norm_fp8(z, None, w, group=group)
+        t, _ = quotients(z, w, group or d)
+        plain = kind >= 4
+        assert torch.equal(q[plain].float(), t.float().to(torch.float8_e4m3fn).float()[plain]), group
+        assert (q[kind == 0].float() == 0).all() and (scales[kind == 0] == 1).all() and q[kind == 2].float().isnan().all() and (scales[kind == 2] == 1).all()
+        bad = q[kind == 3].float()
+        assert bad[:, 7].isnan().all() and (bad[:, :7] == 0).all() and (bad[:, 8:] == 0).all()
+        # tiny rows: half a step of e4m3 and 2^-21 of the quotient
+        tiny, got = t[kind == 1], q[kind == 1].float().double()
+        assert ((got - tiny).abs() <= torch.maximum(2.0 ** -4 * tiny.abs(), torch.full_like(tiny, 2.0 ** -10)) * (1 + 2.0 ** -16)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("size", [1e-24, 1e-12, 1.0, 1e12])
 def test_e4m3_of_gains_of_every_size(size, dtype):
