@@ -24,7 +24,7 @@ namespace pair {
 // type, 32 of fp32).  All others are moved in units of two 16-bit channels where rows start on 4-byte boundaries, of four fp32 where the
 // addition alone finds 16-byte ones, else of one channel: a warp's accesses are then still contiguous, where groups of eight at odd
 // addresses would make each access of a warp touch every line of the row.  Such rows are bound by the instructions that move them:
-// the norm of 80000 fp16 rows takes 11 us at 128 channels, 23 at 130 and at 131; of fp32 rows 30 and 39.
+// the norm of 80000 fp16 rows with a residual takes 11 us at 128 channels, 22 at 130 and at 131 (alone 9, 19 and 18); of fp32 rows 28 and 36.
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
 template <>
@@ -105,7 +105,7 @@ __device__ __forceinline__ void stage_wait() { asm volatile("cp.async.wait_group
 
 // Which rows travel that way: not octs of fp32, whose two 16-byte halves would each touch every sector of the row, where direct loads
 // find the second half in L1 (131072 rows of 256 channels: 95 against 126 us), nor 2-byte units, which cp.async does not know
-// (copying the 4-byte words under them takes more instructions than the loads do: 80000 rows of 131 channels 26 against 17 us).
+// (copying the 4-byte words under them takes more instructions than the loads do: 80000 rows of 131 channels without a residual 26 against 17 us).
 template <typename T, int kU, int kGroup, int kUnits>
 struct Rows {
   static constexpr int kWide = kGroup <= 32 ? 256 : kGroup;  // threads of the CTA

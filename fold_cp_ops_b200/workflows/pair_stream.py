@@ -17,7 +17,7 @@ context-parallel grid draw the same mask as one GPU would.
 
 Tensors may be DTensors sharded over batch and token dims, as the distributed triangle update takes them: the blocks'
 positions are then taken from the placements, and gains and tables may be replicated DTensors.  Gradients are for plain
-tensors only.  Inputs need contiguous channels
+tensors only; those of gains and tables are of the block that was passed, to be added up over ranks.  Inputs need contiguous channels
 (others are copied); other strides -- a transposed view, a block of a larger tensor, a broadcast axis -- are read in place.
 There is no CPU path.
 """
