@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import re
 import threading
 from pathlib import Path
 
@@ -214,12 +215,19 @@ def pair_host():
     with _lock:
         if _pair is not None:
             return _pair
+        import torch  # the host module links to its libraries
+
         try:
             from . import _pair_host as host
         except ImportError as exc:
             raise TrimulLibraryError(
                 f"cannot load the host module {_PKG_DIR / '_pair_host.so'}: {exc}. Build it with "
                 "`python -m fold_cp_ops_b200.build`.") from exc
+        # the header's version has no suffix: 2.11.0 of 2.11.0a0+git...
+        if not re.match(re.escape(host.torch_version) + r"(?!\d)", torch.__version__):
+            raise TrimulLibraryError(
+                f"{host.__file__} was built against torch {host.torch_version}, this is torch {torch.__version__}; rebuild it with "
+                "`python -m fold_cp_ops_b200.build`.")
         from .build import source_digest
 
         if host.build_id() != source_digest():

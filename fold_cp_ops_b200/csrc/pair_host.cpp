@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
+#include <torch/version.h>
 
 #include <cmath>
 #include <cstring>
@@ -532,6 +533,7 @@ PYBIND11_MODULE(_pair_host, m) {
   });
   m.def("bind", &bind);
   m.def("build_id", &build_id);
+  m.attr("torch_version") = TORCH_VERSION;  // the headers that this was compiled against
   m.def("dropout_add", &dropout_add);
   m.def("add_rms_norm", &add_rms_norm);
   m.def("add_rms_norm_fp8", &add_rms_norm_fp8);
