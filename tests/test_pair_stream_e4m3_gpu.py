@@ -96,3 +96,21 @@ def test_e4m3_of_gains_of_every_size(size, dtype):
         # values below 2^-126 are flushed: 2^-126 over a scale of at least 2^-126 is 1
         flushed = 2.0 ** -126 / scales.double()[..., None]
         assert (err <= torch.maximum(2.0 ** -4 * t.abs(), torch.full_like(t, 2.0 ** -10)) * (1 + 2.0 ** -18) + flushed).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [32, 64, 96, 128, 384, 512, 1024, 8192, 67, 130, 1031])
+def test_e4m3_of_whole_numbers(d, dtype):
+    """z and w of few bits, in every type: products below 2^10, so that quotients are ties or at least 2^-15 away from one (a tie has
+    five bits), and one in some 30 is a tie."""
+    p = P()
+    g = torch.Generator(device=DEV).manual_seed(d)
+    z = (torch.randint(-40, 41, (1, 5, 41, d), generator=g, device=DEV) / 8).to(dtype)
+    w = (torch.randint(1, 21, (d,), generator=g, device=DEV) / 16).to(dtype)
+    for group in (None, 32, 64, 128):
+        if group is not None and d % group:
+            continue
+        q, _, _ = p.add_rms_norm_fp8(z, None, w, group=group)
+        t, tie = quotients(z, w, group or d)
+        assert tie.sum() > q.numel() / 1000
+        assert torch.equal(q.float(), t.float().to(torch.float8_e4m3fn).float()), group
