@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
       for (int k = 0; k < kUnits; ++k)
         if (valid && lane + k * kGroup < units) store_unit<T, kU>(yp + k * kGroup * kU, u[k]);
     } else if constexpr (kMode == kNormE4m3) {
-      const bool whole = a.scale_shift < 0;  // the only form of narrow units
+      const bool whole = kU < 8 || a.scale_shift < 0;  // the only form of narrow units
       float top[kUnits];
       const auto find_top = [&] {
 #pragma unroll
@@ -289,21 +289,32 @@ __global__ void __launch_bounds__(threads_of(kGroup), (kUnits * kU > 16 ? 768 : 
       if (!valid) continue;
       uint8_t* yp = static_cast<uint8_t*>(a.y) + out;
       float* sp = a.scales + scale_row;
+      if constexpr (kU == 8) {
 #pragma unroll
-      for (int k = 0; k < kUnits; ++k) {
-        const int n = lane + k * kGroup;
-        if (n >= units) continue;
-        const Quotient by = !far || is_near(top[k], rest) ? quotient_near(top[k], rest) : quotient_far(top[k], rest);
-        if (whole ? n == 0 : (n & ((1 << a.scale_shift) - 1)) == 0) sp[whole ? 0 : n >> a.scale_shift] = by.scale;
-        if constexpr (kU == 8) {
+        for (int k = 0; k < kUnits; ++k) {
+          const int n = lane + k * kGroup;
+          if (n >= units) continue;
+          const Quotient by = !far || is_near(top[k], rest) ? quotient_near(top[k], rest) : quotient_far(top[k], rest);
+          if (whole ? n == 0 : (n & ((1 << a.scale_shift) - 1)) == 0) sp[whole ? 0 : n >> a.scale_shift] = by.scale;
           uint32_t q[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) q[e] = e4m3x2(by(v.p[4 * k + e]));
           __stcs(reinterpret_cast<uint2*>(yp + k * kGroup * 8), make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16)));
-        } else if constexpr (kU == 2) {
-          *reinterpret_cast<uint16_t*>(yp + k * kGroup * 2) = static_cast<uint16_t>(e4m3x2(by(v.p[k])));
-        } else {
-          yp[k * kGroup] = static_cast<uint8_t>(e4m3x2(by(both(k & 1 ? v.p[k / 2].y : v.p[k / 2].x))));
+        }
+      } else {
+        const Quotient by = is_near(top[0], rest) ? quotient_near(top[0], rest) : quotient_far(top[0], rest);
+        if (lane == 0) sp[0] = by.scale;
+#pragma unroll
+        for (int m = 0; m < kPairs; ++m) {
+          const uint32_t q = e4m3x2(by(v.p[m]));  // a unit of two channels, or two units
+          constexpr int kStep = 2 / kU;
+          const int n = lane + m * kStep * kGroup;
+          if constexpr (kU == 2) {
+            if (n < units) *reinterpret_cast<uint16_t*>(yp + m * kGroup * 2) = static_cast<uint16_t>(q);
+          } else {
+            if (n < units) yp[2 * m * kGroup] = static_cast<uint8_t>(q);
+            if (n + kGroup < units) yp[(2 * m + 1) * kGroup] = static_cast<uint8_t>(q >> 8);
+          }
         }
       }
     }
