@@ -471,6 +471,7 @@ __device__ __forceinline__ void drop_all(const Dropout& d, uint32_t line, uint32
     for (int n = 0; n < v.kPairs; ++n) {
       const uint32_t x = narrow_bits<kU, kUnits>(mask, 2 * n / kU) >> (2 * n % kU);
       const uint32_t y = kU > 1 ? x >> 1 : narrow_bits<kU, kUnits>(mask, 2 * n + 1);
+      // one by one: packed, the compiler joins this product and the residual's addition, and rows on other boundaries would round otherwise
       v.p[n].x = x & 1u ? mul_whole(v.p[n].x, d.gain) : 0.f;
       v.p[n].y = y & 1u ? mul_whole(v.p[n].y, d.gain) : 0.f;
     }

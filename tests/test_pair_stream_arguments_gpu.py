@@ -52,3 +52,22 @@ def test_the_addition_keeps_subnormals(d, dtype):
     table, index = u[0, :, 0].contiguous(), torch.tensor([2, -1, 0, 1, 2], device=DEV)
     want = torch.where((index >= 0)[:, None], table.double()[index.clamp(min=0)], 0.0) * 2 + r[0, 0].double()
     assert torch.equal(p.pair_embedding(index, table, scale=2.0, base=r[0, 0]), want.to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128, 384, 512, 1024, 8192, 66, 130, 131, 132, 1031, 4099])
+def test_the_stream_has_the_same_bits_in_every_form(d, dtype):
+    """fp32 product, fp32 sum, one rounding to the type: whatever the width and the boundaries (every rank of a grid has to store what one
+    GPU would), in the addition and in each norm."""
+    p = P()
+    drop = p.PairDropout(0.25, seed=3)
+    gain = torch.tensor(65536 / 49152, dtype=torch.float32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(d)
+    flat = [torch.randn(3 * 7 * d + 1, generator=g, device=DEV).to(dtype) for _ in range(2)]
+    w = torch.ones(d, device=DEV)
+    for first in (0, 1):
+        u, r = (t[first:first + 3 * 7 * d].view(1, 3, 7, d) for t in flat)
+        kept = p.dropout_add(torch.ones_like(u), None, drop) != 0
+        want = (torch.where(kept, u.float() * gain, 0.0) + r.float()).to(dtype)
+        for z in (p.dropout_add(u, r, drop), p.add_rms_norm(u, r, w, dropout=drop)[1], p.add_rms_norm_fp8(u, r, w, group=None, dropout=drop)[2]):
+            assert torch.equal(z, want)
